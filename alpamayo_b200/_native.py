@@ -41,6 +41,13 @@ def load_ops() -> None:
     _ops_loaded = True
 
 
+class Kv8Cache(ctypes.Structure):
+    """paro_kv8_cache of include/paro_b200.h."""
+    _fields_ = [("k_codes", ctypes.c_void_p), ("v_codes", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("num_pages", ctypes.c_int64), ("kv_heads", ctypes.c_int),
+                ("page_size", ctypes.c_int), ("head_dim", ctypes.c_int)]
+
+
 def capi() -> ctypes.CDLL:
     """The C ABI as a ctypes library with argument types declared."""
     global _capi
@@ -86,6 +93,14 @@ def capi() -> ctypes.CDLL:
         "paro_w4a8_gemm_multicast": (i32, [vp, vp, i64, i32, i32, vp, vp, i32, vp, vp]),
         "paro_add_rmsnorm": (i32, [vp, vp, vp, i64, i32, ctypes.c_float, vp, vp]),
         "paro_silu_mul": (i32, [vp, i64, i32, vp, vp]),
+        "paro_attention_prefill": (i32, [vp, vp, vp, i32, vp, vp, vp, i32, i64, i64, i32, i32, i32, ctypes.c_float,
+                                         vp, vp]),
+        "paro_kv8_append": (i32, [vp, vp, i32, vp, vp, i32, vp, vp, vp, i32, i64, vp]),
+        "paro_kv8_gather": (i32, [vp, vp, i32, vp, vp, i32, i64, vp, vp, i32, vp]),
+        "paro_attention_kv8_workspace_size": (sz, [vp, i32, i32, i32, i32, i32]),
+        "paro_attention_kv8": (i32, [vp, vp, i32, vp, i32, vp, i32, i32, i32, vp, ctypes.c_float, vp, vp, i64, vp,
+                                     vp, sz, vp]),
+        "paro_kv8_evict": (i32, [vp, vp, i32, vp, i64, vp, i32, i32, i32, i32, vp, vp, vp, vp, i32, vp]),
     }
     for name, (res, args) in sigs.items():
         f = getattr(L, name)

@@ -25,8 +25,10 @@ OBJ = os.path.join(PKG, "_build")
 CUDA_HOME = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 NVCC = os.path.join(CUDA_HOME, "bin", "nvcc")
 
-CU_SOURCES = ["capi.cu", "rotq.cu", "rotq_fused.cu", "rotq_rows.cu", "rotq_decode.cu", "rotq_tc.cu", "prepare.cu", "gemm_decode.cu", "gemm_rows.cu", "gemm_tc.cu", "elementwise.cu"]
-HEADERS = ["paro_common.cuh", "tc_ptx.cuh", "umma.cuh", "stream_segs.cuh"]
+CU_SOURCES = ["capi.cu", "rotq.cu", "rotq_fused.cu", "rotq_rows.cu", "rotq_decode.cu", "rotq_tc.cu", "prepare.cu", "gemm_decode.cu", "gemm_rows.cu", "gemm_tc.cu", "elementwise.cu",
+              "attn_prefill.cu", "kv8_cache.cu", "kv8_attn.cu"]
+HEADERS = ["paro_common.cuh", "tc_ptx.cuh", "umma.cuh", "stream_segs.cuh", "kv8.cuh"]
+SHIM_SOURCES = ["torch_ops.cpp", "torch_attention.cpp"]
 GENCODE = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
               "-Xptxas", "-warn-spills"] + GENCODE
@@ -66,19 +68,26 @@ def build(force: bool = False, verbose: bool = False) -> dict:
         logs.append(_run([NVCC, "-shared"] + GENCODE + ["-cudart", "static", "-o", core] + objs))
 
     shim = os.path.join(LIB, "libparo_torch.so")
-    shim_src = os.path.join(HERE, "torch_ops.cpp")
-    if force or _newer([shim_src, core] + hdrs, shim):
+    shim_srcs = [os.path.join(HERE, f) for f in SHIM_SOURCES]
+    if force or _newer(shim_srcs + [core] + hdrs, shim):
         import torch
         from torch.utils import cpp_extension as ce
         inc = ce.include_paths() + [os.path.join(CUDA_HOME, "include")]
         tlib = os.path.join(os.path.dirname(torch.__file__), "lib")
         abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-        cmd = (["g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-                "-DTORCH_API_INCLUDE_EXTENSION_H=0"]
-               + [f"-I{p}" for p in inc]
-               + [shim_src, "-o", shim, f"-L{tlib}", f"-L{LIB}", "-lparo_b200", "-lc10", "-lc10_cuda",
-                  "-ltorch", "-ltorch_cpu", "-ltorch_cuda", f"-Wl,-rpath,{tlib}", "-Wl,-rpath,$ORIGIN"])
-        logs.append(_run(cmd))
+        cxx = ["g++", "-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+               "-DTORCH_API_INCLUDE_EXTENSION_H=0"]
+        shim_objs, jobs = [], []
+        for src in shim_srcs:
+            o = os.path.join(OBJ, os.path.basename(src).replace(".cpp", ".cpp.o"))
+            shim_objs.append(o)
+            if force or _newer([src] + hdrs, o):
+                jobs.append(cxx + [f"-I{p}" for p in inc] + ["-c", src, "-o", o])
+        with cf.ThreadPoolExecutor(max_workers=max(1, len(jobs))) as ex:
+            logs += list(ex.map(_run, jobs))
+        logs.append(_run(cxx + ["-shared", "-o", shim] + shim_objs
+                         + [f"-L{tlib}", f"-L{LIB}", "-lparo_b200", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
+                            "-ltorch_cuda", f"-Wl,-rpath,{tlib}", "-Wl,-rpath,$ORIGIN"]))
     if verbose:
         print("\n".join(l for l in logs if l.strip()))
     return {"core": core, "shim": shim}

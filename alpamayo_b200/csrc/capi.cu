@@ -9,7 +9,7 @@
 #include <cstring>
 #include <string>
 
-#include "tc_ptx.cuh"
+#include "kv8.cuh"
 
 namespace paro {
 cudaError_t launch_rotate(int x_dtype, int krot, int group, const void* x, int64_t M, int K, const void* scales,
@@ -64,6 +64,21 @@ cudaError_t launch_gemm_tc_sets(const int8_t* xq, const float* xscale, int64_t M
                                 const void* bias, int bias_dtype, void* out, int out_dtype, void* workspace,
                                 size_t workspace_bytes, int T, const int* tab_nb, cudaStream_t st);
 int gemm_tc_sets_ok(int T, const int* tab_nb);
+cudaError_t launch_attn_prefill(const void* q, const void* k, const void* v, int dtype, const int64_t* strides,
+                                const int32_t* cu_q, const int32_t* cu_k, int B, int64_t rows, int64_t k_rows,
+                                int heads, int kv_heads, int dim, float scale, void* out, cudaStream_t st);
+cudaError_t launch_kv8_append(const Kv8View& c, const void* k, const void* v, int dtype, const int64_t* strides,
+                              const int32_t* cu, const int32_t* starts, int B, int64_t rows, cudaStream_t st);
+cudaError_t launch_kv8_gather(const Kv8View& c, const int32_t* starts, const int32_t* cu, int B, int64_t rows, void* k,
+                              void* v, int dtype, cudaStream_t st);
+cudaError_t launch_kv8_evict(const Kv8View& c, const float* weights, int64_t cap, const int32_t* lens, int B,
+                             int budget, int sink, int recent, int32_t* kept, float* new_weights, int32_t* new_lens,
+                             const int32_t* out_table, int out_width, cudaStream_t st);
+int kv8_attn_max_rows();
+size_t kv8_attn_workspace(const Kv8View& c, int B, int T, int heads, int with_weights);
+cudaError_t launch_kv8_attn(const Kv8View& c, const void* q, int dtype, const int64_t* strides, int B, int T, int heads,
+                            const int32_t* lens, float scale, const float* weights, float* weights_out, int64_t cap,
+                            void* out, void* workspace, cudaStream_t st);
 }  // namespace paro
 
 #include <map>
@@ -74,6 +89,8 @@ uint32_t error_word_decode(int clear);
 uint32_t error_word_tc(int clear);
 uint32_t error_word_rtc(int clear);
 uint32_t error_word_rows(int clear);
+uint32_t error_word_kv8(int clear);
+uint32_t error_word_kv8a(int clear);
 
 cudaError_t ensure_smem_limit(const void* kernel, int bytes) {
   static std::mutex mu;
@@ -111,6 +128,33 @@ int device_check() {
   int major = 0;
   if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess) return PARO_ERR_DEVICE;
   return major == 10 ? PARO_OK : PARO_ERR_DEVICE;
+}
+}  // namespace
+
+namespace {
+int64_t c_page(const Kv8View& c) { return (int64_t)1 << c.page_shift; }
+
+// The cache and its page table as the kernels take them, or a status.
+int kv8_view(const paro_kv8_cache* cache, const int32_t* table, int table_width, int B, Kv8View* out) {
+  if (!cache || !table || B < 0 || table_width <= 0) return PARO_ERR_INVALID_ARGUMENT;
+  if (!cache->k_codes || !cache->v_codes || !cache->k_scale || !cache->v_scale || cache->num_pages <= 0 ||
+      cache->kv_heads <= 0)
+    return PARO_ERR_INVALID_ARGUMENT;
+  if (cache->page_size != 16 && cache->page_size != 32 && cache->page_size != 64 && cache->page_size != 128)
+    return PARO_ERR_SHAPE;
+  if (cache->head_dim != 64 && cache->head_dim != 128) return PARO_ERR_SHAPE;
+  // grid dimensions: kv_heads in y, 2 B in z; lengths are 32-bit
+  if (cache->kv_heads > 1024 || B > 32767 || cache->num_pages > 0x7FFFFFFF ||
+      (int64_t)table_width * cache->page_size > 0x7FFFFFFF)
+    return PARO_ERR_TOO_LARGE;
+  if (!aligned(cache->k_codes, 16) || !aligned(cache->v_codes, 16) || !aligned(cache->k_scale, 4) ||
+      !aligned(cache->v_scale, 4) || !aligned(table, 4))
+    return PARO_ERR_MISALIGNED;
+  int shift = 4;
+  while ((1 << shift) < cache->page_size) ++shift;
+  *out = Kv8View{cache->k_codes, cache->v_codes, cache->k_scale, cache->v_scale, cache->num_pages, table, table_width,
+                 cache->kv_heads, shift, cache->head_dim};
+  return PARO_OK;
 }
 }  // namespace
 
@@ -596,10 +640,14 @@ int paro_silu_mul(const void* x, int64_t M, int I, void* out, paro_stream_t stre
 }
 
 int paro_device_error_word(int clear) {
-  const uint32_t a = error_word_decode(clear), b = error_word_tc(clear), c = error_word_rtc(clear),
-                 d = error_word_rows(clear);
-  if (a == ~0u || b == ~0u || c == ~0u || d == ~0u) return -1;
-  return (int)(a | b | c | d);
+  const uint32_t words[] = {error_word_decode(clear), error_word_tc(clear),  error_word_rtc(clear),
+                            error_word_rows(clear),   error_word_kv8(clear), error_word_kv8a(clear)};
+  uint32_t all = 0;
+  for (const uint32_t w : words) {
+    if (w == ~0u) return -1;
+    all |= w;
+  }
+  return (int)all;
 }
 
 int paro_selftest_wait_timeout(long long limit_cycles, paro_stream_t stream) {
@@ -767,6 +815,106 @@ int paro_w4a8_gemm_noalloc(const int8_t* xq, const float* xscale, int64_t M, int
   if (e != cudaSuccess) return cuda_status(e);
   return cuda_status(launch_gemm_decode(xq, xscale, M, N, K, packed, bias, bias_dtype, out, out_dtype, scratch,
                                         (cudaStream_t)stream));
+}
+
+// ---- attention and the int8 key/value cache ---------------------------------
+
+size_t paro_attention_kv8_workspace_size(const paro_kv8_cache* cache, int table_width, int B, int T, int heads,
+                                         int with_weights) {
+  Kv8View c;
+  if (kv8_view(cache, reinterpret_cast<const int32_t*>(16), table_width, B, &c) || B <= 0 || T <= 0 || heads <= 0 ||
+      heads % c.kv_heads || (int64_t)T * (heads / c.kv_heads) > kv8_attn_max_rows())
+    return 0;
+  return kv8_attn_workspace(c, B, T, heads, with_weights);
+}
+
+int paro_attention_prefill(const void* q, const void* k, const void* v, int dtype, const int64_t* strides,
+                           const int32_t* cu_q, const int32_t* cu_k, int B, int64_t rows, int64_t k_rows, int heads,
+                           int kv_heads, int head_dim, float scale, void* out, paro_stream_t stream) {
+  if (rows < 0 || k_rows < 0 || B < 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return PARO_ERR_INVALID_ARGUMENT;
+  if (dtype != PARO_BF16 && dtype != PARO_F16) return PARO_ERR_UNSUPPORTED;
+  if (heads % kv_heads || (head_dim != 64 && head_dim != 128)) return PARO_ERR_SHAPE;
+  if (rows > 0x7FFFFFFF || k_rows > 0x7FFFFFFF || heads > 65535) return PARO_ERR_TOO_LARGE;
+  if (rows == 0) return PARO_OK;
+  if (!q || !out || !strides || !cu_q || !cu_k || (k_rows > 0 && (!k || !v))) return PARO_ERR_INVALID_ARGUMENT;
+  if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16) || !aligned(cu_q, 4) ||
+      !aligned(cu_k, 4))
+    return PARO_ERR_MISALIGNED;
+  for (int i = 0; i < 6; ++i)
+    if (strides[i] < 0 || strides[i] % 8) return PARO_ERR_MISALIGNED;
+  if (int d = device_check()) return d;
+  return cuda_status(launch_attn_prefill(q, k, v, dtype, strides, cu_q, cu_k, B, rows, k_rows, heads, kv_heads,
+                                         head_dim, scale, out, (cudaStream_t)stream));
+}
+
+int paro_kv8_append(const paro_kv8_cache* cache, const int32_t* page_table, int table_width, const void* k,
+                    const void* v, int dtype, const int64_t* strides, const int32_t* cu, const int32_t* starts, int B,
+                    int64_t rows, paro_stream_t stream) {
+  Kv8View c;
+  if (rows < 0) return PARO_ERR_INVALID_ARGUMENT;
+  if (!valid_dtype(dtype)) return PARO_ERR_UNSUPPORTED;
+  if (int rc = kv8_view(cache, page_table, table_width, B, &c)) return rc;
+  if (rows == 0 || B == 0) return PARO_OK;
+  if (!k || !v || !strides || !cu || !starts) return PARO_ERR_INVALID_ARGUMENT;
+  if (rows > 0x7FFFFFFF) return PARO_ERR_TOO_LARGE;
+  if (!aligned(k, 16) || !aligned(v, 16)) return PARO_ERR_MISALIGNED;
+  for (int i = 0; i < 4; ++i)
+    if (strides[i] < 0 || strides[i] % (16 / (int64_t)elem_bytes(dtype))) return PARO_ERR_MISALIGNED;
+  if (int d = device_check()) return d;
+  return cuda_status(launch_kv8_append(c, k, v, dtype, strides, cu, starts, B, rows, (cudaStream_t)stream));
+}
+
+int paro_kv8_gather(const paro_kv8_cache* cache, const int32_t* page_table, int table_width, const int32_t* starts,
+                    const int32_t* cu, int B, int64_t rows, void* out_k, void* out_v, int dtype,
+                    paro_stream_t stream) {
+  Kv8View c;
+  if (rows < 0) return PARO_ERR_INVALID_ARGUMENT;
+  if (!valid_dtype(dtype)) return PARO_ERR_UNSUPPORTED;
+  if (int rc = kv8_view(cache, page_table, table_width, B, &c)) return rc;
+  if (rows == 0) return PARO_OK;
+  if (!out_k || !out_v || !cu || !starts) return PARO_ERR_INVALID_ARGUMENT;
+  if (rows > 0x7FFFFFFF) return PARO_ERR_TOO_LARGE;
+  if (!aligned(out_k, 16) || !aligned(out_v, 16)) return PARO_ERR_MISALIGNED;
+  if (int d = device_check()) return d;
+  return cuda_status(launch_kv8_gather(c, starts, cu, B, rows, out_k, out_v, dtype, (cudaStream_t)stream));
+}
+
+int paro_attention_kv8(const paro_kv8_cache* cache, const int32_t* page_table, int table_width, const void* q,
+                       int dtype, const int64_t* strides, int B, int T, int heads, const int32_t* lens, float scale,
+                       const float* weights, float* weights_out, int64_t cap, void* out, void* workspace,
+                       size_t workspace_bytes, paro_stream_t stream) {
+  Kv8View c;
+  if (T < 0 || heads <= 0) return PARO_ERR_INVALID_ARGUMENT;
+  if (dtype != PARO_BF16 && dtype != PARO_F16) return PARO_ERR_UNSUPPORTED;
+  if (int rc = kv8_view(cache, page_table, table_width, B, &c)) return rc;
+  if (heads % c.kv_heads) return PARO_ERR_SHAPE;
+  if (B == 0 || T == 0) return PARO_OK;
+  if ((int64_t)T * (heads / c.kv_heads) > kv8_attn_max_rows()) return PARO_ERR_TOO_LARGE;
+  if (!q || !strides || !lens || !out || !workspace || !weights != !weights_out) return PARO_ERR_INVALID_ARGUMENT;
+  if (weights && cap < (int64_t)table_width * c_page(c)) return PARO_ERR_SHAPE;
+  if (!aligned(q, 16) || !aligned(out, 16) || !aligned(workspace, 256)) return PARO_ERR_MISALIGNED;
+  for (int i = 0; i < 3; ++i)
+    if (strides[i] < 0 || strides[i] % 8) return PARO_ERR_MISALIGNED;
+  if (workspace_bytes < kv8_attn_workspace(c, B, T, heads, weights != nullptr)) return PARO_ERR_WORKSPACE;
+  if (int d = device_check()) return d;
+  return cuda_status(launch_kv8_attn(c, q, dtype, strides, B, T, heads, lens, scale, weights, weights_out, cap, out,
+                                     workspace, (cudaStream_t)stream));
+}
+
+int paro_kv8_evict(const paro_kv8_cache* cache, const int32_t* page_table, int table_width, const float* weights,
+                   int64_t cap, const int32_t* lens, int B, int budget, int sink, int recent, int32_t* kept,
+                   float* new_weights, int32_t* new_lens, const int32_t* out_table, int out_width,
+                   paro_stream_t stream) {
+  Kv8View c;
+  if (int rc = kv8_view(cache, page_table, table_width, B, &c)) return rc;
+  if (budget <= 0 || sink < 0 || recent < 0 || (int64_t)sink + recent > budget || out_width <= 0)
+    return PARO_ERR_INVALID_ARGUMENT;
+  if ((int64_t)out_width * c_page(c) < budget || cap < (int64_t)table_width * c_page(c)) return PARO_ERR_SHAPE;
+  if (B == 0) return PARO_OK;
+  if (!weights || !lens || !kept || !new_weights || !new_lens || !out_table) return PARO_ERR_INVALID_ARGUMENT;
+  if (int d = device_check()) return d;
+  return cuda_status(launch_kv8_evict(c, weights, cap, lens, B, budget, sink, recent, kept, new_weights, new_lens,
+                                      out_table, out_width, (cudaStream_t)stream));
 }
 
 }  // extern "C"

@@ -13,6 +13,7 @@ namespace paro {
 constexpr uint32_t kErrMbarTimeout = 1u;
 constexpr uint32_t kErrTmemAlloc = 2u;
 constexpr uint32_t kErrGridWait = 4u;     // a wait for other CTAs of the same launch gave up
+constexpr uint32_t kErrBadPage = 8u;      // a page-table entry outside the pool, or lengths that do not fit their table
 
 // One error word per translation unit (no relocatable device code needed);
 // each .cu that uses these helpers exposes it through

@@ -188,10 +188,96 @@ def silu_mul(x):
     return _ops.silu_mul(x)
 
 
+@torch.library.register_fake("paro_b200::attention_prefill")
+def _attention_prefill_fake(q, k, v, cu_seqlens, cu_seqlens_k, scale):
+    return q.new_empty(q.shape)
+
+
+@torch.library.register_fake("paro_b200::kv8_append")
+def _kv8_append_fake(k, v, cu_seqlens, starts, k_codes, v_codes, k_scale, v_scale, page_table):
+    return None
+
+
+@torch.library.register_fake("paro_b200::kv8_gather")
+def _kv8_gather_fake(k_codes, v_codes, k_scale, v_scale, page_table, starts, cu_seqlens, rows, dtype):
+    shape = (rows, k_codes.shape[1], k_codes.shape[3])
+    return (torch.empty(shape, dtype=dtype, device=k_codes.device),
+            torch.empty(shape, dtype=dtype, device=k_codes.device))
+
+
+@torch.library.register_fake("paro_b200::attention_kv8")
+def _attention_kv8_fake(q, k_codes, v_codes, k_scale, v_scale, page_table, seq_lens, scale, weights, weights_out):
+    return q.new_empty(q.shape)
+
+
+@torch.library.register_fake("paro_b200::kv8_evict")
+def _kv8_evict_fake(weights, k_codes, v_codes, k_scale, v_scale, page_table, seq_lens, out_table, budget, sink,
+                    recent):
+    shape = (weights.shape[0], weights.shape[1], budget)
+    return (torch.empty(shape, dtype=torch.int32, device=weights.device), weights.new_empty(shape),
+            torch.empty_like(seq_lens))
+
+
+def attention_prefill(q, k, v, cu_seqlens, cu_seqlens_k=None, scale=None):
+    """Causal attention over packed sequences with grouped heads.
+
+    q [rows, heads, dim], k and v [k_rows, kv_heads, dim] (bf16 or fp16, dim
+    64 or 128; views of a fused projection are read in place), cu_seqlens
+    int32 [B + 1]: each sequence's first row, and the end.  With
+    ``cu_seqlens_k`` the queries are the last ones of longer sequences of
+    keys (a chunk behind its history): query i of Lq sees the keys j <= i +
+    Lk - Lq, and one that sees none gives zeros.  What a query does not see
+    has no effect on it.  ``scale`` defaults to dim ** -0.5."""
+    return _ops.attention_prefill(q, k, v, cu_seqlens, cu_seqlens_k, q.shape[-1] ** -0.5 if scale is None else scale)
+
+
+def kv8_append(k, v, cu_seqlens, starts, k_codes, v_codes, k_scale, v_scale, page_table):
+    """Quantise new tokens (rows cu_seqlens[b] .. of k and v [rows, kv_heads,
+    dim]) into the paged int8 cache as sequence b's tokens starts[b], ... .
+    A page's scale is max|x| / 127 per head; a page that already holds tokens
+    keeps the larger scale and its codes are rescaled.  In place; see
+    ``alpamayo_b200.kv_cache.KV8Cache`` for the layout."""
+    _ops.kv8_append(k, v, cu_seqlens, starts, k_codes, v_codes, k_scale, v_scale, page_table)
+
+
+def kv8_gather(k_codes, v_codes, k_scale, v_scale, page_table, starts, cu_seqlens, rows, dtype=torch.bfloat16):
+    """Token ranges of the cache as (k, v) [rows, kv_heads, dim] of ``dtype``:
+    output rows cu_seqlens[b] .. are sequence b's tokens starts[b], ... ."""
+    return _ops.kv8_gather(k_codes, v_codes, k_scale, v_scale, page_table, starts, cu_seqlens, rows, dtype)
+
+
+def attention_kv8(q, k_codes, v_codes, k_scale, v_scale, page_table, seq_lens, scale=None, weights=None,
+                  weights_out=None):
+    """Attention of each sequence's newest T tokens, q [B, T, heads, dim],
+    over its cached tokens (their own included): query i sees the tokens t <=
+    seq_lens[b] - T + i.
+
+    ``weights`` (float32 [B, kv_heads, capacity]) accumulates the softmax
+    weight every cached token got, summed over the queries and the heads that
+    share a KV head: ``weights_out`` = ``weights`` + that, in place where
+    ``weights_out`` is not given."""
+    if weights is not None and weights_out is None:
+        weights_out = weights
+    return _ops.attention_kv8(q, k_codes, v_codes, k_scale, v_scale, page_table, seq_lens,
+                              q.shape[-1] ** -0.5 if scale is None else scale, weights, weights_out)
+
+
+def kv8_evict(weights, k_codes, v_codes, k_scale, v_scale, page_table, seq_lens, out_table, budget, sink=4, recent=0):
+    """Eviction by accumulated attention weight: every sequence longer than
+    ``budget`` keeps, per KV head, its first ``sink`` and last ``recent``
+    tokens and of the others those with the largest ``weights`` (equal ones:
+    the lowest index).  The kept tokens are written, in order, to the pages of
+    ``out_table``, which no sequence's page_table row may use.  Returns (kept
+    tokens int32 [B, kv_heads, budget], their weights, new lengths)."""
+    return _ops.kv8_evict(weights, k_codes, v_codes, k_scale, v_scale, page_table, seq_lens, out_table, budget, sink,
+                          recent)
+
+
 def device_error_word(clear=True):
-    """Error bits the kernels raised instead of hanging (1 = a bounded
-    pipeline wait ran out, 2 = tensor-memory allocation failed, 4 = a wait
-    for the other CTAs of the same launch ran out); 0 when all
+    """Error bits the kernels raised instead of hanging or leaving their
+    buffers (1 = a bounded pipeline wait ran out, 2 = tensor-memory allocation
+    failed, 4 = a wait for the other CTAs of the same launch ran out, 8 = a
+    page-table entry or a sequence length out of range); 0 when all
     is well, -1 if the word could not be read.  Synchronises the device.
 
     A non-zero word means the outputs of the calls since the last clean read

@@ -265,8 +265,9 @@ int paro_silu_mul(const void* x, int64_t M, int I, void* out, paro_stream_t stre
 
 /* Error bits kernels raise instead of hanging (1 = a pipeline wait timed
  * out, 2 = tensor-memory allocation failed, 4 = a wait for the other CTAs of
- * the same launch timed out); synchronises with the device to
- * read them.  clear != 0 resets the word.  Returns -1 if it cannot be read.
+ * the same launch timed out, 8 = a page-table entry outside the page pool, or
+ * lengths that do not fit their page table or packed rows: the tokens
+ * concerned were left out); synchronises with the device to read them.  clear != 0 resets the word.  Returns -1 if it cannot be read.
  *
  * Recovery: a kernel whose wait ran out stops where it was, so the outputs
  * of the calls made since the last clean read are invalid, and the
@@ -481,6 +482,128 @@ int paro_w4a8_gemm_multicast(const int8_t* xq, const float* xscale, int64_t M, i
 int paro_w4a8_gemm_noalloc(const int8_t* xq, const float* xscale, int64_t M, int N, int K,
                            const void* packed, const void* bias, int bias_dtype,
                            void* out, int out_dtype, paro_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Attention and the int8 key/value cache (a decoder layer between its qkv
+ * and o linears; the reference calls scaled_dot_product_attention over a
+ * bf16 StaticCache, src/alpamayo_r1/utils/system/patches.py:381-548)
+ * ------------------------------------------------------------------------ */
+
+/*
+ * A paged key/value cache in 8 bits.  A page holds page_size tokens of one
+ * sequence for every KV head; K and V each have one float32 scale per (page,
+ * head), and an element stands for code * scale.
+ *   k_codes, v_codes : int8 [num_pages][kv_heads][page_size][head_dim], 16-byte aligned
+ *   k_scale, v_scale : float32 [num_pages][kv_heads]
+ *   page_table       : int32 [B][table_width]; token t of sequence b lies in
+ *                      page page_table[b][t / page_size]; entries behind a
+ *                      sequence's last token are not read
+ * page_size 16, 32, 64 or 128; head_dim 64 or 128.  A page belongs to one
+ * sequence while it is written.  A page-table entry outside the pool, or a
+ * length beyond the table's row, sets bit 8 of the device error word, and
+ * the tokens concerned are left out (nothing out of bounds is touched).
+ */
+typedef struct paro_kv8_cache {
+  int8_t* k_codes;
+  int8_t* v_codes;
+  float* k_scale;
+  float* v_scale;
+  int64_t num_pages;
+  int kv_heads;
+  int page_size;
+  int head_dim;
+} paro_kv8_cache;
+
+/*
+ * Causal attention over packed sequences with grouped heads:
+ *   o_i = sum_{j <= i + Lk - Lq} softmax_j(scale * q_i . k_j) v_j
+ * for query i (of Lq) of each sequence over that sequence's Lk keys; a query
+ * that sees no key gives zeros, and so do rows behind the last sequence.
+ * What a query does not see has no effect on it, whatever it holds.
+ *   q   : [rows][heads][head_dim] of dtype (F16 / BF16), strides in elements
+ *   k, v: [k_rows][kv_heads][head_dim] of the same dtype
+ *   strides[6]: q token, q head, k token, k head, v token, v head; multiples
+ *               of 8; the head_dim elements are contiguous
+ *   cu_q, cu_k: int32 [B + 1] on the device: first row of each sequence, and
+ *               the end; the same pointer for whole prompts
+ *   out : [rows][heads][head_dim] of dtype, contiguous
+ * head_dim 64 or 128; heads a multiple of kv_heads; pointers 16-byte aligned.
+ */
+int paro_attention_prefill(const void* q, const void* k, const void* v, int dtype, const int64_t* strides,
+                           const int32_t* cu_q, const int32_t* cu_k, int B, int64_t rows, int64_t k_rows,
+                           int heads, int kv_heads, int head_dim, float scale, void* out,
+                           paro_stream_t stream);
+
+/*
+ * Writes new tokens' keys and values into the cache: sequence b's rows
+ * cu[b] .. cu[b + 1] - 1 become its tokens starts[b], starts[b] + 1, ...
+ * Per page and head: scale = max|x| / 127 over the page's tokens, code = the
+ * nearest integer to x / scale (ties to even).  A page that already holds
+ * tokens (starts[b] inside it) keeps the larger of its scale and the new
+ * one, and its codes become the nearest integer to code * (old / scale).
+ * Tokens from starts[b] on count as not there before.  Elements that are not
+ * finite make their (page, head) read back as NaN.
+ *   k, v: [rows][kv_heads][head_dim] of dtype (F32 / F16 / BF16)
+ *   strides[4]: k token, k head, v token, v head in elements, multiples of
+ *               16 bytes; cu int32 [B + 1], starts int32 [B], on the device
+ */
+int paro_kv8_append(const paro_kv8_cache* cache, const int32_t* page_table, int table_width,
+                    const void* k, const void* v, int dtype, const int64_t* strides, const int32_t* cu,
+                    const int32_t* starts, int B, int64_t rows, paro_stream_t stream);
+
+/*
+ * Reads token ranges back: output rows cu[b] .. cu[b + 1] - 1 are sequence
+ * b's tokens starts[b], starts[b] + 1, ..., code * scale rounded to dtype.
+ * Rows behind cu[B] are zeros.  out_k, out_v: [rows][kv_heads][head_dim].
+ */
+int paro_kv8_gather(const paro_kv8_cache* cache, const int32_t* page_table, int table_width,
+                    const int32_t* starts, const int32_t* cu, int B, int64_t rows, void* out_k,
+                    void* out_v, int dtype, paro_stream_t stream);
+
+/*
+ * Attention of the newest T tokens of each sequence over the cache (their
+ * own keys and values already appended): query i of sequence b sees the
+ * tokens t <= lens[b] - T + i.  Sums and softmax statistics in float32; a
+ * query that sees nothing gives zeros.
+ *   q   : [B][T][heads][head_dim] of dtype (F16 / BF16); strides[3]: batch,
+ *         token, head in elements, multiples of 8
+ *   lens: int32 [B] on the device
+ *   weights, weights_out: NULL, or float32 [B][kv_heads][cap] with cap >=
+ *         table_width * page_size: weights_out = weights + the softmax
+ *         weight of each of the first lens[b] tokens, summed over the T
+ *         queries and the heads that share the KV head.  The two may be the
+ *         same buffer; apart, a verify step whose draft is rejected can be
+ *         dropped.
+ *   workspace: paro_attention_kv8_workspace_size bytes, 256-byte aligned, of
+ *         any content
+ * T * heads / kv_heads at most 512.
+ */
+size_t paro_attention_kv8_workspace_size(const paro_kv8_cache* cache, int table_width, int B, int T,
+                                         int heads, int with_weights);
+int paro_attention_kv8(const paro_kv8_cache* cache, const int32_t* page_table, int table_width,
+                       const void* q, int dtype, const int64_t* strides, int B, int T, int heads,
+                       const int32_t* lens, float scale, const float* weights, float* weights_out,
+                       int64_t cap, void* out, void* workspace, size_t workspace_bytes,
+                       paro_stream_t stream);
+
+/*
+ * Eviction by accumulated attention weight: for each sequence longer than
+ * budget and each KV head, keeps the first `sink` tokens, the last `recent`
+ * ones and, of the others, those with the largest weights (equal weights:
+ * the lowest index; NaN counts as largest) until budget tokens stay; a
+ * shorter sequence keeps all.  The kept tokens, in order, are written to the
+ * pages of out_table (int32 [B][out_width], out_width * page_size >= budget;
+ * pages that no sequence's page_table row uses), each page with a scale of
+ * its own.
+ *   weights: float32 [B][kv_heads][cap], cap >= table_width * page_size
+ *   kept: int32 [B][kv_heads][budget], the tokens kept, -1 behind the last
+ *   new_weights: float32 [B][kv_heads][budget], their weights, 0 behind
+ *   new_lens: int32 [B], min(lens, budget)
+ */
+int paro_kv8_evict(const paro_kv8_cache* cache, const int32_t* page_table, int table_width,
+                   const float* weights, int64_t cap, const int32_t* lens, int B, int budget, int sink,
+                   int recent, int32_t* kept, float* new_weights, int32_t* new_lens,
+                   const int32_t* out_table, int out_width, paro_stream_t stream);
 
 #ifdef __cplusplus
 }
