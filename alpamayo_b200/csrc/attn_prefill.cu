@@ -1,74 +1,554 @@
-// attn_prefill.cu — causal attention over packed prompts with grouped heads.
+// attn_prefill.cu — causal attention over packed prompts with grouped heads,
+// on the 5th-generation tensor cores (sm_100a).
 //
 //   o_i = sum_{j <= i + Lk - Lq} softmax_j(scale * q_i . k_j) v_j
 //
-// One warp per (query token, head): the lanes hold D / 32 columns each and
-// walk the visible keys with a running maximum and sum.
-#include "tc_ptx.cuh"
+// One CTA per (256 query rows of one sequence, head): two tiles of 128 rows
+// that share every key/value tile of 128 tokens, walked with a running
+// maximum and sum.  Bound by the tensor cores (4 * dim flops per pair) and,
+// nearly as much, by the exponentials: a 128 x 128 tile takes 2 * 512 clocks
+// of tcgen05.mma (dim 128) and 1024 clocks of the SM's 16 exp2 lanes.
+//
+//  * warps 0-3 / 4-7: softmax of tile 0 / 1, one thread per row.  The scores
+//    come from tensor memory into registers; the probabilities go back over
+//    the same columns in 16 bits (the value product takes them from there).
+//    The output is rescaled only when a row's maximum has grown by more than
+//    2^8 since the reference maximum in use (any exact common factor of
+//    terms and sum cancels), so nearly never.
+//  * warp 8: TMA loads, K_0 V_0 K_1 V_1 ... through one ring of tiles.
+//  * warp 9: MMAs, one thread: S = Q K^T (both K-major in shared memory) and
+//    O += P V (P in tensor memory, V with its columns contiguous, i.e.
+//    MN-major).  In issue order ... O_0 += P_0(j) V_j, S_0 = Q_0 K_(j+1),
+//    O_1 += P_1(j) V_j, S_1 = Q_1 K_(j+1) ..., so one tile's softmax runs
+//    under the other's MMAs.  tcgen05 operations of one thread complete in
+//    order: S(j + 1) being ready says that O has taken in P(j).
+//  * warps 10-11: the value tiles that some row of the CTA sees only in part
+//    (at most three: the diagonal ones).  A product with a zero probability
+//    is not zero where the value is not finite, so these warps zero the rows
+//    behind the last key and every value that is not finite, and note the
+//    keys concerned; the epilogue adds those values back, each to the rows
+//    that see it.  What a row does not see has no effect on it.
+//
+// Probabilities are rounded to the inputs' type for the value product (the
+// relative error of 2^-9 that bf16 operands of the tensor core have anyhow;
+// it is of the size of the output's own rounding); sums, maxima and the
+// output stay in float32, and the denominator adds the unrounded terms.
+#include "umma.cuh"
 
 namespace paro {
 
+PARO_DEFINE_ERROR_ACCESSOR(attn)
+
+constexpr int kPfRows = 128;       // query rows per tile, keys per tile
+constexpr int kPfThreads = 384;
+constexpr int kPfMasked = 3;       // key tiles that a CTA's rows see in part, at most
+
 struct PrefillParams {
-  const void* q;
-  const void* k;
-  const void* v;
-  int64_t sq_t, sq_h, sk_t, sk_h, sv_t, sv_h;
   const int32_t* cu_q;
   const int32_t* cu_k;
   int B, heads, group;
-  int64_t rows, k_rows;
+  int rows, k_rows;
   float scale_log2;
   void* out;
+  const void* v;                   // for the values that are not finite
+  int64_t sv_t, sv_h;
 };
 
+template <int D>
+struct PrefillTile {
+  static constexpr int kAtoms = D / 64;                    // 128-byte wide columns of a tile
+  static constexpr int kTileBytes = kPfRows * D * 2;       // one Q, K or V tile
+  static constexpr int kSlots = 5;
+  static constexpr int kOffKv = 2 * kTileBytes;
+  static constexpr int kOffBar = kOffKv + kSlots * kTileBytes;
+  static constexpr int kSmem = kOffBar + 512 + 1024;
+  static constexpr int kTmemO = 256;                       // S_0, S_1: columns 0 and 128; O_0, O_1: from 256
+};
+
+namespace {
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+      ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+      "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]),
+      "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]),
+      "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// D[tmem] (+)= A[smem] * B[smem], one CTA
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem]
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(
+          d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// Arrives on `bar` when every tcgen05 operation issued so far by this thread is done.
+__device__ __forceinline__ void umma_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+
+// MN-major operand with 128-byte swizzle: 64 columns (128 bytes) by 8 rows
+// per 1024-byte atom; the next 8 rows 1024 bytes on (stride byte offset), the
+// next 64 columns a whole 128-row column block on (leading byte offset).
+__device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)((kPfRows * 128) >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <typename T> __device__ __forceinline__ uint32_t pack16(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack16<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack16<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <typename T> struct Type16;
+template <> struct Type16<__nv_bfloat16> {
+  static constexpr uint32_t kFmt = 1;                 // instruction descriptor's operand type
+  static constexpr uint32_t kExp = 0x7F807F80u, kOne = 0x00800080u;   // exponent bits, their lowest
+  static constexpr float kShift = 0.f;
+};
+template <> struct Type16<__half> {
+  static constexpr uint32_t kFmt = 0;
+  static constexpr uint32_t kExp = 0x7C007C00u, kOne = 0x04000400u;
+  // terms are kept times 2^6: up to 2^14 with the lazy maximum, and normal
+  // fp16 numbers down to 2^-20 of the reference maximum
+  static constexpr float kShift = 6.f;
+};
+
+// Whether either half of the word is infinite or NaN: the exponent bits all
+// set carry into the sign bit.
+template <typename T> __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+  return ((w & Type16<T>::kExp) + Type16<T>::kOne) & 0x80008000u;
+}
+
+}  // namespace
+
 template <typename T, int D>
-__global__ void __launch_bounds__(128) attn_prefill_kernel(PrefillParams p) {
-  constexpr int E = D / 32;
-  const int lane = threadIdx.x & 31;
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (w >= p.rows * p.heads) return;
-  const int64_t row = w / p.heads;
-  const int h = (int)(w - row * p.heads), hk = h / p.group;
-  int b = 0;
-  while (b < p.B && row >= p.cu_q[b + 1]) ++b;
-  float o[E] = {}, m = -INFINITY, l = 0.f;
-  if (b < p.B) {
-    const int64_t lq = p.cu_q[b + 1] - p.cu_q[b], lk = p.cu_k[b + 1] - p.cu_k[b];
-    const int64_t see = row - p.cu_q[b] + lk - lq + 1;
-    float qf[E];
-    for (int e = 0; e < E; ++e)
-      qf[e] = to_f32(static_cast<const T*>(p.q)[row * p.sq_t + h * p.sq_h + lane * E + e]) * p.scale_log2;
-    for (int64_t j = 0; j < see; ++j) {
-      const T* k = static_cast<const T*>(p.k) + (p.cu_k[b] + j) * p.sk_t + hk * p.sk_h + lane * E;
-      const T* v = static_cast<const T*>(p.v) + (p.cu_k[b] + j) * p.sv_t + hk * p.sv_h + lane * E;
-      float s = 0.f;
-      for (int e = 0; e < E; ++e) s = fmaf(qf[e], to_f32(k[e]), s);
-      for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-      const float mn = fmaxf(m, s), a = exp2f(m - mn), e0 = exp2f(s - mn);
-      m = mn;
-      l = fmaf(l, a, e0);
-      for (int e = 0; e < E; ++e) o[e] = fmaf(e0, to_f32(v[e]), o[e] * a);
+__global__ void __launch_bounds__(kPfThreads, 1)
+attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                    const __grid_constant__ CUtensorMap vmap, const __grid_constant__ PrefillParams p) {
+  using C = PrefillTile<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + C::kOffBar);  // [2]
+  uint64_t* full = q_full + 2;                                        // [slots] a K or V tile has landed
+  uint64_t* empty = full + C::kSlots;                                 // [slots] its MMAs are done
+  uint64_t* s_full = empty + C::kSlots;                               // [2] scores ready (and O up to date)
+  uint64_t* p_ready = s_full + 2;                                     // [2] probabilities written
+  uint64_t* o_full = p_ready + 2;                                     // [2] output complete
+  uint64_t* v_full = o_full + 2;                                      // [3] partly seen value tile has landed
+  uint64_t* v_ok = v_full + kPfMasked;                                // [3] ... and is cleaned
+  uint64_t* done = v_ok + kPfMasked;                                  // [1] every MMA is done
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  uint32_t* poison = tmem_slot + 1;                                   // [3][4] keys with values that are not finite
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int h = blockIdx.x % p.heads, hk = h / p.group;
+  const int slot = blockIdx.x / p.heads;
+
+  // this CTA's rows: sequence b, rows r0 .. of it, the last ones first (the
+  // longest work starts earliest); b = B: rows behind the last sequence
+  int64_t first = 0;
+  int b = -1;
+  {
+    int64_t before = 0;
+    for (int b0 = 0; b0 <= p.B && b < 0; b0 += 32) {
+      const int i = b0 + lane;
+      int64_t mine = 0;
+      if (i <= p.B) {
+        const int lo = min(max(p.cu_q[i], 0), p.rows), hi = i < p.B ? min(max(p.cu_q[i + 1], lo), p.rows) : p.rows;
+        mine = (hi - lo + 2 * kPfRows - 1) / (2 * kPfRows);
+      }
+      int64_t incl = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, before + incl > slot);
+      if (hit) {
+        const int src = __ffs(hit) - 1;
+        b = b0 + src;
+        first = before + __shfl_sync(0xffffffffu, incl - mine, src);
+      }
+      before += __shfl_sync(0xffffffffu, incl, 31);
     }
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  for (int e = 0; e < E; ++e) static_cast<T*>(p.out)[(row * p.heads + h) * D + lane * E + e] = from_f32<T>(o[e] * inv);
+  if (b < 0) return;
+  const int q0 = min(max(p.cu_q[b], 0), p.rows);
+  const int lq = (b < p.B ? min(max(p.cu_q[b + 1], q0), p.rows) : p.rows) - q0;
+  const int k0 = b < p.B ? min(max(p.cu_k[b], 0), p.k_rows) : 0;
+  const int lk = b < p.B ? min(max(p.cu_k[b + 1], k0), p.k_rows) - k0 : 0;
+  if (threadIdx.x == 0 && b < p.B && (q0 != p.cu_q[b] || lq != p.cu_q[b + 1] - q0 || k0 != p.cu_k[b] ||
+                                      lk != p.cu_k[b + 1] - k0))
+    report_error(kErrBadPage);
+  const int tiles_q = (lq + 2 * kPfRows - 1) / (2 * kPfRows);
+  const int r0 = (tiles_q - 1 - (int)(slot - first)) * 2 * kPfRows;
+  const int off = lk - lq;                                 // row i sees keys j <= i + off
+  // key tiles of each row tile (0: no rows, or none that sees a key)
+  int nk[2];
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const int begin = r0 + s * kPfRows, end = min(lq, begin + kPfRows);
+    nk[s] = begin < lq && end + off > 0 ? (end + off + kPfRows - 1) / kPfRows : 0;
+  }
+  const int nmax = max(nk[0], nk[1]);
+  const int jm = min(nmax, max(0, (r0 + off + 1) / kPfRows));   // tiles from jm on are seen in part by some row
+  T* out = static_cast<T*>(p.out);
+  if (nmax == 0) {                                         // nothing to see: zeros
+    const int n = min(2 * kPfRows, lq - r0);
+    for (int e = threadIdx.x; e < n * (D / 8); e += kPfThreads) {
+      const int r = e / (D / 8), d = (e - r * (D / 8)) * 8;
+      *reinterpret_cast<uint4*>(out + ((int64_t)(q0 + r0 + r) * p.heads + h) * D + d) = make_uint4(0u, 0u, 0u, 0u);
+    }
+    return;
+  }
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&q_full[s], 1);
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_ready[s], 4);
+      mbar_init(&o_full[s], 1);
+    }
+    for (int i = 0; i < C::kSlots; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < kPfMasked; ++i) {
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_ok[i], 2);
+    }
+    mbar_init(done, 1);
+    fence_mbar_init();
+  }
+  if (threadIdx.x < 4 * kPfMasked) poison[threadIdx.x] = 0u;
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "n"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  bool failed = false;
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == 8 && lane == 0) {
+      // loader: ring position 2 j holds K_j, 2 j + 1 holds V_j
+      auto load = [&](const CUtensorMap* map, uint8_t* dst, int head, int row, uint64_t* bar) {
+        mbar_arrive_expect_tx(bar, C::kTileBytes);
+#pragma unroll
+        for (int a = 0; a < C::kAtoms; ++a) tma_load_3d(dst + a * kPfRows * 128, map, a * 64, head, row, bar);
+      };
+      if (nk[0]) load(&qmap, smem, h, q0 + r0, &q_full[0]);
+      int n = 0;
+      for (; n < 2 * nmax; ++n) {
+        const int s = n % C::kSlots;
+        if (n >= C::kSlots && !mbar_wait(&empty[s], ((n / C::kSlots) - 1) & 1)) {
+          failed = true;
+          break;
+        }
+        // a partly seen value tile goes to the cleaning warps: it has a
+        // barrier of its own, and the slot's passes on to the next phase
+        const bool masked = (n & 1) && (n >> 1) >= jm;
+        if (masked) mbar_arrive(&full[s]);
+        load((n & 1) ? &vmap : &kmap, smem + C::kOffKv + s * C::kTileBytes, hk, k0 + (n >> 1) * kPfRows,
+             masked ? &v_full[(n >> 1) - jm] : &full[s]);
+        if (n == 0 && nk[1]) load(&qmap, smem + C::kTileBytes, h, q0 + r0 + kPfRows, &q_full[1]);
+      }
+      // no copy is left in flight, whatever became of its readers
+      for (int i = max(0, n - C::kSlots); i < n; ++i)
+        mbar_wait((i & 1) && (i >> 1) >= jm ? &v_full[(i >> 1) - jm] : &full[i % C::kSlots],
+                  (i & 1) && (i >> 1) >= jm ? 0 : (i / C::kSlots) & 1);
+      if (nk[0]) mbar_wait(&q_full[0], 0);
+      if (nk[1] && n > 0) mbar_wait(&q_full[1], 0);
+    } else if (warp == 9 && lane == 0) {
+      constexpr uint32_t kFmt = (1u << 4) | (Type16<T>::kFmt << 7) | (Type16<T>::kFmt << 10) |
+                                ((uint32_t)(kPfRows >> 4) << 24);
+      constexpr uint32_t kIdS = kFmt | ((uint32_t)(kPfRows >> 3) << 17);
+      constexpr uint32_t kIdO = kFmt | (1u << 16) | ((uint32_t)(D >> 3) << 17);   // B is MN-major
+      const uint32_t q_at = smem_u32(smem), kv_at = smem_u32(smem + C::kOffKv);
+      auto scores = [&](int s, int j) {        // S_s = Q_s K_j^T
+        const uint64_t da = umma_desc_sw128(q_at + s * C::kTileBytes);
+        const uint64_t db = umma_desc_sw128(kv_at + ((2 * j) % C::kSlots) * C::kTileBytes);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t o = ((k >> 2) * (kPfRows * 128) + (k & 3) * 32) >> 4;
+          mma_f16_ss(tmem + s * kPfRows, da + o, db + o, kIdS, k > 0);
+        }
+        umma_commit(&s_full[s]);
+      };
+      auto values = [&](int s, int j) {        // O_s += P_s V_j
+        const uint64_t db = umma_desc_mn_sw128(kv_at + ((2 * j + 1) % C::kSlots) * C::kTileBytes);
+#pragma unroll
+        for (int k = 0; k < kPfRows / 16; ++k)
+          mma_f16_ts(tmem + C::kTmemO + s * 128, tmem + s * kPfRows + k * 8, db + k * (2048 >> 4), kIdO, j > 0 || k > 0);
+      };
+      auto landed = [&](int n) { return mbar_wait(&full[n % C::kSlots], (n / C::kSlots) & 1); };
+      if (!landed(0)) failed = true;
+      for (int s = 0; s < 2 && !failed; ++s) {
+        if (!nk[s]) continue;
+        if (!mbar_wait(&q_full[s], 0)) failed = true;
+        else scores(s, 0);
+      }
+      if (!failed) umma_commit(&empty[0]);
+      for (int j = 0; j < nmax && !failed; ++j) {
+        if (!(j < jm ? landed(2 * j + 1) : mbar_wait(&v_ok[j - jm], 0)) || (j + 1 < nmax && !landed(2 * j + 2))) {
+          failed = true;
+          break;
+        }
+        for (int s = 0; s < 2; ++s) {
+          if (j >= nk[s]) continue;
+          if (!mbar_wait(&p_ready[s], j & 1)) {
+            failed = true;
+            break;
+          }
+          tc_fence_after();
+          values(s, j);
+          if (j + 1 < nk[s]) scores(s, j + 1);
+          else umma_commit(&o_full[s]);
+        }
+        if (failed) break;
+        umma_commit(&empty[(2 * j + 1) % C::kSlots]);
+        if (j + 1 < nmax) umma_commit(&empty[(2 * j + 2) % C::kSlots]);
+      }
+      umma_commit(done);                       // the tensor memory is not freed under an MMA
+      mbar_wait(done, 0);
+    } else if (warp >= 10) {
+      for (int j = jm; j < nmax; ++j) {
+        const int n = 2 * j + 1;
+        if (!__all_sync(0xffffffffu, mbar_wait(&v_full[j - jm], 0))) break;
+        uint8_t* tile = smem + C::kOffKv + (n % C::kSlots) * C::kTileBytes;
+        const int keys = min(kPfRows, lk - j * kPfRows);
+        for (int c = threadIdx.x - 320; c < C::kTileBytes / 16; c += 64) {   // 16-byte pieces, 8 to a 128-byte row
+          uint4* at = reinterpret_cast<uint4*>(tile) + c;
+          const int key = (c >> 3) % kPfRows;
+          if (key >= keys) {
+            *at = make_uint4(0u, 0u, 0u, 0u);
+            continue;
+          }
+          uint4 w = *at;
+          if (not_finite<T>(w.x) | not_finite<T>(w.y) | not_finite<T>(w.z) | not_finite<T>(w.w)) {
+            atomicOr(&poison[(j - jm) * 4 + (key >> 5)], 1u << (key & 31));
+            uint32_t* x = &w.x;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t bad = not_finite<T>(x[i]);
+              if (bad & 0x8000u) x[i] &= 0xffff0000u;
+              if (bad & 0x80000000u) x[i] &= 0x0000ffffu;
+            }
+            *at = w;
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_ok[j - jm]);
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int s = warp >> 2, quarter = warp & 3;
+    const int row = r0 + s * kPfRows + quarter * 32 + lane;      // within the sequence
+    const uint32_t t_s = tmem + s * kPfRows + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t t_o = tmem + C::kTmemO + s * 128 + ((uint32_t)(quarter * 32) << 16);
+    const int n = nk[s], see = min(lk, row + off + 1);           // keys this row sees
+    const int seen_by_all = r0 + s * kPfRows + off + 1;          // keys the tile's first row sees
+    float m = -INFINITY, sum = 0.f;                              // reference maximum of the raw scores, sum of terms
+    const float scale = p.scale_log2;
+    bool fail = false;
+    for (int j = 0; j < n; ++j) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&s_full[s], j & 1))) {
+        fail = true;
+        break;
+      }
+      tc_fence_after();
+      uint32_t x[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, x[c]);
+      tmem_wait_ld();
+      const int here = see - j * kPfRows;
+      if ((j + 1) * kPfRows > seen_by_all) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) x[c][i] = c * 32 + i < here ? x[c][i] : 0xff800000u;
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int i = 0; i < 32; i += 2)
+          top = fmaxf(fmaxf(top, __uint_as_float(x[c][i])), __uint_as_float(x[c][i + 1]));
+      // a new reference maximum where the terms would pass 2^8
+      const bool grow = top > m && (m == -INFINITY || (top - m) * scale > 8.f);
+      if (__any_sync(0xffffffffu, grow)) {
+        const float a = grow ? (m == -INFINITY ? 0.f : ex2((m - top) * scale)) : 1.f;
+        if (grow) {
+          m = top;
+          sum *= a;
+        }
+        if (j > 0) {
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32(t_o + c * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
+            tmem_st32(t_o + c * 32, o);
+          }
+        }
+      }
+      const float neg = m == -INFINITY ? 0.f : Type16<T>::kShift - m * scale;
+      float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t w[32];
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            const float e0 = ex2(fmaf(__uint_as_float(x[half * 2 + c][i]), scale, neg));
+            const float e1 = ex2(fmaf(__uint_as_float(x[half * 2 + c][i + 1]), scale, neg));
+            part[(i >> 1) & 1] += e0;
+            part[2 + ((i >> 1) & 1)] += e1;
+            w[c * 16 + (i >> 1)] = pack16<T>(e0, e1);
+          }
+        tmem_st32(t_s + half * 32, w);
+      }
+      sum += (part[0] + part[1]) + (part[2] + part[3]);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_ready[s]);
+    }
+    const bool live = row < lq;
+    T* dst = out + ((int64_t)(q0 + row) * p.heads + h) * D;
+    if (n && !fail && __all_sync(0xffffffffu, mbar_wait(&o_full[s], 0))) {
+      tc_fence_after();
+      const float inv = see > 0 ? 1.f / sum : 0.f;
+      uint32_t any = 0;
+#pragma unroll
+      for (int i = 0; i < 4 * kPfMasked; ++i) any |= poison[i];
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld32(t_o + c * 32, o);
+        tmem_wait_ld();
+        float f[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) f[i] = see > 0 ? __uint_as_float(o[i]) * inv : 0.f;
+        if (any) {
+          for (int i = 0; i < 4 * kPfMasked; ++i) {
+            uint32_t bits = poison[i];
+            while (bits) {
+              const int key = jm * kPfRows + i * 32 + __ffs(bits) - 1;
+              bits &= bits - 1;
+              if (key >= see) continue;
+              const T* vr = static_cast<const T*>(p.v) + (int64_t)(k0 + key) * p.sv_t + (int64_t)hk * p.sv_h + c * 32;
+#pragma unroll
+              for (int d = 0; d < 32; ++d) {
+                const float v = to_f32(vr[d]);
+                if (!isfinite(v)) f[d] += v;
+              }
+            }
+          }
+        }
+        if (live) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8)
+            *reinterpret_cast<uint4*>(dst + c * 32 + i) =
+                make_uint4(pack16<T>(f[i], f[i + 1]), pack16<T>(f[i + 2], f[i + 3]), pack16<T>(f[i + 4], f[i + 5]),
+                           pack16<T>(f[i + 6], f[i + 7]));
+        }
+      }
+    } else if (!n && live) {                                     // this tile's rows see nothing
+#pragma unroll 1
+      for (int d = 0; d < D; d += 8) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512));
+}
+
+// ---------------------------------------------------------------------------
+// launch
+// ---------------------------------------------------------------------------
+// [tokens][heads][dim] with the given element strides; boxes of 128 tokens
+// by 64 columns of one head.
+static bool encode_rows(CUtensorMap* map, const void* base, int dtype, int64_t rows, int heads, int dim, int64_t st_t,
+                        int64_t st_h) {
+  auto encode = get_encode();
+  if (!encode) return false;
+  // the stride of a dimension of one element is not used, but has to be valid
+  if (heads == 1) st_h = dim;
+  if (rows == 1) st_t = dim;
+  const cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)rows};
+  const cuuint64_t strides[2] = {(cuuint64_t)st_h * 2, (cuuint64_t)st_t * 2};
+  const cuuint32_t box[3] = {64, 1, (cuuint32_t)kPfRows}, estr[3] = {1, 1, 1};
+  return encode(map, dtype == PARO_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int D>
+static cudaError_t launch_prefill(const CUtensorMap* maps, const PrefillParams& p, int64_t slots, cudaStream_t st) {
+  using C = PrefillTile<D>;
+  const cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(attn_prefill_kernel<T, D>), C::kSmem);
+  if (e != cudaSuccess) return e;
+  attn_prefill_kernel<T, D><<<(unsigned)(slots * p.heads), kPfThreads, C::kSmem, st>>>(maps[0], maps[1], maps[2], p);
+  return cudaGetLastError();
 }
 
 cudaError_t launch_attn_prefill(const void* q, const void* k, const void* v, int dtype, const int64_t* s,
                                 const int32_t* cu_q, const int32_t* cu_k, int B, int64_t rows, int64_t k_rows,
                                 int heads, int kv_heads, int dim, float scale, void* out, cudaStream_t st) {
-  PrefillParams p{q, k, v, s[0], s[1], s[2], s[3], s[4], s[5], cu_q, cu_k, B, heads, heads / kv_heads, rows, k_rows,
-                  scale * 1.4426950408889634f, out};
-  const int64_t blocks = (rows * heads + 3) / 4;
-  if (blocks > 0x7FFFFFFF) return cudaErrorInvalidValue;
-  if (dtype == PARO_BF16) {
-    if (dim == 128) attn_prefill_kernel<__nv_bfloat16, 128><<<(unsigned)blocks, 128, 0, st>>>(p);
-    else attn_prefill_kernel<__nv_bfloat16, 64><<<(unsigned)blocks, 128, 0, st>>>(p);
-  } else {
-    if (dim == 128) attn_prefill_kernel<__half, 128><<<(unsigned)blocks, 128, 0, st>>>(p);
-    else attn_prefill_kernel<__half, 64><<<(unsigned)blocks, 128, 0, st>>>(p);
-  }
-  return cudaGetLastError();
+  if (k_rows == 0) return cudaMemsetAsync(out, 0, (size_t)rows * heads * dim * 2, st);
+  CUtensorMap maps[3];
+  if (!encode_rows(&maps[0], q, dtype, rows, heads, dim, s[0], s[1]) ||
+      !encode_rows(&maps[1], k, dtype, k_rows, kv_heads, dim, s[2], s[3]) ||
+      !encode_rows(&maps[2], v, dtype, k_rows, kv_heads, dim, s[4], s[5]))
+    return cudaErrorInvalidValue;
+  // a scale of zero still has to leave -infinity where a key is not seen
+  const float scale_log2 = fmaxf(scale * 1.4426950408889634f, 1e-37f);
+  const PrefillParams p{cu_q, cu_k, B, heads, heads / kv_heads, (int)rows, (int)k_rows, scale_log2, out, v, s[4], s[5]};
+  // at most one tile more than whole ones per sequence (and for the rows behind the last)
+  int64_t slots = rows / (2 * kPfRows) + B + 1;
+  if (slots > rows) slots = rows;
+  if (slots * heads > 0x7FFFFFFF) return cudaErrorInvalidValue;
+  if (dtype == PARO_BF16)
+    return dim == 128 ? launch_prefill<__nv_bfloat16, 128>(maps, p, slots, st)
+                      : launch_prefill<__nv_bfloat16, 64>(maps, p, slots, st);
+  return dim == 128 ? launch_prefill<__half, 128>(maps, p, slots, st) : launch_prefill<__half, 64>(maps, p, slots, st);
 }
 
 }  // namespace paro

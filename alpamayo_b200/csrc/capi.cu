@@ -91,6 +91,7 @@ uint32_t error_word_rtc(int clear);
 uint32_t error_word_rows(int clear);
 uint32_t error_word_kv8(int clear);
 uint32_t error_word_kv8a(int clear);
+uint32_t error_word_attn(int clear);
 
 cudaError_t ensure_smem_limit(const void* kernel, int bytes) {
   static std::mutex mu;
@@ -641,7 +642,8 @@ int paro_silu_mul(const void* x, int64_t M, int I, void* out, paro_stream_t stre
 
 int paro_device_error_word(int clear) {
   const uint32_t words[] = {error_word_decode(clear), error_word_tc(clear),  error_word_rtc(clear),
-                            error_word_rows(clear),   error_word_kv8(clear), error_word_kv8a(clear)};
+                            error_word_rows(clear),   error_word_kv8(clear), error_word_kv8a(clear),
+                            error_word_attn(clear)};
   uint32_t all = 0;
   for (const uint32_t w : words) {
     if (w == ~0u) return -1;
@@ -834,6 +836,7 @@ int paro_attention_prefill(const void* q, const void* k, const void* v, int dtyp
   if (rows < 0 || k_rows < 0 || B < 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return PARO_ERR_INVALID_ARGUMENT;
   if (dtype != PARO_BF16 && dtype != PARO_F16) return PARO_ERR_UNSUPPORTED;
   if (heads % kv_heads || (head_dim != 64 && head_dim != 128)) return PARO_ERR_SHAPE;
+  if (!(scale >= 0.f) || scale > 3.0e38f) return PARO_ERR_INVALID_ARGUMENT;
   if (rows > 0x7FFFFFFF || k_rows > 0x7FFFFFFF || heads > 65535) return PARO_ERR_TOO_LARGE;
   if (rows == 0) return PARO_OK;
   if (!q || !out || !strides || !cu_q || !cu_k || (k_rows > 0 && (!k || !v))) return PARO_ERR_INVALID_ARGUMENT;

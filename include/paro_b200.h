@@ -527,7 +527,8 @@ typedef struct paro_kv8_cache {
  *   cu_q, cu_k: int32 [B + 1] on the device: first row of each sequence, and
  *               the end; the same pointer for whole prompts
  *   out : [rows][heads][head_dim] of dtype, contiguous
- * head_dim 64 or 128; heads a multiple of kv_heads; pointers 16-byte aligned.
+ * head_dim 64 or 128; heads a multiple of kv_heads; pointers 16-byte aligned;
+ * scale finite and not negative.
  */
 int paro_attention_prefill(const void* q, const void* k, const void* v, int dtype, const int64_t* strides,
                            const int32_t* cu_q, const int32_t* cu_k, int B, int64_t rows, int64_t k_rows,
