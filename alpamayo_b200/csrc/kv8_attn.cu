@@ -10,10 +10,12 @@
 // for all the query heads that share the head.  The work is cut into units
 // of 32 tokens of one (sequence, KV head); the grid's CTAs take equal runs
 // of consecutive units (the lengths are read on the device), so ragged
-// lengths and few long sequences balance alike.  Inside a CTA the four warps
-// take units in turn, each with a private ring of cp.async stages in which a
-// lane copies exactly the 16-byte pieces that it will itself read: no
-// barrier and no bank conflict between the copy and its use.
+// lengths and few long sequences balance alike.  Inside a CTA teams of 1, 2 or
+// 4 warps (16 query rows each) take units in turn, each team with its own
+// ring of cp.async stages, laid out so that a lane reads back the 16-byte
+// places of its own lane number: no bank conflicts, and for teams of one
+// warp no barrier between the copy and its use.  The page table is read a
+// unit ahead of the copies.
 //
 // The products run on mma.sync m16n8k16 in fp16 with float32 sums: int8
 // codes are exact in fp16, q is scaled per row by a power of two to fill
@@ -55,6 +57,7 @@ struct DecodeParams {
   float* part_o;               // [row blocks][slots][RB][dim]
   float2* part_ml;             // [row blocks][slots][RB] (M, sum)
   int slots;                   // B * kv_heads + ctas
+  int lanes, out_blocks;       // second kernel: threads per output column group, blocks of output rows
   float* scores;               // [B * kv_heads][rows][score_cap] log2-scaled scores, or null
   int64_t score_cap;
   const float* weights;        // [B][kv_heads][cap] or null
@@ -97,8 +100,6 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-template <typename T> __device__ __forceinline__ T from_out(float v) { return from_f32<T>(v); }
-
 // units of sequence b per KV head
 __device__ __forceinline__ int64_t seq_units(const DecodeParams& p, int b) {
   const int64_t cap = (int64_t)p.c.table_width << p.c.page_shift;
@@ -120,32 +121,37 @@ __device__ __forceinline__ int64_t units_per_cta(const DecodeParams& p, int64_t*
 
 }  // namespace
 
-// RB rows per CTA: 8 (the upper half of the only m16 tile idle), 16 or 32.
-template <typename T, int D, int RB>
+// Warps of a CTA: WR of them share a unit and hold 16 rows each (8 for RB =
+// 8), and 4 / WR such teams take units in turn.  More rows than one warp's
+// mean that every team member expands the unit's codes for itself; the
+// cache's bytes still come once.
+template <int D, int RB>
 struct DecodeTile {
-  static constexpr int kMt = RB <= 16 ? 1 : RB / 16;     // m16 tiles
-  static constexpr int kSlots = D / 8;                    // 16-byte slots per lane and stage (K and V)
-  static constexpr int kStage = kSlots * 512 + 32;        // + the unit's four scales
-  static constexpr int kStages = D == 128 ? 3 : 4;
-  static constexpr int kRing = kDecWarps * kStages * kStage;
-  static constexpr int kComb = RB * D * 4;                // one warp's partial on its way to the next warp
-  static constexpr int kSmem = kRing + kComb + RB * 4 * 8;
+  static constexpr int kWr = RB <= 16 ? 1 : RB / 16;     // warps of a team
+  static constexpr int kTeams = kDecWarps / kWr;
+  static constexpr int kWarpRows = RB / kWr;             // 8 or 16
+  static constexpr int kSlots = D / 8;                   // 16-byte slots per lane and stage (K and V)
+  static constexpr int kStage = kSlots * 512 + 32;       // + the unit's four scales
+  static constexpr int kStages = kWr == 1 ? (D == 128 ? 3 : 4) : 4;
+  static constexpr int kRing = kTeams * kStages * kStage;
+  static constexpr int kComb = kTeams > 1 ? RB * D * 4 + RB * 32 : 0;   // one team's partial on its way to the next
+  static constexpr int kSmem = kRing + kComb;
 };
 
 template <typename T, int D, int RB>
-__global__ void __launch_bounds__(kDecWarps * 32) kv8_attn_kernel(const __grid_constant__ DecodeParams p) {
-  using C = DecodeTile<T, D, RB>;
-  constexpr int MT = C::kMt;
-  constexpr bool kUpper = RB > 8;           // rows g + 8 of a tile in use
+__global__ void __launch_bounds__(kDecWarps * 32, 2) kv8_attn_kernel(const __grid_constant__ DecodeParams p) {
+  using C = DecodeTile<D, RB>;
+  constexpr bool kUpper = RB > 8;           // rows g + 8 of the m16 tile in use
   constexpr int kHalves = kUpper ? 2 : 1;
   constexpr int KS = D / 16;                // k16 steps of the score product
   constexpr int NT = D / 8;                 // n8 tiles of the value product
   constexpr int VW = D / 32;                // 4-byte words of a lane's piece of a V token
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  uint8_t* ring = smem + warp * (C::kStages * C::kStage);
-  float4* comb = reinterpret_cast<float4*>(smem + C::kRing);                // [row halves][NT / 2][32 lanes]
-  float2* comb_ml = reinterpret_cast<float2*>(smem + C::kRing + C::kComb);  // [row halves][32 lanes]
+  const int team = warp / C::kWr, wr = warp % C::kWr;
+  uint8_t* ring = smem + team * (C::kStages * C::kStage);
+  float4* comb = reinterpret_cast<float4*>(smem + C::kRing) + wr * (kHalves * (NT / 2) * 32);   // [halves][NT / 2][lanes]
+  float2* comb_ml = reinterpret_cast<float2*>(smem + C::kRing + RB * D * 4) + wr * (kHalves * 32);
   const Kv8View& c = p.c;
   const int page = 1 << c.page_shift;
 
@@ -159,67 +165,88 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv8_attn_kernel(const __grid_c
   int64_t su = seq_units(p, b);
   int h = (int)((u0 - first) / su);
   int64_t unit0 = u0 - first - h * su;      // first unit within (b, h)
-  const int row0 = blockIdx.y * RB;
+  const int row0 = blockIdx.y * RB + wr * C::kWarpRows;
 
-  // the producer's place: this warp's next unit to copy
-  int pb = b, ph = h;
-  int64_t psu = su, pu = u0 + warp, pfirst = first + h * su;   // pfirst: flat index of (pb, ph)'s unit 0
-  auto issue = [&](int stage) {
-    if (pu < u1) {
+  // The copies run ahead of the products, and the page table ahead of the
+  // copies: look_up() loads the next unit's two pages (a unit's 32 tokens
+  // lie in at most two), issue() copies the unit that was looked up before.
+  int pb = b, ph = h, plen = kv8_len(c, p.lens[b]);
+  int64_t psu = su, pu = u0 + team, pfirst = first + h * su;   // pfirst: flat index of (pb, ph)'s unit 0
+  int n_id[2] = {0, 0}, n_tok = 0, n_head = 0;
+  bool n_any = false;
+  auto look_up = [&]() {
+    n_any = pu < u1;
+    if (n_any) {
       while (pu >= pfirst + psu) {          // next (sequence, head) that has units
         pfirst += psu;
         if (++ph == c.kv_heads) {
           ph = 0;
           do ++pb; while (seq_units(p, pb) == 0);
           psu = seq_units(p, pb);
+          plen = kv8_len(c, p.lens[pb]);
         }
       }
-      const int len = kv8_len(c, p.lens[pb]);
-      const int tok0 = (int)(pu - pfirst) * kUnit;
-      const int lastblk = (len - 1) >> c.page_shift;
-      int64_t kb[2];                        // element offset of token tok0 and tok0 + 16's page starts
-      int id[2];
+      n_tok = (int)(pu - pfirst) * kUnit;
+      n_head = ph;
+      const int32_t* row = c.table + (int64_t)pb * c.table_width;
+      const int last = (plen - 1) >> c.page_shift;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) n_id[i] = row[min((n_tok + 16 * i) >> c.page_shift, last)];
+    }
+    pu += C::kTeams;
+  };
+  auto issue = [&](int stage) {
+    if (n_any) {
+      int64_t kb[2];                        // element offsets of tokens n_tok and n_tok + 16
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int blk = min((tok0 + 16 * i) >> c.page_shift, lastblk);
-        id[i] = max(0, kv8_page(c, pb, blk));
-        kb[i] = kv8_base(c, id[i], ph) + (int64_t)((tok0 + 16 * i) & (page - 1)) * D;
+        if (n_id[i] < 0 || n_id[i] >= c.num_pages) {
+          report_error(kErrBadPage);
+          n_id[i] = 0;
+        }
+        kb[i] = kv8_base(c, n_id[i], n_head) + (int64_t)((n_tok + 16 * i) & (page - 1)) * D;
       }
-      const uint32_t dst = smem_u32(ring + stage * C::kStage) + lane * 16;
+      const uint32_t at = smem_u32(ring + stage * C::kStage), dst = at + lane * 16;
+      // the team's warps take the pieces in turn
       // K: slot (j, i) = token 8 j + g, bytes 64 i + 16 t
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int j = 0; j < 4; ++j) {
+        if (j % C::kWr != wr) continue;
 #pragma unroll
         for (int i = 0; i < D / 64; ++i)
           cp_async16(dst + (j * (D / 64) + i) * 512,
                      c.k_codes + kb[j >> 1] + ((j & 1) * 8 + g) * D + i * 64 + t * 16);
+      }
       // V: slot (kk, x) = token 16 kk + {2t, 2t + 1, 2t + 8, 2t + 9}[x], bytes of lane g's D / 8 columns
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
+          if ((kk * 4 + x) % C::kWr != wr) continue;
           const int64_t off = kb[kk] + (2 * t + (x & 1) + (x >> 1) * 8) * D + g * (D / 8);
-          const int s = D / 16 + kk * 4 + x;   // in units of 512 bytes (D = 128) or 256 (D = 64)
-          if constexpr (D == 128) cp_async16(dst + s * 512, c.v_codes + off);
-          else cp_async8(smem_u32(ring + stage * C::kStage) + 4 * 512 + (kk * 4 + x) * 256 + lane * 8, c.v_codes + off);
+          if constexpr (D == 128) cp_async16(dst + (D / 16 + kk * 4 + x) * 512, c.v_codes + off);
+          else cp_async8(at + 4 * 512 + (kk * 4 + x) * 256 + lane * 8, c.v_codes + off);
         }
-      if (lane < 4) {
-        const float* sc = (lane < 2 ? c.k_scale : c.v_scale) + (int64_t)((lane & 1) ? id[1] : id[0]) * c.kv_heads + ph;
-        cp_async4(smem_u32(ring + stage * C::kStage) + C::kSlots * 512 + lane * 4, sc);
+      if (lane < 4 && wr == 0) {
+        const float* sc = (lane < 2 ? c.k_scale : c.v_scale) + (int64_t)((lane & 1) ? n_id[1] : n_id[0]) * c.kv_heads + n_head;
+        cp_async4(at + C::kSlots * 512 + lane * 4, sc);
       }
     }
-    pu += kDecWarps;
     cp_commit();
   };
+  look_up();
 #pragma unroll
-  for (int s = 0; s < C::kStages - 1; ++s) issue(s);
+  for (int s = 0; s < C::kStages - 1; ++s) {
+    issue(s);
+    look_up();
+  }
 
-  uint32_t qf[MT][KS][4];
-  float qs[MT][2];                          // row factor: scale * log2(e) / the power of two q was multiplied by
-  int lim[MT][2];                           // tokens the row may see
-  float o[MT][NT][4], m[MT][2], l[MT][2];   // m: running maximum - kPShift, l: this lane's part of the sum
+  uint32_t qf[KS][4];
+  float qs[2];                         // row factor: scale * log2(e) / the power of two q was multiplied by
+  int lim[2];                          // tokens the row may see
+  float o[NT][4], m[2], l[2];   // m: running maximum - kPShift, l: this lane's part of the sum
   int stage = 0;
-  int64_t cu = u0 + warp;                   // this warp's next unit
+  int64_t cu = u0 + team;                   // this team's next unit
   int64_t seg0 = u0;                        // current segment: units [seg0, seg1) of (b, h)
   int64_t seg_first = u0 - unit0;           // flat index of (b, h)'s unit 0
 
@@ -228,72 +255,72 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv8_attn_kernel(const __grid_c
     const int len = kv8_len(c, p.lens[b]);
     // query fragments and row state
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
+    for (int hf = 0; hf < 2; ++hf) {
+      m[hf] = -INFINITY;
+      l[hf] = 0.f;
+      const int r = row0 + hf * 8 + g;
+      const bool live = r < p.rows && (kUpper || hf == 0);
+      float f[D / 4];
+      float top = 0.f;
+      const int i_tok = r / p.group, head = h * p.group + r % p.group;
+      lim[hf] = live ? len - p.T + i_tok + 1 : 0;
+      const T* src = static_cast<const T*>(p.q) + b * p.q_sb + i_tok * p.q_st + head * p.q_sh;
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        m[mt][hf] = -INFINITY;
-        l[mt][hf] = 0.f;
-        const int r = row0 + mt * 16 + hf * 8 + g;
-        const bool live = r < p.rows && (kUpper || hf == 0);
-        float f[D / 4];
-        float top = 0.f;
-        const int i_tok = r / p.group, head = h * p.group + r % p.group;
-        lim[mt][hf] = live ? len - p.T + i_tok + 1 : 0;
-        const T* src = static_cast<const T*>(p.q) + b * p.q_sb + i_tok * p.q_st + head * p.q_sh;
+      for (int i = 0; i < D / 64; ++i)
 #pragma unroll
-        for (int i = 0; i < D / 64; ++i)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) f[i * 16 + e] = 0.f;
-        if (live) {
-#pragma unroll
-          for (int i = 0; i < D / 64; ++i)
-#pragma unroll
-            for (int v = 0; v < 2; ++v) {
-              const uint4 w = *reinterpret_cast<const uint4*>(src + i * 64 + t * 16 + v * 8);
-              const T* e = reinterpret_cast<const T*>(&w);
-#pragma unroll
-              for (int k = 0; k < 8; ++k) f[i * 16 + v * 8 + k] = to_f32(e[k]);
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < D / 4; ++e) top = fmaxf(top, fabsf(f[e]));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // 2^k that brings the row's largest value to [2^14, 2^15)
-        int k = 14 - ((int)(__float_as_uint(top) >> 23) - 127);
-        k = max(-100, min(100, k));
-        const float up = __uint_as_float((uint32_t)(k + 127) << 23);
-        qs[mt][hf] = p.scale_log2 * __uint_as_float((uint32_t)(127 - k) << 23);
+        for (int e = 0; e < 16; ++e) f[i * 16 + e] = 0.f;
+      if (live) {
 #pragma unroll
         for (int i = 0; i < D / 64; ++i)
 #pragma unroll
-          for (int w = 0; w < 4; ++w)
+          for (int v = 0; v < 2; ++v) {
+            const uint4 w = *reinterpret_cast<const uint4*>(src + i * 64 + t * 16 + v * 8);
+            const T* e = reinterpret_cast<const T*>(&w);
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
-              qf[mt][i * 4 + w][hf + 2 * x] =
-                  pack_f16x2(f[i * 16 + w * 4 + x * 2] * up, f[i * 16 + w * 4 + x * 2 + 1] * up);
+            for (int k = 0; k < 8; ++k) f[i * 16 + v * 8 + k] = to_f32(e[k]);
+          }
       }
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int e = 0; e < D / 4; ++e) top = fmaxf(top, fabsf(f[e]));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^k that brings the row's largest value to [2^14, 2^15)
+      int k = 14 - ((int)(__float_as_uint(top) >> 23) - 127);
+      k = max(-100, min(100, k));
+      const float up = __uint_as_float((uint32_t)(k + 127) << 23);
+      qs[hf] = p.scale_log2 * __uint_as_float((uint32_t)(127 - k) << 23);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[mt][n][e] = 0.f;
+      for (int i = 0; i < D / 64; ++i)
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            qf[i * 4 + w][hf + 2 * x] =
+                pack_f16x2(f[i * 16 + w * 4 + x * 2] * up, f[i * 16 + w * 4 + x * 2 + 1] * up);
     }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
 
-    for (; cu < seg1; cu += kDecWarps) {
+    for (; cu < seg1; cu += C::kTeams) {
       cp_wait<C::kStages - 2>();
-      __syncwarp();                          // the scales come from other lanes' copies
+      // the other lanes' copies (the scales) and the other warps' are in, and
+      // everyone is done with the stage that is filled next
+      if constexpr (C::kWr == 1) __syncwarp();
+      else named_barrier(1 + team, C::kWr * 32);
+      issue(stage == 0 ? C::kStages - 1 : stage - 1);
+      look_up();
       const uint8_t* st = ring + stage * C::kStage;
       const float* sc = reinterpret_cast<const float*>(st + C::kSlots * 512);
       const float ks[2] = {sc[0], sc[1]}, vs[2] = {sc[2], sc[3]};
       const int tok0 = (int)(cu - seg_first) * kUnit;
       // scores
-      float s[MT][4][4];
+      float s[4][4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[mt][j][e] = 0.f;
+        for (int e = 0; e < 4; ++e) s[j][e] = 0.f;
 #pragma unroll
         for (int i = 0; i < D / 64; ++i) {
           const uint4 kw = *reinterpret_cast<const uint4*>(st + (j * (D / 64) + i) * 512 + lane * 16);
@@ -301,9 +328,7 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv8_attn_kernel(const __grid_c
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
             const uint32_t bi = w4[w] ^ 0x80808080u;
-            const uint32_t b0 = codes_f16x2(bi, 0x4140), b1 = codes_f16x2(bi, 0x4342);
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) mma_f16(s[mt][j], qf[mt][i * 4 + w], b0, b1);
+            mma_f16(s[j], qf[i * 4 + w], codes_f16x2(bi, 0x4140), codes_f16x2(bi, 0x4342));
           }
         }
       }
@@ -316,62 +341,59 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv8_attn_kernel(const __grid_c
         vi[i] = __uint_as_float((uint32_t)(127 - e) << 23);   // 2^-e
         vf[i] = vs[i] * vi[i];
       }
-      uint32_t pa[MT][2][4];
+      uint32_t pa[2][4];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
+      for (int hf = 0; hf < kHalves; ++hf) {
+        float x[4][2];
+        float top = -INFINITY;
+        const int r = row0 + hf * 8 + g;
 #pragma unroll
-        for (int hf = 0; hf < kHalves; ++hf) {
-          float x[4][2];
-          float top = -INFINITY;
-          const int r = row0 + mt * 16 + hf * 8 + g;
+        for (int j = 0; j < 4; ++j) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int tok = tok0 + j * 8 + 2 * t + e;
-              const float v = s[mt][j][hf * 2 + e] * (ks[j >> 1] * qs[mt][hf]);
-              s[mt][j][hf * 2 + e] = v;
-              x[j][e] = tok < lim[mt][hf] ? v + ve[j >> 1] : -INFINITY;
-              top = fmaxf(top, x[j][e]);
-            }
-          }
-          if (p.scores && r < p.rows) {
-            float* dst = p.scores + (((int64_t)b * c.kv_heads + h) * p.rows + r) * p.score_cap + tok0 + 2 * t;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              *reinterpret_cast<float2*>(dst + j * 8) = make_float2(s[mt][j][hf * 2], s[mt][j][hf * 2 + 1]);
-          }
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          const float mn = fmaxf(m[mt][hf], top - kPShift);
-          const float base = mn == -INFINITY ? 0.f : mn;            // nothing seen yet: every term is exp2(-inf)
-          const float alpha = mn == -INFINITY ? 1.f : exp2f(m[mt][hf] - mn);
-          m[mt][hf] = mn;
-          float sum = 0.f;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            float pv[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float ex = exp2f(x[j][e] - base);
-              sum = fmaf(ex, vi[j >> 1], sum);
-              pv[e] = ex > 0.f ? ex * vf[j >> 1] : 0.f;   // a masked token's page scale does not matter
-            }
-            pa[mt][j >> 1][(j & 1) * 2 + hf] = pack_f16x2(pv[0], pv[1]);
-          }
-          l[mt][hf] = fmaf(l[mt][hf], alpha, sum);
-          if (alpha != 1.f) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              o[mt][n][hf * 2] *= alpha;
-              o[mt][n][hf * 2 + 1] *= alpha;
-            }
+          for (int e = 0; e < 2; ++e) {
+            const int tok = tok0 + j * 8 + 2 * t + e;
+            const float v = s[j][hf * 2 + e] * (ks[j >> 1] * qs[hf]);
+            s[j][hf * 2 + e] = v;
+            x[j][e] = tok < lim[hf] ? v + ve[j >> 1] : -INFINITY;
+            top = fmaxf(top, x[j][e]);
           }
         }
-        if constexpr (!kUpper) {
+        if (p.scores && r < p.rows) {
+          float* dst = p.scores + (((int64_t)b * c.kv_heads + h) * p.rows + r) * p.score_cap + tok0 + 2 * t;
 #pragma unroll
-          for (int kk = 0; kk < 2; ++kk) pa[mt][kk][1] = pa[mt][kk][3] = 0u;
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<float2*>(dst + j * 8) = make_float2(s[j][hf * 2], s[j][hf * 2 + 1]);
         }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float mn = fmaxf(m[hf], top - kPShift);
+        const float base = mn == -INFINITY ? 0.f : mn;            // nothing seen yet: every term is exp2(-inf)
+        const float alpha = mn == -INFINITY ? 1.f : exp2f(m[hf] - mn);
+        m[hf] = mn;
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float pv[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float ex = exp2f(x[j][e] - base);
+            sum = fmaf(ex, vi[j >> 1], sum);
+            pv[e] = ex > 0.f ? ex * vf[j >> 1] : 0.f;   // a masked token's page scale does not matter
+          }
+          pa[j >> 1][(j & 1) * 2 + hf] = pack_f16x2(pv[0], pv[1]);
+        }
+        l[hf] = fmaf(l[hf], alpha, sum);
+        if (alpha != 1.f) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            o[n][hf * 2] *= alpha;
+            o[n][hf * 2 + 1] *= alpha;
+          }
+        }
+      }
+      if constexpr (!kUpper) {
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) pa[kk][1] = pa[kk][3] = 0u;
       }
       // values
 #pragma unroll
@@ -401,78 +423,69 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv8_attn_kernel(const __grid_c
           for (int e = 0; e < 4; ++e) {
             const uint32_t b0 = codes_f16x2(e < 2 ? a_lo : a_hi, (e & 1) ? 0x4342 : 0x4140);
             const uint32_t b1 = codes_f16x2(e < 2 ? c_lo : c_hi, (e & 1) ? 0x4342 : 0x4140);
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) mma_f16(o[mt][w * 4 + e], pa[mt][kk], b0, b1);
+            mma_f16(o[w * 4 + e], pa[kk], b0, b1);
           }
         }
       }
-      __syncwarp();                          // the stage's scales have been read by every lane
-      issue((stage + C::kStages - 1) % C::kStages);
       stage = stage + 1 == C::kStages ? 0 : stage + 1;
     }
 
-    // Join the warps' partials of this segment: warp 3 hands its own to warp
-    // 2, that one the sum to warp 1 and so on, lane by lane (every lane
-    // writes and reads the same 16-byte places, so no bank conflicts and one
-    // buffer); warp 0 stores the segment's partial in its slot.
+    // Join the teams' partials of this segment: the last team hands its own
+    // to the one before, that one the sum to the one before it and so on,
+    // lane by lane (every lane writes and reads the same 16-byte places, so
+    // no bank conflicts and one buffer); team 0 stores the segment's partial
+    // in its slot.
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int hf = 0; hf < kHalves; ++hf) {
-        l[mt][hf] += __shfl_xor_sync(0xffffffffu, l[mt][hf], 1);
-        l[mt][hf] += __shfl_xor_sync(0xffffffffu, l[mt][hf], 2);
-      }
+    for (int hf = 0; hf < kHalves; ++hf) {
+      l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 1);
+      l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 2);
+    }
 #pragma unroll 1
-    for (int w = kDecWarps - 1; w >= 0; --w) {
-      if (warp == w) {
+    for (int w = C::kTeams - 1; w >= 0; --w) {
+      if (team == w) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int hf = 0; hf < kHalves; ++hf) {
+          if (w < C::kTeams - 1) {
+            const float2 ml = comb_ml[hf * 32 + lane];
+            const float mx = fmaxf(m[hf], ml.x);
+            const float fa = l[hf] == 0.f ? 0.f : exp2f(m[hf] - mx);
+            const float fb = ml.y == 0.f ? 0.f : exp2f(ml.x - mx);
+            l[hf] = l[hf] * fa + ml.y * fb;
+            m[hf] = mx;
 #pragma unroll
-          for (int hf = 0; hf < kHalves; ++hf) {
-            const int pl = mt * kHalves + hf;
-            if (w < kDecWarps - 1) {
-              const float2 ml = comb_ml[pl * 32 + lane];
-              const float mx = fmaxf(m[mt][hf], ml.x);
-              const float fa = l[mt][hf] == 0.f ? 0.f : exp2f(m[mt][hf] - mx);
-              const float fb = ml.y == 0.f ? 0.f : exp2f(ml.x - mx);
-              l[mt][hf] = l[mt][hf] * fa + ml.y * fb;
-              m[mt][hf] = mx;
-#pragma unroll
-              for (int n = 0; n < NT / 2; ++n) {
-                const float4 v = comb[(pl * (NT / 2) + n) * 32 + lane];
-                o[mt][2 * n][hf * 2] = fmaf(v.x, fb, o[mt][2 * n][hf * 2] * fa);
-                o[mt][2 * n][hf * 2 + 1] = fmaf(v.y, fb, o[mt][2 * n][hf * 2 + 1] * fa);
-                o[mt][2 * n + 1][hf * 2] = fmaf(v.z, fb, o[mt][2 * n + 1][hf * 2] * fa);
-                o[mt][2 * n + 1][hf * 2 + 1] = fmaf(v.w, fb, o[mt][2 * n + 1][hf * 2 + 1] * fa);
-              }
-            }
-            if (w > 0) {
-              comb_ml[pl * 32 + lane] = make_float2(m[mt][hf], l[mt][hf]);
-#pragma unroll
-              for (int n = 0; n < NT / 2; ++n)
-                comb[(pl * (NT / 2) + n) * 32 + lane] =
-                    make_float4(o[mt][2 * n][hf * 2], o[mt][2 * n][hf * 2 + 1], o[mt][2 * n + 1][hf * 2],
-                                o[mt][2 * n + 1][hf * 2 + 1]);
-            } else {
-              const int r = mt * 16 + hf * 8 + g;
-              if (row0 + r < p.rows) {
-                const int slot = b * c.kv_heads + h + blockIdx.x;
-                const int64_t at = ((int64_t)blockIdx.y * p.slots + slot) * RB + r;
-                if (t == 0) p.part_ml[at] = make_float2(m[mt][hf], l[mt][hf]);
-                // column n of value tile i is value column (D / 8) n + i
-                float* dst = p.part_o + at * D + (D / 8) * 2 * t;
-#pragma unroll
-                for (int x = 0; x < 2; ++x)
-#pragma unroll
-                  for (int n = 0; n < NT; n += 4)
-                    *reinterpret_cast<float4*>(dst + x * (D / 8) + n) =
-                        make_float4(o[mt][n][hf * 2 + x], o[mt][n + 1][hf * 2 + x], o[mt][n + 2][hf * 2 + x],
-                                    o[mt][n + 3][hf * 2 + x]);
-              }
+            for (int n = 0; n < NT / 2; ++n) {
+              const float4 v = comb[(hf * (NT / 2) + n) * 32 + lane];
+              o[2 * n][hf * 2] = fmaf(v.x, fb, o[2 * n][hf * 2] * fa);
+              o[2 * n][hf * 2 + 1] = fmaf(v.y, fb, o[2 * n][hf * 2 + 1] * fa);
+              o[2 * n + 1][hf * 2] = fmaf(v.z, fb, o[2 * n + 1][hf * 2] * fa);
+              o[2 * n + 1][hf * 2 + 1] = fmaf(v.w, fb, o[2 * n + 1][hf * 2 + 1] * fa);
             }
           }
+          if (w > 0) {
+            comb_ml[hf * 32 + lane] = make_float2(m[hf], l[hf]);
+#pragma unroll
+            for (int n = 0; n < NT / 2; ++n)
+              comb[(hf * (NT / 2) + n) * 32 + lane] = make_float4(o[2 * n][hf * 2], o[2 * n][hf * 2 + 1],
+                                                                  o[2 * n + 1][hf * 2], o[2 * n + 1][hf * 2 + 1]);
+          } else {
+            const int r = hf * 8 + g;
+            if (row0 + r < p.rows) {
+              const int64_t slot = (int64_t)blockIdx.y * p.slots + b * c.kv_heads + h + blockIdx.x;
+              const int64_t at = slot * RB + wr * C::kWarpRows + r;
+              if (t == 0) p.part_ml[at] = make_float2(m[hf], l[hf]);
+              // column n of value tile i is value column (D / 8) n + i
+              float* dst = p.part_o + at * D + (D / 8) * 2 * t;
+#pragma unroll
+              for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int n = 0; n < NT; n += 4)
+                  *reinterpret_cast<float4*>(dst + x * (D / 8) + n) = make_float4(
+                      o[n][hf * 2 + x], o[n + 1][hf * 2 + x], o[n + 2][hf * 2 + x], o[n + 3][hf * 2 + x]);
+            }
+          }
+        }
       }
-      if (w > 0) __syncthreads();
+      if constexpr (C::kTeams > 1) __syncthreads();   // the next team may read, or the next segment write
     }
     // next (sequence, head) with units
     seg0 = seg1;
@@ -488,9 +501,12 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv8_attn_kernel(const __grid_c
   cp_wait<0>();
 }
 
-// Second kernel: grid (B * kv_heads, 1 + weight chunks).  Block y = 0 joins
-// the partials of one (sequence, head) and stores the output; the others
-// turn the scores of kJoinTokens tokens into weights.
+// Second kernel: grid (B * kv_heads, output blocks + weight blocks).  An
+// output block joins the partials of a few rows of one (sequence, head),
+// `lanes` threads taking every lanes-th partial of the same four columns (a
+// long sequence has one partial per CTA of the first kernel, and reading
+// them one after the other would cost more than the attention); a weight
+// block turns the scores of kJoinTokens tokens into weights.
 constexpr int kJoinTokens = 1024;
 constexpr int kJoinThreads = 256;
 constexpr int kMaxRows = 512;
@@ -498,77 +514,116 @@ constexpr int kMaxRows = 512;
 template <typename T, int D, int RB>
 __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const __grid_constant__ DecodeParams p) {
   __shared__ float2 s_ml[kMaxRows];           // (M - kPShift, 1 / sum) per row; 1 / sum = 0: the row sees nothing
+  __shared__ float4 s_part[kJoinThreads];
+  constexpr int kCols = D / 4;                // threads across a row
   const Kv8View& c = p.c;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int bh = blockIdx.x, b = bh / c.kv_heads, h = bh - b * c.kv_heads;
-  // lens and the page table are the caller's; the partials are the first kernel's
+  const int64_t tok0 = (int64_t)((int)blockIdx.y - p.out_blocks) * kJoinTokens;
+  const int len = kv8_len(c, p.lens[b]);
+  if (tok0 >= len && tok0 >= 0) return;
+  // the CTAs of the first kernel that hold partials of (b, h): c0 .. c1
   int64_t total;
   const int64_t per = units_per_cta(p, &total);
   int64_t before = 0;
-  for (int i = threadIdx.x & 31; i < b; i += 32) before += seq_units(p, i);
+  for (int i = lane; i < b; i += 32) before += seq_units(p, i);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
   const int64_t su = seq_units(p, b), ub = before * c.kv_heads + h * su;
-  const int c0 = (int)(ub / per), c1 = su ? (int)((ub + su - 1) / per) : c0 - 1;   // CTAs that hold parts
-  const int len = kv8_len(c, p.lens[b]);
-  const int64_t tok0 = (int64_t)(blockIdx.y - 1) * kJoinTokens;
-  if (blockIdx.y > 0 && tok0 >= len) return;
+  const int c0 = (int)(ub / per), c1 = su ? (int)((ub + su - 1) / per) : c0 - 1;
+  // rows whose statistics this block needs
+  const int per_block = kJoinThreads / kCols / p.lanes;
+  const int ra = tok0 < 0 ? blockIdx.y * per_block : 0, rz = tok0 < 0 ? min(p.rows, ra + per_block) : p.rows;
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
-  for (int r = threadIdx.x; r < p.rows; r += kJoinThreads) {
-    const int64_t at = ((int64_t)(r / RB) * p.slots + bh) * RB + r % RB;
+  for (int r = ra + warp; r < rz; r += kJoinThreads / 32) {
+    const float2* ml = p.part_ml + ((int64_t)(r / RB) * p.slots + bh) * RB + r % RB;
     float mx = -INFINITY, sum = 0.f;
-    for (int i = c0; i <= c1; ++i) mx = fmaxf(mx, p.part_ml[at + (int64_t)i * RB].x);
-    for (int i = c0; i <= c1; ++i) {
-      const float2 ml = p.part_ml[at + (int64_t)i * RB];
-      if (ml.y != 0.f) sum = fmaf(ml.y, exp2f(ml.x - mx), sum);
+    for (int i = c0 + lane; i <= c1; i += 32) {
+      const float2 v = ml[(int64_t)i * RB];
+      if (v.y == 0.f) continue;
+      const float m = fmaxf(mx, v.x);
+      sum = (sum == 0.f ? 0.f : sum * exp2f(mx - m)) + v.y * exp2f(v.x - m);
+      mx = m;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float om = __shfl_xor_sync(0xffffffffu, mx, o), os = __shfl_xor_sync(0xffffffffu, sum, o);
+      const float m = fmaxf(mx, om);
+      sum = (sum == 0.f ? 0.f : sum * exp2f(mx - m)) + (os == 0.f ? 0.f : os * exp2f(om - m));
+      mx = m;
     }
     // a sum that is NaN (a page scale that is not finite) stays NaN
-    s_ml[r] = make_float2(mx, sum == 0.f ? 0.f : 1.f / sum);
+    if (lane == 0) s_ml[r] = make_float2(mx, sum == 0.f ? 0.f : 1.f / sum);
   }
   __syncthreads();
-  if (blockIdx.y == 0) {
-    for (int e = threadIdx.x; e < p.rows * (D / 4); e += kJoinThreads) {
-      const int r = e / (D / 4), d = (e - r * (D / 4)) * 4;
+  if (tok0 < 0) {
+    const int col = threadIdx.x % kCols, rest = threadIdx.x / kCols, part = rest % p.lanes, r = ra + rest / p.lanes;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (r < rz) {
       const int64_t at = ((int64_t)(r / RB) * p.slots + bh) * RB + r % RB;
-      const float2 row = s_ml[r];
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int i = c0; i <= c1; ++i) {
+      const float mx = s_ml[r].x;
+#pragma unroll 4
+      for (int i = c0 + part; i <= c1; i += p.lanes) {
         const float2 ml = p.part_ml[at + (int64_t)i * RB];
-        if (ml.y == 0.f) continue;
-        const float f = exp2f(ml.x - row.x);
-        const float4 v = *reinterpret_cast<const float4*>(p.part_o + (at + (int64_t)i * RB) * D + d);
+        const float4 v = *reinterpret_cast<const float4*>(p.part_o + (at + (int64_t)i * RB) * D + col * 4);
+        const float f = ml.y == 0.f ? 0.f : exp2f(ml.x - mx);
         acc.x = fmaf(v.x, f, acc.x);
         acc.y = fmaf(v.y, f, acc.y);
         acc.z = fmaf(v.z, f, acc.z);
         acc.w = fmaf(v.w, f, acc.w);
       }
-      T* dst = static_cast<T*>(p.out) + (((int64_t)b * p.T + r / p.group) * p.heads + h * p.group + r % p.group) * D + d;
-      dst[0] = from_out<T>(acc.x * row.y);
-      dst[1] = from_out<T>(acc.y * row.y);
-      dst[2] = from_out<T>(acc.z * row.y);
-      dst[3] = from_out<T>(acc.w * row.y);
+    }
+    if (p.lanes > 1) {
+      s_part[threadIdx.x] = acc;
+      __syncthreads();
+      if (part == 0)
+        for (int i = 1; i < p.lanes; ++i) {
+          const float4 v = s_part[threadIdx.x + i * kCols];
+          acc.x += v.x;
+          acc.y += v.y;
+          acc.z += v.z;
+          acc.w += v.w;
+        }
+    }
+    if (part == 0 && r < rz) {
+      const float inv = s_ml[r].y;
+      T* dst = static_cast<T*>(p.out) + (((int64_t)b * p.T + r / p.group) * p.heads + h * p.group + r % p.group) * D + col * 4;
+      const T o[4] = {from_f32<T>(acc.x * inv), from_f32<T>(acc.y * inv), from_f32<T>(acc.z * inv),
+                      from_f32<T>(acc.w * inv)};
+      *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(o);
     }
     return;
   }
-  const int64_t end = min((int64_t)len, tok0 + kJoinTokens);
-  for (int64_t t = tok0 + threadIdx.x; t < end; t += kJoinThreads) {
-    const float* s = p.scores + (int64_t)bh * p.rows * p.score_cap + t;
-    float mass = 0.f;
-    for (int r = 0; r < p.rows; ++r) {
-      const float2 row = s_ml[r];
-      if (t < len - p.T + r / p.group + 1 && row.y != 0.f)
-        mass = fmaf(exp2f(s[(int64_t)r * p.score_cap] - row.x), row.y, mass);
-    }
-    const int64_t at = (int64_t)bh * p.cap + t;
-    p.weights_out[at] = p.weights[at] + mass;
+  // four tokens per thread; a masked or padded score is never used
+  const int64_t tok = tok0 + threadIdx.x * 4;
+  if (tok >= len) return;
+  const float* s = p.scores + (int64_t)bh * p.rows * p.score_cap + tok;
+  float mass[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int r = 0; r < p.rows; ++r) {
+    const float4 v = *reinterpret_cast<const float4*>(s + (int64_t)r * p.score_cap);
+    const float2 row = s_ml[r];
+    const int see = row.y == 0.f ? 0 : len - p.T + r / p.group + 1;
+    const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (tok + e < see) mass[e] = fmaf(exp2f(x[e] - row.x), row.y, mass[e]);
   }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (tok + e < len) {
+      const int64_t at = (int64_t)bh * p.cap + tok + e;
+      p.weights_out[at] = p.weights[at] + mass[e];
+    }
 }
 
 // ---------------------------------------------------------------------------
 // launches
 // ---------------------------------------------------------------------------
-static int row_block(int rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
-static int decode_ctas_per_sm(int dim, int rb) { return rb == 32 ? 1 : 2; }
+// Rows per CTA; beyond 64 the cache is read once for each 64.
+static int row_block(int rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+constexpr int kDecodeCtasPerSm = 2;
 
 static int sm_count() {
   int dev = 0, n = 0;
@@ -582,12 +637,17 @@ static void decode_plan(DecodeParams& p, size_t* bytes) {
   const int rb = row_block(p.rows), blocks = (p.rows + rb - 1) / rb;
   const int64_t cap_units = (((int64_t)p.c.table_width << p.c.page_shift) + kUnit - 1) / kUnit;
   const int64_t most = (cap_units * p.B * p.c.kv_heads + kMinUnits - 1) / kMinUnits;
-  int64_t ctas = (int64_t)sm_count() * decode_ctas_per_sm(p.c.dim, rb);
+  int64_t ctas = (int64_t)sm_count() * kDecodeCtasPerSm;
   ctas = (ctas + blocks - 1) / blocks;
   p.ctas = (int)(most < ctas ? most : ctas);
   if (p.ctas < 1) p.ctas = 1;
   p.slots = p.B * p.c.kv_heads + p.ctas;
   p.score_cap = cap_units * kUnit;
+  // a (sequence, head) has about ctas / (B * kv_heads) partials
+  p.lanes = 1;
+  while (p.lanes < 8 && p.lanes * p.B * p.c.kv_heads * 2 <= p.ctas) p.lanes *= 2;
+  const int per_block = kJoinThreads / (p.c.dim / 4) / p.lanes;
+  p.out_blocks = (p.rows + per_block - 1) / per_block;
   const size_t part_rows = (size_t)blocks * p.slots * rb;
   uint8_t* w = reinterpret_cast<uint8_t*>(p.part_o);
   auto al = [](size_t x) { return (x + 255) & ~(size_t)255; };
@@ -618,7 +678,7 @@ size_t kv8_attn_workspace(const Kv8View& c, int B, int T, int heads, int with_we
 
 template <typename T, int D, int RB>
 static cudaError_t launch_decode(const DecodeParams& p, cudaStream_t st) {
-  using C = DecodeTile<T, D, RB>;
+  using C = DecodeTile<D, RB>;
   cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(kv8_attn_kernel<T, D, RB>), C::kSmem);
   if (e != cudaSuccess) return e;
   const int blocks = (p.rows + RB - 1) / RB;
@@ -627,7 +687,7 @@ static cudaError_t launch_decode(const DecodeParams& p, cudaStream_t st) {
   const int64_t cap = (int64_t)p.c.table_width << p.c.page_shift;
   const int64_t chunks = p.weights ? (cap + kJoinTokens - 1) / kJoinTokens : 0;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(p.B * p.c.kv_heads), (unsigned)(1 + chunks));
+  cfg.gridDim = dim3((unsigned)(p.B * p.c.kv_heads), (unsigned)(p.out_blocks + chunks));
   cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
@@ -642,8 +702,14 @@ template <typename T>
 static cudaError_t launch_decode_dim(const DecodeParams& p, cudaStream_t st) {
   const int rb = row_block(p.rows);
   if (p.c.dim == 128)
-    return rb == 8 ? launch_decode<T, 128, 8>(p, st) : rb == 16 ? launch_decode<T, 128, 16>(p, st) : launch_decode<T, 128, 32>(p, st);
-  return rb == 8 ? launch_decode<T, 64, 8>(p, st) : rb == 16 ? launch_decode<T, 64, 16>(p, st) : launch_decode<T, 64, 32>(p, st);
+    return rb == 8    ? launch_decode<T, 128, 8>(p, st)
+           : rb == 16 ? launch_decode<T, 128, 16>(p, st)
+           : rb == 32 ? launch_decode<T, 128, 32>(p, st)
+                      : launch_decode<T, 128, 64>(p, st);
+  return rb == 8    ? launch_decode<T, 64, 8>(p, st)
+         : rb == 16 ? launch_decode<T, 64, 16>(p, st)
+         : rb == 32 ? launch_decode<T, 64, 32>(p, st)
+                    : launch_decode<T, 64, 64>(p, st);
 }
 
 cudaError_t launch_kv8_attn(const Kv8View& c, const void* q, int dtype, const int64_t* strides, int B, int T, int heads,

@@ -208,6 +208,31 @@ def test_kv8_attention(heads, kv_heads, dim, T, page, dtype):
         assert torch.equal(w_in[b, :, n:], w[b, :, n:])
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("page", [16, 128])
+@pytest.mark.parametrize("heads,kv_heads,dim,T", [(14, 2, 128, 16), (5, 1, 64, 7), (5, 1, 128, 5), (16, 1, 64, 16),
+                                                  (3, 1, 128, 3), (28, 4, 128, 8)])
+def test_kv8_attention_many_rows(heads, kv_heads, dim, T, page, dtype):
+    # up to 256 rows a KV head; an output below 2^-14 rounds to a multiple of fp16's 2^-24
+    import alpamayo_b200.ops as ops
+    lens = [16 + T, 1 + T, 300, 129, 32, 1000]
+    *cache, table = R.make_pool(lens, page, kv_heads, dim, 11)
+    q = (torch.randn(len(lens), T, heads, dim, generator=torch.Generator().manual_seed(12)) * 1.5).to(dtype).cuda()
+    w = torch.zeros(len(lens), kv_heads, table.shape[1] * page, device="cuda")
+    out = ops.attention_kv8(q, *cache, table, R.i32(lens), None, w)
+    for b, n in enumerate(lens):
+        k = torch.stack([R.read(cache, 0, table, b, h, n) for h in range(kv_heads)], 1)
+        v = torch.stack([R.read(cache, 1, table, b, h, n) for h in range(kv_heads)], 1)
+        ref, p, size, sb = R.attend(q[b].double().cpu(), k, v, dim ** -0.5)
+        bound = R.out_bound(ref, size, sb, dtype, 2.0 ** -11) + (2.0 ** -25 if dtype == F16 else 0.0)
+        assert R.max_excess(out[b], ref, bound) <= 1.0, (b, n)
+        mass = p.view(kv_heads, heads // kv_heads, T, n).sum((1, 2))
+        err = (p * (2.0 * sb[..., None] + 2.0 ** -18)).view(kv_heads, heads // kv_heads, T, n).sum((1, 2))
+        got = w[b, :, :n].double().cpu()
+        assert ((got - mass).abs() <= err + mass * 2.0 ** -20 + 1e-30).all(), (b, n)
+        assert (w[b, :, n:] == 0).all()
+
+
 def test_kv8_attention_lengths_zero_and_shorter_than_the_new_tokens():
     import alpamayo_b200.ops as ops
     lens, T = [0, 2, 5, 40], 5
