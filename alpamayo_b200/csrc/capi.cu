@@ -825,7 +825,8 @@ size_t paro_attention_kv8_workspace_size(const paro_kv8_cache* cache, int table_
                                          int with_weights) {
   Kv8View c;
   if (kv8_view(cache, reinterpret_cast<const int32_t*>(16), table_width, B, &c) || B <= 0 || T <= 0 || heads <= 0 ||
-      heads % c.kv_heads || (int64_t)T * (heads / c.kv_heads) > kv8_attn_max_rows())
+      heads % c.kv_heads || (int64_t)T * (heads / c.kv_heads) > kv8_attn_max_rows() ||
+      (int64_t)table_width * c_page(c) / 16 * B >= 0x7FFFFFFF / c.kv_heads)
     return 0;
   return kv8_attn_workspace(c, B, T, heads, with_weights);
 }
@@ -895,6 +896,8 @@ int paro_attention_kv8(const paro_kv8_cache* cache, const int32_t* page_table, i
   if ((int64_t)T * (heads / c.kv_heads) > kv8_attn_max_rows()) return PARO_ERR_TOO_LARGE;
   if (!q || !strides || !lens || !out || !workspace || !weights != !weights_out) return PARO_ERR_INVALID_ARGUMENT;
   if (weights && cap < (int64_t)table_width * c_page(c)) return PARO_ERR_SHAPE;
+  // pieces of 32 tokens of all sequences and heads are counted in 31 bits
+  if ((int64_t)table_width * c_page(c) / 16 * B >= 0x7FFFFFFF / c.kv_heads) return PARO_ERR_TOO_LARGE;
   if (!aligned(q, 16) || !aligned(out, 16) || !aligned(workspace, 256)) return PARO_ERR_MISALIGNED;
   for (int i = 0; i < 3; ++i)
     if (strides[i] < 0 || strides[i] % 8) return PARO_ERR_MISALIGNED;

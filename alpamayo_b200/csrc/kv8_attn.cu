@@ -95,28 +95,54 @@ __device__ __forceinline__ uint32_t codes_f16x2(uint32_t biased, uint32_t sel) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// units of sequence b per KV head
-__device__ __forceinline__ int64_t seq_units(const DecodeParams& p, int b) {
-  const int64_t cap = (int64_t)p.c.table_width << p.c.page_shift;
-  const int64_t len = max((int64_t)0, min((int64_t)p.lens[b], cap));
-  return (len + kUnit - 1) / kUnit;
+// Units of sequence b per KV head.  All sequences' units together fit 31
+// bits (the launch refuses more).
+__device__ __forceinline__ int seq_units(const DecodeParams& p, int b) {
+  const int cap = p.c.table_width << p.c.page_shift;
+  return (int)(((unsigned)max(0, min(p.lens[b], cap)) + kUnit - 1) / kUnit);
 }
 
-// Units of all sequences together, and per CTA.
-__device__ __forceinline__ int64_t units_per_cta(const DecodeParams& p, int64_t* total) {
+// Units per CTA; *total: units of all sequences and heads.
+__device__ __forceinline__ int units_per_cta(const DecodeParams& p, int* total) {
+  int u = 0;
+  for (int b = threadIdx.x & 31; b < p.B; b += 32) u += seq_units(p, b);
+  u = __reduce_add_sync(0xffffffffu, u) * p.c.kv_heads;
+  *total = u;
+  return max(kMinUnits, (u + p.ctas - 1) / p.ctas);
+}
+
+// The sequence that unit `u` lies in; *first: the sequence's first unit.
+// All lanes of a warp call it, with u inside the total.
+__device__ __forceinline__ int find_unit(const DecodeParams& p, int u, int* first) {
   const int lane = threadIdx.x & 31;
-  int64_t u = 0;
-  for (int b = lane; b < p.B; b += 32) u += seq_units(p, b);
+  int before = 0;
+  for (int b0 = 0;; b0 += 32) {
+    const int mine = b0 + lane < p.B ? seq_units(p, b0 + lane) * p.c.kv_heads : 0;
+    int incl = mine;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
-  *total = u * p.c.kv_heads;
-  const int64_t per = (*total + p.ctas - 1) / p.ctas;
-  return per < kMinUnits ? kMinUnits : per;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, before + incl > u);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      *first = before + __shfl_sync(0xffffffffu, incl - mine, src);
+      return b0 + src;
+    }
+    before += __shfl_sync(0xffffffffu, incl, 31);
+  }
 }
 
 }  // namespace
@@ -132,51 +158,61 @@ struct DecodeTile {
   static constexpr int kWarpRows = RB / kWr;             // 8 or 16
   static constexpr int kSlots = D / 8;                   // 16-byte slots per lane and stage (K and V)
   static constexpr int kStage = kSlots * 512 + 32;       // + the unit's four scales
-  static constexpr int kStages = kWr == 1 ? (D == 128 ? 3 : 4) : 4;
+  static constexpr int kCtas = RB == 8 ? 3 : 2;          // CTAs per SM
+  static constexpr int kStages = RB == 8 ? (D == 128 ? 2 : 4) : kWr == 1 ? (D == 128 ? 3 : 4) : 4;
   static constexpr int kRing = kTeams * kStages * kStage;
   static constexpr int kComb = kTeams > 1 ? RB * D * 4 + RB * 32 : 0;   // one team's partial on its way to the next
   static constexpr int kSmem = kRing + kComb;
 };
 
 template <typename T, int D, int RB>
-__global__ void __launch_bounds__(kDecWarps * 32, 2) kv8_attn_kernel(const __grid_constant__ DecodeParams p) {
+__global__ void __launch_bounds__(kDecWarps * 32, (DecodeTile<D, RB>::kCtas)) kv8_attn_kernel(const __grid_constant__ DecodeParams p) {
   using C = DecodeTile<D, RB>;
   constexpr bool kUpper = RB > 8;           // rows g + 8 of the m16 tile in use
   constexpr int kHalves = kUpper ? 2 : 1;
   constexpr int KS = D / 16;                // k16 steps of the score product
-  constexpr int NT = D / 8;                 // n8 tiles of the value product
+  // Value product.  RB = 8: V^T is the 16-row operand and P^T the 8-column
+  // one, O^T comes out (columns (D / 8) g + 2 n + {0, 1} of rows 2t, 2t + 1
+  // in tile n); otherwise P is the 16-row operand (rows g, g + 8, columns
+  // (D / 8) (2t + {0, 1}) + n in tile n).
+  constexpr int NT = kUpper ? D / 8 : D / 16;
   constexpr int VW = D / 32;                // 4-byte words of a lane's piece of a V token
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int team = warp / C::kWr, wr = warp % C::kWr;
   uint8_t* ring = smem + team * (C::kStages * C::kStage);
-  float4* comb = reinterpret_cast<float4*>(smem + C::kRing) + wr * (kHalves * (NT / 2) * 32);   // [halves][NT / 2][lanes]
+  float4* comb = reinterpret_cast<float4*>(smem + C::kRing) + wr * (NT * 32);   // [NT][lanes]
   float2* comb_ml = reinterpret_cast<float2*>(smem + C::kRing + RB * D * 4) + wr * (kHalves * 32);
   const Kv8View& c = p.c;
   const int page = 1 << c.page_shift;
 
-  int64_t total;
-  const int64_t per = units_per_cta(p, &total);
-  const int64_t u0 = blockIdx.x * per, u1 = min(total, u0 + per);
+  int total;
+  const int per = units_per_cta(p, &total);
+  const int u0 = min(total, (int)blockIdx.x * per), u1 = min(total, u0 + per);
   asm volatile("griddepcontrol.launch_dependents;");
   if (u0 >= u1) return;
-  int64_t first;
-  int b = warp_find_seq(u0, p.B, [&](int i) { return seq_units(p, i) * c.kv_heads; }, &first);
-  int64_t su = seq_units(p, b);
-  int h = (int)((u0 - first) / su);
-  int64_t unit0 = u0 - first - h * su;      // first unit within (b, h)
+  int first;
+  int b = find_unit(p, u0, &first);
+  int su = seq_units(p, b);
+  int h = (u0 - first) / su;
+  int unit0 = u0 - first - h * su;          // first unit within (b, h)
   const int row0 = blockIdx.y * RB + wr * C::kWarpRows;
 
-  // The copies run ahead of the products, and the page table ahead of the
-  // copies: look_up() loads the next unit's two pages (a unit's 32 tokens
-  // lie in at most two), issue() copies the unit that was looked up before.
+  // The copies run ahead of the products, and the page table two units
+  // ahead of the copies: look_up() loads a unit's two pages (its 32 tokens
+  // lie in at most two), issue() copies the unit that was looked up before
+  // the last one.
+  struct Pages {
+    int id[2], tok, head;
+    bool any;
+  };
   int pb = b, ph = h, plen = kv8_len(c, p.lens[b]);
-  int64_t psu = su, pu = u0 + team, pfirst = first + h * su;   // pfirst: flat index of (pb, ph)'s unit 0
-  int n_id[2] = {0, 0}, n_tok = 0, n_head = 0;
-  bool n_any = false;
+  int psu = su, pu = u0 + team, pfirst = first + h * su;   // pfirst: flat index of (pb, ph)'s unit 0
+  Pages ahead[2] = {};
   auto look_up = [&]() {
-    n_any = pu < u1;
-    if (n_any) {
+    Pages r{};
+    r.any = pu < u1;
+    if (r.any) {
       while (pu >= pfirst + psu) {          // next (sequence, head) that has units
         pfirst += psu;
         if (++ph == c.kv_heads) {
@@ -186,25 +222,29 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2) kv8_attn_kernel(const __gri
           plen = kv8_len(c, p.lens[pb]);
         }
       }
-      n_tok = (int)(pu - pfirst) * kUnit;
-      n_head = ph;
+      r.tok = (pu - pfirst) * kUnit;
+      r.head = ph;
       const int32_t* row = c.table + (int64_t)pb * c.table_width;
       const int last = (plen - 1) >> c.page_shift;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) n_id[i] = row[min((n_tok + 16 * i) >> c.page_shift, last)];
+      for (int i = 0; i < 2; ++i) r.id[i] = row[min((r.tok + 16 * i) >> c.page_shift, last)];
     }
     pu += C::kTeams;
+    return r;
   };
   auto issue = [&](int stage) {
-    if (n_any) {
-      int64_t kb[2];                        // element offsets of tokens n_tok and n_tok + 16
+    Pages n = ahead[0];
+    ahead[0] = ahead[1];
+    ahead[1] = look_up();
+    if (n.any) {
+      int64_t kb[2];                        // element offsets of tokens tok and tok + 16
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        if (n_id[i] < 0 || n_id[i] >= c.num_pages) {
+        if (n.id[i] < 0 || n.id[i] >= c.num_pages) {
           report_error(kErrBadPage);
-          n_id[i] = 0;
+          n.id[i] = 0;
         }
-        kb[i] = kv8_base(c, n_id[i], n_head) + (int64_t)((n_tok + 16 * i) & (page - 1)) * D;
+        kb[i] = kv8_base(c, n.id[i], n.head) + (int64_t)((n.tok + 16 * i) & (page - 1)) * D;
       }
       const uint32_t at = smem_u32(ring + stage * C::kStage), dst = at + lane * 16;
       // the team's warps take the pieces in turn
@@ -228,30 +268,50 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2) kv8_attn_kernel(const __gri
           else cp_async8(at + 4 * 512 + (kk * 4 + x) * 256 + lane * 8, c.v_codes + off);
         }
       if (lane < 4 && wr == 0) {
-        const float* sc = (lane < 2 ? c.k_scale : c.v_scale) + (int64_t)((lane & 1) ? n_id[1] : n_id[0]) * c.kv_heads + n_head;
+        const float* sc = (lane < 2 ? c.k_scale : c.v_scale) + (int64_t)((lane & 1) ? n.id[1] : n.id[0]) * c.kv_heads + n.head;
         cp_async4(at + C::kSlots * 512 + lane * 4, sc);
       }
     }
     cp_commit();
   };
-  look_up();
+  ahead[0] = look_up();
+  ahead[1] = look_up();
+  // A team of one warp refills a stage when it has used it; a larger team
+  // when the barrier of the next unit says that all of it has.
+  constexpr bool kAlone = C::kWr == 1;
 #pragma unroll
-  for (int s = 0; s < C::kStages - 1; ++s) {
-    issue(s);
-    look_up();
-  }
+  for (int s = 0; s < C::kStages - (kAlone ? 0 : 1); ++s) issue(s);
 
   uint32_t qf[KS][4];
   float qs[2];                         // row factor: scale * log2(e) / the power of two q was multiplied by
   int lim[2];                          // tokens the row may see
   float o[NT][4], m[2], l[2];   // m: running maximum - kPShift, l: this lane's part of the sum
+  // o = o * f for the rows of half hf; f is the row's (lanes 4 g ..)
+  auto scale_rows = [&](int hf, float f) {
+    if constexpr (kUpper) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        o[n][hf * 2] *= f;
+        o[n][hf * 2 + 1] *= f;
+      }
+    } else {
+      const float f0 = __shfl_sync(0xffffffffu, f, 8 * t), f1 = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        o[n][0] *= f0;
+        o[n][1] *= f1;
+        o[n][2] *= f0;
+        o[n][3] *= f1;
+      }
+    }
+  };
   int stage = 0;
-  int64_t cu = u0 + team;                   // this team's next unit
-  int64_t seg0 = u0;                        // current segment: units [seg0, seg1) of (b, h)
-  int64_t seg_first = u0 - unit0;           // flat index of (b, h)'s unit 0
+  int cu = u0 + team;                       // this team's next unit
+  int seg0 = u0;                            // current segment: units [seg0, seg1) of (b, h)
+  int seg_first = u0 - unit0;               // flat index of (b, h)'s unit 0
 
   while (seg0 < u1) {
-    const int64_t seg1 = min(u1, seg_first + su);
+    const int seg1 = min(u1, seg_first + su);
     const int len = kv8_len(c, p.lens[b]);
     // query fragments and row state
 #pragma unroll
@@ -296,7 +356,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2) kv8_attn_kernel(const __gri
 #pragma unroll
           for (int x = 0; x < 2; ++x)
             qf[i * 4 + w][hf + 2 * x] =
-                pack_f16x2(f[i * 16 + w * 4 + x * 2] * up, f[i * 16 + w * 4 + x * 2 + 1] * up);
+                hf < kHalves ? pack_f16x2(f[i * 16 + w * 4 + x * 2] * up, f[i * 16 + w * 4 + x * 2 + 1] * up) : 0u;
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -304,17 +364,18 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2) kv8_attn_kernel(const __gri
       for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
 
     for (; cu < seg1; cu += C::kTeams) {
-      cp_wait<C::kStages - 2>();
-      // the other lanes' copies (the scales) and the other warps' are in, and
-      // everyone is done with the stage that is filled next
-      if constexpr (C::kWr == 1) __syncwarp();
-      else named_barrier(1 + team, C::kWr * 32);
-      issue(stage == 0 ? C::kStages - 1 : stage - 1);
-      look_up();
+      // the other lanes' copies (the scales) and the other warps' are in
+      cp_wait<C::kStages - (kAlone ? 1 : 2)>();
+      if constexpr (kAlone) {
+        __syncwarp();
+      } else {
+        named_barrier(1 + team, C::kWr * 32);
+        issue(stage == 0 ? C::kStages - 1 : stage - 1);
+      }
       const uint8_t* st = ring + stage * C::kStage;
       const float* sc = reinterpret_cast<const float*>(st + C::kSlots * 512);
       const float ks[2] = {sc[0], sc[1]}, vs[2] = {sc[2], sc[3]};
-      const int tok0 = (int)(cu - seg_first) * kUnit;
+      const int tok0 = (cu - seg_first) * kUnit;
       // scores
       float s[4][4];
 #pragma unroll
@@ -368,7 +429,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2) kv8_attn_kernel(const __gri
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const float mn = fmaxf(m[hf], top - kPShift);
         const float base = mn == -INFINITY ? 0.f : mn;            // nothing seen yet: every term is exp2(-inf)
-        const float alpha = mn == -INFINITY ? 1.f : exp2f(m[hf] - mn);
+        const float alpha = mn == -INFINITY ? 1.f : ex2(m[hf] - mn);
         m[hf] = mn;
         float sum = 0.f;
 #pragma unroll
@@ -376,24 +437,14 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2) kv8_attn_kernel(const __gri
           float pv[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float ex = exp2f(x[j][e] - base);
+            const float ex = ex2(x[j][e] - base);
             sum = fmaf(ex, vi[j >> 1], sum);
             pv[e] = ex > 0.f ? ex * vf[j >> 1] : 0.f;   // a masked token's page scale does not matter
           }
           pa[j >> 1][(j & 1) * 2 + hf] = pack_f16x2(pv[0], pv[1]);
         }
         l[hf] = fmaf(l[hf], alpha, sum);
-        if (alpha != 1.f) {
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            o[n][hf * 2] *= alpha;
-            o[n][hf * 2 + 1] *= alpha;
-          }
-        }
-      }
-      if constexpr (!kUpper) {
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) pa[kk][1] = pa[kk][3] = 0u;
+        if (__any_sync(0xffffffffu, alpha != 1.f)) scale_rows(hf, alpha);
       }
       // values
 #pragma unroll
@@ -415,6 +466,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2) kv8_attn_kernel(const __gri
         }
 #pragma unroll
         for (int w = 0; w < VW; ++w) {
+          [[maybe_unused]] uint32_t va[4];
           const uint32_t a_lo = __byte_perm(vw[0][w], vw[1][w], 0x5140) ^ 0x80808080u;
           const uint32_t a_hi = __byte_perm(vw[0][w], vw[1][w], 0x7362) ^ 0x80808080u;
           const uint32_t c_lo = __byte_perm(vw[2][w], vw[3][w], 0x5140) ^ 0x80808080u;
@@ -423,9 +475,19 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2) kv8_attn_kernel(const __gri
           for (int e = 0; e < 4; ++e) {
             const uint32_t b0 = codes_f16x2(e < 2 ? a_lo : a_hi, (e & 1) ? 0x4342 : 0x4140);
             const uint32_t b1 = codes_f16x2(e < 2 ? c_lo : c_hi, (e & 1) ? 0x4342 : 0x4140);
-            mma_f16(o[w * 4 + e], pa[kk], b0, b1);
+            if constexpr (kUpper) {
+              mma_f16(o[w * 4 + e], pa[kk], b0, b1);
+            } else {
+              va[(e & 1)] = b0;
+              va[2 + (e & 1)] = b1;
+              if (e & 1) mma_f16(o[w * 2 + (e >> 1)], va, pa[kk][0], pa[kk][2]);
+            }
           }
         }
+      }
+      if constexpr (kAlone) {
+        __syncwarp();                        // every lane has read the stage's scales
+        issue(stage);
       }
       stage = stage + 1 == C::kStages ? 0 : stage + 1;
     }
@@ -443,45 +505,63 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2) kv8_attn_kernel(const __gri
 #pragma unroll 1
     for (int w = C::kTeams - 1; w >= 0; --w) {
       if (team == w) {
+        if (w < C::kTeams - 1) {
+          float fb[2] = {0.f, 0.f};
 #pragma unroll
-        for (int hf = 0; hf < kHalves; ++hf) {
-          if (w < C::kTeams - 1) {
+          for (int hf = 0; hf < kHalves; ++hf) {
             const float2 ml = comb_ml[hf * 32 + lane];
             const float mx = fmaxf(m[hf], ml.x);
             const float fa = l[hf] == 0.f ? 0.f : exp2f(m[hf] - mx);
-            const float fb = ml.y == 0.f ? 0.f : exp2f(ml.x - mx);
-            l[hf] = l[hf] * fa + ml.y * fb;
+            fb[hf] = ml.y == 0.f ? 0.f : exp2f(ml.x - mx);
+            l[hf] = l[hf] * fa + ml.y * fb[hf];
             m[hf] = mx;
-#pragma unroll
-            for (int n = 0; n < NT / 2; ++n) {
-              const float4 v = comb[(hf * (NT / 2) + n) * 32 + lane];
-              o[2 * n][hf * 2] = fmaf(v.x, fb, o[2 * n][hf * 2] * fa);
-              o[2 * n][hf * 2 + 1] = fmaf(v.y, fb, o[2 * n][hf * 2 + 1] * fa);
-              o[2 * n + 1][hf * 2] = fmaf(v.z, fb, o[2 * n + 1][hf * 2] * fa);
-              o[2 * n + 1][hf * 2 + 1] = fmaf(v.w, fb, o[2 * n + 1][hf * 2 + 1] * fa);
-            }
+            scale_rows(hf, fa);
           }
-          if (w > 0) {
-            comb_ml[hf * 32 + lane] = make_float2(m[hf], l[hf]);
+          const float f0 = kUpper ? fb[0] : __shfl_sync(0xffffffffu, fb[0], 8 * t);
+          const float f1 = kUpper ? fb[0] : __shfl_sync(0xffffffffu, fb[0], 8 * t + 4);
+          const float f2 = kUpper ? fb[1] : f0, f3 = kUpper ? fb[1] : f1;
 #pragma unroll
-            for (int n = 0; n < NT / 2; ++n)
-              comb[(hf * (NT / 2) + n) * 32 + lane] = make_float4(o[2 * n][hf * 2], o[2 * n][hf * 2 + 1],
-                                                                  o[2 * n + 1][hf * 2], o[2 * n + 1][hf * 2 + 1]);
+          for (int n = 0; n < NT; ++n) {
+            const float4 v = comb[n * 32 + lane];
+            o[n][0] = fmaf(v.x, f0, o[n][0]);
+            o[n][1] = fmaf(v.y, f1, o[n][1]);
+            o[n][2] = fmaf(v.z, f2, o[n][2]);
+            o[n][3] = fmaf(v.w, f3, o[n][3]);
+          }
+        }
+        if (w > 0) {
+#pragma unroll
+          for (int hf = 0; hf < kHalves; ++hf) comb_ml[hf * 32 + lane] = make_float2(m[hf], l[hf]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) comb[n * 32 + lane] = make_float4(o[n][0], o[n][1], o[n][2], o[n][3]);
+        } else {
+          const int64_t slot = (int64_t)blockIdx.y * p.slots + b * c.kv_heads + h + blockIdx.x;
+          const int64_t at = slot * RB + wr * C::kWarpRows;
+#pragma unroll
+          for (int hf = 0; hf < kHalves; ++hf) {
+            if (row0 + hf * 8 + g < p.rows && t == 0) p.part_ml[at + hf * 8 + g] = make_float2(m[hf], l[hf]);
+          }
+          if constexpr (kUpper) {
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf)
+              if (row0 + hf * 8 + g < p.rows) {
+                float* dst = p.part_o + (at + hf * 8 + g) * D + (D / 8) * 2 * t;
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                  for (int n = 0; n < NT; n += 4)
+                    *reinterpret_cast<float4*>(dst + x * (D / 8) + n) = make_float4(
+                        o[n][hf * 2 + x], o[n + 1][hf * 2 + x], o[n + 2][hf * 2 + x], o[n + 3][hf * 2 + x]);
+              }
           } else {
-            const int r = hf * 8 + g;
-            if (row0 + r < p.rows) {
-              const int64_t slot = (int64_t)blockIdx.y * p.slots + b * c.kv_heads + h + blockIdx.x;
-              const int64_t at = slot * RB + wr * C::kWarpRows + r;
-              if (t == 0) p.part_ml[at] = make_float2(m[hf], l[hf]);
-              // column n of value tile i is value column (D / 8) n + i
-              float* dst = p.part_o + at * D + (D / 8) * 2 * t;
 #pragma unroll
-              for (int x = 0; x < 2; ++x)
+            for (int x = 0; x < 2; ++x)
+              if (row0 + 2 * t + x < p.rows) {
+                float* dst = p.part_o + (at + 2 * t + x) * D + (D / 8) * g;
 #pragma unroll
-                for (int n = 0; n < NT; n += 4)
-                  *reinterpret_cast<float4*>(dst + x * (D / 8) + n) = make_float4(
-                      o[n][hf * 2 + x], o[n + 1][hf * 2 + x], o[n + 2][hf * 2 + x], o[n + 3][hf * 2 + x]);
-            }
+                for (int n = 0; n < NT; n += 2)
+                  *reinterpret_cast<float4*>(dst + 2 * n) = make_float4(o[n][x], o[n][2 + x], o[n + 1][x], o[n + 1][2 + x]);
+              }
           }
         }
       }
@@ -502,92 +582,100 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2) kv8_attn_kernel(const __gri
 }
 
 // Second kernel: grid (B * kv_heads, output blocks + weight blocks).  An
-// output block joins the partials of a few rows of one (sequence, head),
-// `lanes` threads taking every lanes-th partial of the same four columns (a
-// long sequence has one partial per CTA of the first kernel, and reading
-// them one after the other would cost more than the attention); a weight
-// block turns the scores of kJoinTokens tokens into weights.
+// output block joins the partials of kJoinThreads / lanes groups of four
+// columns of one (sequence, head), `lanes` threads taking every lanes-th
+// partial of the same group (a long sequence has one partial per CTA of the
+// first kernel, and reading them one after the other would cost more than
+// the attention).  A weight block turns the scores of kJoinTokens tokens
+// into weights.
 constexpr int kJoinTokens = 1024;
 constexpr int kJoinThreads = 256;
+constexpr int kJoinRows = 8;                  // rows of scores in flight per thread
 constexpr int kMaxRows = 512;
+
+// (m, l) joined with (m2, l2); f, f2: what the two sides' values are scaled
+// by.  A side that has seen nothing has l = 0; a NaN stays NaN.
+__device__ __forceinline__ void join_stats(float& m, float& l, float m2, float l2, float& f, float& f2) {
+  const float mx = fmaxf(m, m2);
+  f = l == 0.f ? 0.f : exp2f(m - mx);
+  f2 = l2 == 0.f ? 0.f : exp2f(m2 - mx);
+  l = l * f + l2 * f2;
+  m = mx;
+}
 
 template <typename T, int D, int RB>
 __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const __grid_constant__ DecodeParams p) {
-  __shared__ float2 s_ml[kMaxRows];           // (M - kPShift, 1 / sum) per row; 1 / sum = 0: the row sees nothing
+  __shared__ float2 s_ml[kMaxRows];           // weights: (M - kPShift, 1 / sum) per row; 0: the row sees nothing
   __shared__ float4 s_part[kJoinThreads];
-  constexpr int kCols = D / 4;                // threads across a row
+  constexpr int kCols = D / 4;                // column groups of a row
   const Kv8View& c = p.c;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31;
   const int bh = blockIdx.x, b = bh / c.kv_heads, h = bh - b * c.kv_heads;
-  const int64_t tok0 = (int64_t)((int)blockIdx.y - p.out_blocks) * kJoinTokens;
+  const int chunk = (int)blockIdx.y - p.out_blocks;
   const int len = kv8_len(c, p.lens[b]);
-  if (tok0 >= len && tok0 >= 0) return;
+  if (chunk >= 0 && (int64_t)chunk * kJoinTokens >= len) return;
   // the CTAs of the first kernel that hold partials of (b, h): c0 .. c1
-  int64_t total;
-  const int64_t per = units_per_cta(p, &total);
-  int64_t before = 0;
+  int total;
+  const int per = units_per_cta(p, &total);
+  int before = 0;
   for (int i = lane; i < b; i += 32) before += seq_units(p, i);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-  const int64_t su = seq_units(p, b), ub = before * c.kv_heads + h * su;
-  const int c0 = (int)(ub / per), c1 = su ? (int)((ub + su - 1) / per) : c0 - 1;
-  // rows whose statistics this block needs
-  const int per_block = kJoinThreads / kCols / p.lanes;
-  const int ra = tok0 < 0 ? blockIdx.y * per_block : 0, rz = tok0 < 0 ? min(p.rows, ra + per_block) : p.rows;
+  before = __reduce_add_sync(0xffffffffu, before);
+  const int su = seq_units(p, b), ub = before * c.kv_heads + h * su;
+  const int c0 = ub / per, c1 = su ? (ub + su - 1) / per : c0 - 1;
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
-  for (int r = ra + warp; r < rz; r += kJoinThreads / 32) {
-    const float2* ml = p.part_ml + ((int64_t)(r / RB) * p.slots + bh) * RB + r % RB;
-    float mx = -INFINITY, sum = 0.f;
-    for (int i = c0 + lane; i <= c1; i += 32) {
-      const float2 v = ml[(int64_t)i * RB];
-      if (v.y == 0.f) continue;
-      const float m = fmaxf(mx, v.x);
-      sum = (sum == 0.f ? 0.f : sum * exp2f(mx - m)) + v.y * exp2f(v.x - m);
-      mx = m;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float om = __shfl_xor_sync(0xffffffffu, mx, o), os = __shfl_xor_sync(0xffffffffu, sum, o);
-      const float m = fmaxf(mx, om);
-      sum = (sum == 0.f ? 0.f : sum * exp2f(mx - m)) + (os == 0.f ? 0.f : os * exp2f(om - m));
-      mx = m;
-    }
-    // a sum that is NaN (a page scale that is not finite) stays NaN
-    if (lane == 0) s_ml[r] = make_float2(mx, sum == 0.f ? 0.f : 1.f / sum);
-  }
-  __syncthreads();
-  if (tok0 < 0) {
-    const int col = threadIdx.x % kCols, rest = threadIdx.x / kCols, part = rest % p.lanes, r = ra + rest / p.lanes;
+  if (chunk < 0) {
+    const int groups = kJoinThreads / p.lanes;
+    const int part = threadIdx.x / groups, item = blockIdx.y * groups + threadIdx.x % groups;
+    const int r = item / kCols, col = item - r * kCols;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (r < rz) {
+    float m = -INFINITY, l = 0.f;
+    if (r < p.rows) {
       const int64_t at = ((int64_t)(r / RB) * p.slots + bh) * RB + r % RB;
-      const float mx = s_ml[r].x;
-#pragma unroll 4
-      for (int i = c0 + part; i <= c1; i += p.lanes) {
-        const float2 ml = p.part_ml[at + (int64_t)i * RB];
-        const float4 v = *reinterpret_cast<const float4*>(p.part_o + (at + (int64_t)i * RB) * D + col * 4);
-        const float f = ml.y == 0.f ? 0.f : exp2f(ml.x - mx);
-        acc.x = fmaf(v.x, f, acc.x);
-        acc.y = fmaf(v.y, f, acc.y);
-        acc.z = fmaf(v.z, f, acc.z);
-        acc.w = fmaf(v.w, f, acc.w);
+      const float2* mls = p.part_ml + at;
+      const float4* os = reinterpret_cast<const float4*>(p.part_o + at * D) + col;
+      for (int i0 = c0 + part; i0 <= c1; i0 += 4 * p.lanes) {
+        float2 ml[4];
+        float4 v[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int64_t i = i0 + x * p.lanes;
+          ml[x] = make_float2(-INFINITY, 0.f);
+          v[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (i <= c1) {
+            ml[x] = mls[i * RB];
+            v[x] = os[i * RB * kCols];
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          float f, f2;
+          join_stats(m, l, ml[x].x, ml[x].y, f, f2);
+          acc.x = acc.x * f + v[x].x * f2;
+          acc.y = acc.y * f + v[x].y * f2;
+          acc.z = acc.z * f + v[x].z * f2;
+          acc.w = acc.w * f + v[x].w * f2;
+        }
       }
     }
     if (p.lanes > 1) {
       s_part[threadIdx.x] = acc;
+      s_ml[threadIdx.x] = make_float2(m, l);
       __syncthreads();
       if (part == 0)
         for (int i = 1; i < p.lanes; ++i) {
-          const float4 v = s_part[threadIdx.x + i * kCols];
-          acc.x += v.x;
-          acc.y += v.y;
-          acc.z += v.z;
-          acc.w += v.w;
+          const float4 v = s_part[threadIdx.x + i * groups];
+          const float2 ml = s_ml[threadIdx.x + i * groups];
+          float f, f2;
+          join_stats(m, l, ml.x, ml.y, f, f2);
+          acc.x = acc.x * f + v.x * f2;
+          acc.y = acc.y * f + v.y * f2;
+          acc.z = acc.z * f + v.z * f2;
+          acc.w = acc.w * f + v.w * f2;
         }
     }
-    if (part == 0 && r < rz) {
-      const float inv = s_ml[r].y;
+    if (part == 0 && r < p.rows) {
+      const float inv = l == 0.f ? 0.f : 1.f / l;   // zeros where the row sees nothing
       T* dst = static_cast<T*>(p.out) + (((int64_t)b * p.T + r / p.group) * p.heads + h * p.group + r % p.group) * D + col * 4;
       const T o[4] = {from_f32<T>(acc.x * inv), from_f32<T>(acc.y * inv), from_f32<T>(acc.z * inv),
                       from_f32<T>(acc.w * inv)};
@@ -595,27 +683,62 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const __grid_con
     }
     return;
   }
-  // four tokens per thread; a masked or padded score is never used
-  const int64_t tok = tok0 + threadIdx.x * 4;
-  if (tok >= len) return;
+  // Four tokens per thread.  The first rows' scores and the old weights are
+  // on their way while the statistics are joined; a masked or padded score is
+  // loaded (inside its row) but never used.
+  const int tok = chunk * kJoinTokens + threadIdx.x * 4;
+  const bool live = tok < len;
   const float* s = p.scores + (int64_t)bh * p.rows * p.score_cap + tok;
-  float mass[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-  for (int r = 0; r < p.rows; ++r) {
-    const float4 v = *reinterpret_cast<const float4*>(s + (int64_t)r * p.score_cap);
-    const float2 row = s_ml[r];
-    const int see = row.y == 0.f ? 0 : len - p.T + r / p.group + 1;
-    const float x[4] = {v.x, v.y, v.z, v.w};
+  const int64_t wat = (int64_t)bh * p.cap + tok;
+  float4 v[kJoinRows];
+  auto fetch = [&](int r0) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (tok + e < see) mass[e] = fmaf(exp2f(x[e] - row.x), row.y, mass[e]);
+    for (int r = 0; r < kJoinRows; ++r)
+      if (live && r0 + r < p.rows) v[r] = *reinterpret_cast<const float4*>(s + (int64_t)(r0 + r) * p.score_cap);
+  };
+  fetch(0);
+  float w[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = tok + e < len ? p.weights[wat + e] : 0.f;
+  // `per_row` lanes join a row's statistics
+  int per_row = 32;
+  while (per_row > 1 && kJoinThreads / per_row < p.rows) per_row >>= 1;
+  for (int r0 = 0; r0 < p.rows; r0 += kJoinThreads / per_row) {
+    const int r = r0 + threadIdx.x / per_row;
+    float m = -INFINITY, l = 0.f, f, f2;
+    if (r < p.rows) {
+      const float2* mls = p.part_ml + ((int64_t)(r / RB) * p.slots + bh) * RB + r % RB;
+#pragma unroll 4
+      for (int i = c0 + threadIdx.x % per_row; i <= c1; i += per_row) {
+        const float2 ml = mls[(int64_t)i * RB];
+        join_stats(m, l, ml.x, ml.y, f, f2);
+      }
+    }
+    for (int o = per_row >> 1; o > 0; o >>= 1) {
+      const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o);
+      join_stats(m, l, m2, l2, f, f2);
+    }
+    if (r < p.rows && threadIdx.x % per_row == 0) s_ml[r] = make_float2(m, l == 0.f ? 0.f : 1.f / l);
+  }
+  __syncthreads();
+  if (!live) return;
+  float mass[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int r0 = 0; r0 < p.rows; r0 += kJoinRows) {
+    if (r0) fetch(r0);
+#pragma unroll
+    for (int r = 0; r < kJoinRows; ++r) {
+      if (r0 + r >= p.rows) break;
+      const float2 row = s_ml[r0 + r];
+      const int see = row.y == 0.f ? 0 : len - p.T + (r0 + r) / p.group + 1;
+      const float x[4] = {v[r].x, v[r].y, v[r].z, v[r].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (tok + e < see) mass[e] = fmaf(ex2(x[e] - row.x), row.y, mass[e]);
+    }
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e)
-    if (tok + e < len) {
-      const int64_t at = (int64_t)bh * p.cap + tok + e;
-      p.weights_out[at] = p.weights[at] + mass[e];
-    }
+    if (tok + e < len) p.weights_out[wat + e] = w[e] + mass[e];
 }
 
 // ---------------------------------------------------------------------------
@@ -623,7 +746,6 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const __grid_con
 // ---------------------------------------------------------------------------
 // Rows per CTA; beyond 64 the cache is read once for each 64.
 static int row_block(int rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
-constexpr int kDecodeCtasPerSm = 2;
 
 static int sm_count() {
   int dev = 0, n = 0;
@@ -637,17 +759,21 @@ static void decode_plan(DecodeParams& p, size_t* bytes) {
   const int rb = row_block(p.rows), blocks = (p.rows + rb - 1) / rb;
   const int64_t cap_units = (((int64_t)p.c.table_width << p.c.page_shift) + kUnit - 1) / kUnit;
   const int64_t most = (cap_units * p.B * p.c.kv_heads + kMinUnits - 1) / kMinUnits;
-  int64_t ctas = (int64_t)sm_count() * kDecodeCtasPerSm;
+  int64_t ctas = (int64_t)sm_count() * (rb == 8 ? 3 : 2);   // DecodeTile's kCtas
   ctas = (ctas + blocks - 1) / blocks;
   p.ctas = (int)(most < ctas ? most : ctas);
   if (p.ctas < 1) p.ctas = 1;
   p.slots = p.B * p.c.kv_heads + p.ctas;
   p.score_cap = cap_units * kUnit;
-  // a (sequence, head) has about ctas / (B * kv_heads) partials
+  // a (sequence, head) has about ctas / (B * kv_heads) partials; more lanes
+  // than keep the output blocks to one wave (four to an SM) cost more than
+  // they save (8 verify tokens of 8 sequences: 8 lanes 13 us, 2 lanes 5 us)
   p.lanes = 1;
-  while (p.lanes < 8 && p.lanes * p.B * p.c.kv_heads * 2 <= p.ctas) p.lanes *= 2;
-  const int per_block = kJoinThreads / (p.c.dim / 4) / p.lanes;
-  p.out_blocks = (p.rows + per_block - 1) / per_block;
+  while (p.lanes < 32 && p.lanes * p.B * p.c.kv_heads * 2 <= p.ctas &&
+         (int64_t)p.lanes * 2 * p.B * p.c.kv_heads * p.rows * (p.c.dim / 4) <= (int64_t)kJoinThreads * 4 * sm_count())
+    p.lanes *= 2;
+  const int groups = kJoinThreads / p.lanes;
+  p.out_blocks = (p.rows * (p.c.dim / 4) + groups - 1) / groups;
   const size_t part_rows = (size_t)blocks * p.slots * rb;
   uint8_t* w = reinterpret_cast<uint8_t*>(p.part_o);
   auto al = [](size_t x) { return (x + 255) & ~(size_t)255; };

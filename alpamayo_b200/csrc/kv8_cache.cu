@@ -13,6 +13,8 @@
 //  * gather: code * scale in float32, rounded once to the output type.
 //  * compact (eviction's second half): code * scale of the kept tokens,
 //    requantised per destination page.
+#include <cooperative_groups.h>
+
 #include "kv8.cuh"
 
 namespace paro {
@@ -56,12 +58,44 @@ __device__ __forceinline__ void unpack(const Vec8<float>& v, float (&f)[8]) {
   for (int i = 0; i < 8; ++i) f[i] = s[i];
 }
 
+// (Assembling 2^23 + code with byte permutes instead of converting was
+// slower: the read-back of 131072 tokens 82 against 61 us.)
 __device__ __forceinline__ void unpack_codes8(uint2 u, float (&f)[8]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     f[i] = (float)(int8_t)(u.x >> (8 * i));
     f[4 + i] = (float)(int8_t)(u.y >> (8 * i));
   }
+}
+
+// Codes of N elements under `scale`, as kv8_code gives them, without a
+// division each: x times the reciprocal is within 2.3e-5 of the rounded
+// quotient (three units in the last place below 128), so both round to the
+// same integer unless the product is that close to the middle between two;
+// those few are divided.  Adding 1.5 * 2^23 rounds to an integer (ties to
+// even) that stands in the low bits.
+template <int N>
+__device__ __forceinline__ void codes_of(const float (&x)[N], float scale, uint32_t (&out)[N / 4]) {
+  uint32_t q[N];
+  bool slow = !(scale > 1e-30f && scale < 1e30f);   // reciprocal or quotients out of range, zero, not finite
+  if (!slow) {
+    const float inv = __fdiv_rn(1.f, scale);
+    float far = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float y = __fmul_rn(x[i], inv), z = __fadd_rn(y, 12582912.f);
+      q[i] = __float_as_uint(z);
+      far = fmaxf(far, fabsf(__fadd_rn(y, -__fadd_rn(z, -12582912.f))));
+    }
+    slow = far > 0.49996f;
+  }
+  if (slow) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) q[i] = (uint32_t)kv8_code(x[i], scale);
+  }
+#pragma unroll
+  for (int i = 0; i < N; i += 4)
+    out[i / 4] = __byte_perm(__byte_perm(q[i], q[i + 1], 0x0040), __byte_perm(q[i + 2], q[i + 3], 0x0040), 0x5410);
 }
 
 __device__ __forceinline__ uint32_t pack4(const int* c) {
@@ -115,8 +149,7 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(AppendParams p) {
     if (threadIdx.x == 0) report_error(kErrBadPage);
     return;
   }
-  const int id = kv8_page(c, b, (int)blk);
-  if (id < 0) return;
+  const int id = c.table[(int64_t)b * c.table_width + blk];   // checked below, behind the new tokens' loads
   const int h = blockIdx.y, which = blockIdx.z;
   const int64_t t0 = blk << c.page_shift;               // first token of the page
   const int old = (int)max((int64_t)0, start - t0);     // its tokens that were there before
@@ -125,10 +158,6 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(AppendParams p) {
   const T* src = static_cast<const T*>(which ? p.src[1] : p.src[0]);
   const int64_t st = which ? p.stride_t[1] : p.stride_t[0], sh = which ? p.stride_h[1] : p.stride_h[0];
   const int64_t row0 = (int64_t)p.cu[b] + (t0 - start);  // source row of the page's token 0
-  int8_t* codes = (which ? c.v_codes : c.k_codes) + kv8_base(c, id, h);
-  float* scale_at = (which ? c.v_scale : c.k_scale) + ((int64_t)id * c.kv_heads + h);
-  const float prior = old ? *scale_at : 0.f;
-
   Vec8<T> v[kVpt];
   uint2 prev[kVpt];
   uint32_t top = 0;
@@ -136,7 +165,18 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(AppendParams p) {
   for (int i = 0; i < kVpt; ++i) {
     const int e = i * blockDim.x + threadIdx.x, tok = e / per_tok, d = (e - tok * per_tok) * 8;
     if (tok >= old && tok < end) load8(v[i], src + (row0 + tok) * st + h * sh + d);
-    if (tok < old) prev[i] = *reinterpret_cast<const uint2*>(codes + (int64_t)e * 8);
+  }
+  if (id < 0 || id >= c.num_pages) {
+    if (threadIdx.x == 0) report_error(kErrBadPage);
+    return;
+  }
+  int8_t* codes = (which ? c.v_codes : c.k_codes) + kv8_base(c, id, h);
+  float* scale_at = (which ? c.v_scale : c.k_scale) + ((int64_t)id * c.kv_heads + h);
+  const float prior = old ? *scale_at : 0.f;
+#pragma unroll
+  for (int i = 0; i < kVpt; ++i) {
+    const int e = i * blockDim.x + threadIdx.x;
+    if (e / per_tok < old) prev[i] = *reinterpret_cast<const uint2*>(codes + (int64_t)e * 8);
   }
 #pragma unroll
   for (int i = 0; i < kVpt; ++i) {
@@ -158,20 +198,21 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(AppendParams p) {
   for (int i = 0; i < kVpt; ++i) {
     const int e = i * blockDim.x + threadIdx.x, tok = e / per_tok;
     if (tok >= end) continue;
-    int q[8];
+    float f[8];
+    uint32_t q[2];
     if (tok >= old) {
-      float f[8];
       unpack(v[i], f);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) q[k] = kv8_code(f[k], s);
+      codes_of(f, s, q);
     } else {
       if (ratio == 1.f) continue;
-      float f[8];
       unpack_codes8(prev[i], f);
+      int r[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) q[k] = __float2int_rn(__fmul_rn(f[k], ratio));
+      for (int k = 0; k < 8; ++k) r[k] = __float2int_rn(__fmul_rn(f[k], ratio));
+      q[0] = pack4(r);
+      q[1] = pack4(r + 4);
     }
-    *reinterpret_cast<uint2*>(codes + (int64_t)e * 8) = make_uint2(pack4(q), pack4(q + 4));
+    *reinterpret_cast<uint2*>(codes + (int64_t)e * 8) = make_uint2(q[0], q[1]);
   }
 }
 
@@ -184,59 +225,84 @@ struct GatherParams {
   void* out[2];
 };
 
-constexpr int kGatherRows = 16;
+constexpr int kGatherRows = 32;
+constexpr int kGatherThreads = 256;
+constexpr int kGatherFlight = 4;   // pieces of 16 codes in flight per thread
 
-// Grid (output rows / 16, 2: keys / values).  One thread turns 8 codes into
-// 8 values at a time.
+__device__ __forceinline__ void unpack_codes16(const uint4& u, float (&f)[16]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 16; ++i) f[i] = (float)(int8_t)(w[i >> 2] >> (8 * (i & 3)));
+}
+
 template <typename T>
-__global__ void __launch_bounds__(256) kv8_gather_kernel(GatherParams p) {
+__device__ __forceinline__ void store16(T* dst, const float (&f)[16]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      reinterpret_cast<float4*>(dst)[i] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+  } else {
+    __align__(16) T o[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i] = from_f32<T>(f[i]);
+    reinterpret_cast<uint4*>(dst)[0] = reinterpret_cast<const uint4*>(o)[0];
+    reinterpret_cast<uint4*>(dst)[1] = reinterpret_cast<const uint4*>(o)[1];
+  }
+}
+
+// Grid (output rows / 32).  One warp finds the rows' tokens; then every
+// thread has several pieces of 16 codes of keys and values on their way.
+template <typename T>
+__global__ void __launch_bounds__(kGatherThreads) kv8_gather_kernel(GatherParams p) {
   const Kv8View& c = p.c;
-  __shared__ int s_b;
+  __shared__ int s_page[kGatherRows], s_at[kGatherRows];   // page (-1: zeros) and place in it
   const int64_t r0 = (int64_t)blockIdx.x * kGatherRows;
   if (threadIdx.x < 32) {
     int64_t first;
-    const int b = warp_find_seq(r0, p.B, [&](int i) -> int64_t { return max(0, p.cu[i + 1] - p.cu[i]); }, &first);
-    if (threadIdx.x == 0) s_b = b;
+    int b = warp_find_seq(r0, p.B, [&](int i) -> int64_t { return max(0, p.cu[i + 1] - p.cu[i]); }, &first);
+    const int64_t row = r0 + threadIdx.x;
+    int page = -1, at = 0;
+    while (b >= 0 && b < p.B && row >= p.cu[b + 1]) ++b;
+    if (row < p.rows && b >= 0 && b < p.B) {               // rows behind the last sequence read as zeros
+      const int64_t tok = (int64_t)p.starts[b] + (row - p.cu[b]), blk = tok >> c.page_shift;
+      if (tok < 0 || blk >= c.table_width) report_error(kErrBadPage);
+      else page = kv8_page(c, b, (int)blk);
+      at = (int)(tok & ((1 << c.page_shift) - 1));
+    }
+    s_page[threadIdx.x] = page;
+    s_at[threadIdx.x] = at;
   }
   __syncthreads();
-  const int b0 = s_b, which = blockIdx.y;
-  const int8_t* codes = which ? c.v_codes : c.k_codes;
-  const float* scales = which ? c.v_scale : c.k_scale;
-  T* out = static_cast<T*>(which ? p.out[1] : p.out[0]);
-  const int per_tok = c.kv_heads * (c.dim >> 3);
-  const int rows = (int)min((int64_t)kGatherRows, p.rows - r0);
-  for (int e = threadIdx.x; e < rows * per_tok; e += blockDim.x) {
-    const int r = e / per_tok, in_tok = e - r * per_tok;
-    const int h = in_tok / (c.dim >> 3), d = (in_tok - h * (c.dim >> 3)) * 8;
-    const int64_t row = r0 + r;
-    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    int b = b0;
-    while (b >= 0 && b < p.B && row >= p.cu[b + 1]) ++b;
-    if (b >= 0 && b < p.B) {   // rows past the last sequence read as zeros
-      const int64_t tok = (int64_t)p.starts[b] + (row - p.cu[b]);
-      const int64_t blk = tok >> c.page_shift;
-      if (tok < 0 || blk >= c.table_width) {
-        report_error(kErrBadPage);
-      } else {
-        const int id = kv8_page(c, b, (int)blk);
-        if (id >= 0) {
-          const float s = scales[(int64_t)id * c.kv_heads + h];
-          unpack_codes8(*reinterpret_cast<const uint2*>(codes + kv8_base(c, id, h) +
-                                                        (tok & ((1 << c.page_shift) - 1)) * c.dim + d), f);
+  const int per_head = c.dim >> 4, per_tok = c.kv_heads * per_head;
+  const int rows = (int)min((int64_t)kGatherRows, p.rows - r0), side = rows * per_tok;
+  for (int e0 = threadIdx.x; e0 < 2 * side; e0 += kGatherFlight * kGatherThreads) {
+    uint4 w[kGatherFlight];
+    float s[kGatherFlight];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) f[k] *= s;
+    for (int x = 0; x < kGatherFlight; ++x) {
+      const int e = e0 + x * kGatherThreads;
+      w[x] = make_uint4(0u, 0u, 0u, 0u);
+      s[x] = 0.f;
+      if (e < 2 * side) {
+        const int which = e >= side, i = e - (which ? side : 0), r = i / per_tok, in_tok = i - r * per_tok;
+        const int h = in_tok / per_head, d = (in_tok - h * per_head) * 16, page = s_page[r];
+        if (page >= 0) {
+          w[x] = *reinterpret_cast<const uint4*>((which ? c.v_codes : c.k_codes) + kv8_base(c, page, h) + s_at[r] * c.dim + d);
+          s[x] = (which ? c.v_scale : c.k_scale)[(int64_t)page * c.kv_heads + h];
         }
       }
     }
-    T* dst = out + (row * c.kv_heads + h) * c.dim + d;
-    if constexpr (sizeof(T) == 4) {
-      reinterpret_cast<float4*>(dst)[0] = make_float4(f[0], f[1], f[2], f[3]);
-      reinterpret_cast<float4*>(dst)[1] = make_float4(f[4], f[5], f[6], f[7]);
-    } else {
-      T o[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) o[k] = from_f32<T>(f[k]);
-      *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(o);
+    for (int x = 0; x < kGatherFlight; ++x) {
+      const int e = e0 + x * kGatherThreads;
+      if (e >= 2 * side) break;
+      const int which = e >= side;
+      float f[16];
+      unpack_codes16(w[x], f);
+#pragma unroll
+      for (int k = 0; k < 16; ++k) f[k] *= s[x];
+      // a row's pieces are contiguous: [row][head][dim]
+      store16(static_cast<T*>(which ? p.out[1] : p.out[0]) + (r0 * per_tok + (e - (which ? side : 0))) * 16, f);
     }
   }
 }
@@ -261,52 +327,42 @@ __device__ __forceinline__ uint32_t order_key(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-constexpr int kSelThreads = 1024;
+constexpr int kSelThreads = 512;
+constexpr int kSelWarps = kSelThreads / 32;
+constexpr int kSelFlight = 8;      // weights in flight per thread
+constexpr int kSelCached = 40960;  // keys of a CTA kept in shared memory, at most
+constexpr int kSelBins = 2048;
 
-// Block-wide exclusive prefix sum of two 16-bit counts packed in a word;
-// *total: their sums.  `slots`: 32 words.
-__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* slots, uint32_t* total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint32_t incl = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t up = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += up;
-  }
-  __syncthreads();   // the slots of the previous call have been read
-  if (lane == 31) slots[warp] = incl;
-  __syncthreads();
-  uint32_t w = slots[lane];
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t up = __shfl_up_sync(0xffffffffu, w, o);
-    if (lane >= o) w += up;
-  }
-  *total = __shfl_sync(0xffffffffu, w, 31);
-  const uint32_t before = __shfl_sync(0xffffffffu, w, warp) - slots[warp];
-  return before + incl - v;
-}
-
-// One CTA per (sequence, KV head): radix select (three digits of 11, 11 and
-// 10 bits, most significant first) of the smallest key still kept, then one
-// ordered pass that writes the kept tokens.
-__global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(EvictParams p) {
-  __shared__ uint32_t hist[2048];
-  __shared__ uint32_t slots[32];
-  __shared__ uint32_t s_digit, s_above;
-  const int bh = blockIdx.x, b = bh / p.c.kv_heads, tid = threadIdx.x;
-  int len = kv8_len(p.c, p.lens[b]);
+// One cluster of CTAs per (sequence, KV head), each CTA with a run of its
+// tokens: radix select (three digits of 11, 11 and 10 bits, most significant
+// first) of the smallest key still kept, on the sum of the CTAs' counts, then
+// an ordered pass: every warp counts its own run of tokens, the counts are
+// added up across warps and CTAs, and the warps write.  The keys are read
+// from global memory once and kept in shared memory as far as they fit
+// (`cached`, from the front of the CTA's run).  Bound by one SM's instruction
+// rate where there are few (sequence, head)s: 32768 tokens of 4 heads took
+// 42 us on one CTA each.
+__global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(EvictParams p, int cached, int with_masks) {
+  namespace cg = cooperative_groups;
+  extern __shared__ uint32_t keys[];           // [cached] keys, then two words per 32 tokens of the CTA's run
+  __shared__ __align__(16) uint32_t hist[3][kSelBins];
+  __shared__ uint32_t slots[kSelWarps], slots2[kSelWarps];
+  __shared__ uint32_t s_digit, s_above, s_total[2];
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int cs = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int bh = blockIdx.x / cs, b = bh / p.c.kv_heads, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int len = kv8_len(p.c, p.lens[b]);
   const float* w = p.weights + (int64_t)bh * p.cap;
   int32_t* kept = p.kept + (int64_t)bh * p.budget;
   float* nw = p.new_weights + (int64_t)bh * p.budget;
   const int n = min(len, p.budget);
-  if (bh % p.c.kv_heads == 0 && tid == 0) p.new_lens[b] = n;
-  for (int i = n + tid; i < p.budget; i += kSelThreads) {
+  if (bh % p.c.kv_heads == 0 && rank == 0 && tid == 0) p.new_lens[b] = n;
+  for (int i = n + rank * kSelThreads + tid; i < p.budget; i += cs * kSelThreads) {
     kept[i] = -1;
     nw[i] = 0.f;
   }
   if (len <= p.budget) {
-    for (int i = tid; i < n; i += kSelThreads) {
+    for (int i = rank * kSelThreads + tid; i < n; i += cs * kSelThreads) {
       kept[i] = i;
       nw[i] = w[i];
     }
@@ -314,88 +370,144 @@ __global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(EvictParams p) 
   }
   const int lo = p.sink, hi = len - p.recent;   // tokens that compete: lo <= t < hi (len > budget >= sink + recent)
   uint32_t need = p.budget - p.sink - p.recent; // how many of them stay
+  const bool any = need > 0;
+  // this CTA's tokens, and inside it each warp's
+  const int slice = (len + cs * 32 - 1) / (cs * 32) * 32, a0 = min(len, rank * slice), a1 = min(len, a0 + slice);
+  const int run = (slice + 32 * kSelWarps - 1) / (32 * kSelWarps) * 32;
+  const int t0 = min(a1, a0 + warp * run), t1 = min(a1, t0 + run);
+  uint32_t* masks = keys + cached;
   uint32_t prefix = 0, known = 0;               // key digits found so far and their mask
-  if (need > 0) {
-    const int shifts[3] = {21, 10, 0};
-#pragma unroll 1
-    for (int pass = 0; pass < 3; ++pass) {
-      const int shift = shifts[pass], digits = pass == 2 ? 1024 : 2048;
-      for (int i = tid; i < 2048; i += kSelThreads) hist[i] = 0;
-      __syncthreads();
-      for (int i = lo + tid; i < hi; i += kSelThreads) {
-        const uint32_t k = order_key(w[i]);
-        if ((k & known) == prefix) atomicAdd(&hist[(k >> shift) & (digits - 1)], 1u);
-      }
-      __syncthreads();
-      // thread i holds digits 2i and 2i + 1 from the top: find where the
-      // running count reaches `need`
-      const int d0 = digits - 1 - 2 * tid, d1 = d0 - 1;
-      const uint32_t c0 = d0 >= 0 ? hist[d0] : 0u, c1 = d1 >= 0 ? hist[d1] : 0u;
-      uint32_t incl = c0 + c1;
-      const int lane = tid & 31, warp = tid >> 5;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t up = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += up;
-      }
-      if (lane == 31) slots[warp] = incl;
-      __syncthreads();
-      uint32_t ws = slots[lane];
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t up = __shfl_up_sync(0xffffffffu, ws, o);
-        if (lane >= o) ws += up;
-      }
-      const uint32_t base = __shfl_sync(0xffffffffu, ws, warp) - slots[warp];
-      const uint32_t before = base + incl - c0 - c1;
-      if (before < need && before + c0 >= need) {
-        s_digit = d0;
-        s_above = before;
-      } else if (before + c0 < need && before + c0 + c1 >= need) {
-        s_digit = d1;
-        s_above = before + c0;
-      }
-      __syncthreads();
-      prefix |= s_digit << shift;
-      known |= (uint32_t)(digits - 1) << shift;
-      need -= s_above;      // still to take among the keys with this prefix
-      __syncthreads();
-    }
+  if (any) {
+    for (int i = tid; i < 3 * kSelBins; i += kSelThreads) hist[0][i] = 0;
+    __syncthreads();
   }
-  // ordered pass: keys above `prefix` stay, of those equal to it the first
-  // `need`; the low half of a count is the kept tokens, the high half the equal ones
-  const uint32_t thr = prefix;
-  const bool any = p.budget > p.sink + p.recent;
-  uint32_t out = 0, ties = 0;
-  for (int base = 0; base < len; base += kSelThreads) {
-    const int i = base + tid;
-    const float x = i < len ? w[i] : 0.f;
-    const bool fixed = i < len && (i < lo || i >= hi);
-    const uint32_t k = order_key(x);
-    const bool cand = any && i >= lo && i < hi;
-    const bool above = fixed || (cand && k > thr), equal = cand && k == thr;
-    uint32_t total;
-    const uint32_t at = block_scan((above ? 1u : 0u) | (equal ? 0x10000u : 0u), slots, &total);
-    // equal tokens before this one that stay: at most `need` in all
-    const uint32_t eq_before = ties + (at >> 16);
-    const uint32_t taken_before = min(eq_before, need) - min(ties, need);
-    const uint32_t pos = out + (at & 0xffffu) + taken_before;
-    if (above || (equal && eq_before < need)) {
-      kept[pos] = i;
-      nw[pos] = x;
+  for (int pass = 0; pass < 3 && any; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, digits = pass == 2 ? 1024 : kSelBins;
+    const int from = max(a0, lo), to = min(a1, hi);
+    for (int i0 = from + tid; i0 < to; i0 += kSelFlight * kSelThreads) {
+      uint32_t k[kSelFlight];
+#pragma unroll
+      for (int x = 0; x < kSelFlight; ++x) {
+        const int i = i0 + x * kSelThreads;
+        if (i < to) k[x] = pass > 0 && i - a0 < cached ? keys[i - a0] : order_key(w[i]);
+      }
+#pragma unroll
+      for (int x = 0; x < kSelFlight; ++x) {
+        const int i = i0 + x * kSelThreads;
+        if (i < to) {
+          if (pass == 0 && i - a0 < cached) keys[i - a0] = k[x];
+          if ((k[x] & known) == prefix) atomicAdd(&hist[pass][(k[x] >> shift) & (digits - 1)], 1u);
+        }
+      }
     }
-    out += (total & 0xffffu) + (min(ties + (total >> 16), need) - min(ties, need));
-    ties += total >> 16;
+    cluster.sync();
+    // thread i holds the four digits from 4 i below the top on: find where
+    // the running count reaches `need`
+    const int d0 = digits - 4 - 4 * tid;
+    uint32_t cnt[4] = {0u, 0u, 0u, 0u};         // from the highest digit down
+    if (d0 >= 0)
+      for (int r = 0; r < cs; ++r) {
+        const uint4 v = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(&hist[pass][d0], r));
+        cnt[0] += v.w;
+        cnt[1] += v.z;
+        cnt[2] += v.y;
+        cnt[3] += v.x;
+      }
+    const uint32_t mine = cnt[0] + cnt[1] + cnt[2] + cnt[3];
+    uint32_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    if (lane == 31) slots[warp] = incl;
+    __syncthreads();
+    uint32_t before = __reduce_add_sync(0xffffffffu, lane < warp ? slots[lane] : 0u) + incl - mine;
+    if (before < need && before + mine >= need) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        if (before < need && before + cnt[x] >= need) {
+          s_digit = d0 + 3 - x;
+          s_above = before;
+          before = need;   // found
+        } else {
+          before += cnt[x];
+        }
+      }
+    }
+    __syncthreads();
+    prefix |= s_digit << shift;
+    known |= (uint32_t)(digits - 1) << shift;
+    need -= s_above;      // still to take among the keys with this prefix
+    __syncthreads();
   }
+  // Keys above `prefix` stay, of those equal to it the first `need`.
+  // masks of the 32 tokens from i0 on that stay, and that are equal to the last kept
+  auto judge = [&](int i0) {
+    const int i = i0 + lane;
+    bool stays = i < t1 && (i < lo || i >= hi), tie = false;
+    if (any && i < t1 && !stays) {
+      const uint32_t k = i - a0 < cached ? keys[i - a0] : order_key(w[i]);
+      stays = k > prefix;
+      tie = k == prefix;
+    }
+    return make_uint2(__ballot_sync(0xffffffffu, stays), __ballot_sync(0xffffffffu, tie));
+  };
+  uint32_t above = 0, equal = 0;
+#pragma unroll 4
+  for (int i0 = t0; i0 < t1; i0 += 32) {
+    const uint2 m = judge(i0);
+    above += __popc(m.x);
+    equal += __popc(m.y);
+    if (with_masks && lane == 0) *reinterpret_cast<uint2*>(masks + (i0 - a0) / 32 * 2) = m;
+  }
+  if (lane == 0) {
+    slots[warp] = above;
+    slots2[warp] = equal;
+  }
+  __syncthreads();
+  uint32_t out = __reduce_add_sync(0xffffffffu, lane < warp ? slots[lane] : 0u);
+  uint32_t ties = __reduce_add_sync(0xffffffffu, lane < warp ? slots2[lane] : 0u);
+  if (tid == kSelThreads - 1) {
+    s_total[0] = out + above;
+    s_total[1] = ties + equal;
+  }
+  cluster.sync();
+  uint32_t out_cta = 0, ties_cta = 0;
+  if (lane < rank) {
+    const uint32_t* o = cluster.map_shared_rank(s_total, lane);
+    out_cta = o[0];
+    ties_cta = o[1];
+  }
+  out += __reduce_add_sync(0xffffffffu, out_cta);
+  ties += __reduce_add_sync(0xffffffffu, ties_cta);
+  out += min(ties, need);
+  const uint32_t below = (1u << lane) - 1u;
+#pragma unroll 4
+  for (int i0 = t0; i0 < t1; i0 += 32) {
+    const uint2 m = with_masks ? *reinterpret_cast<const uint2*>(masks + (i0 - a0) / 32 * 2) : judge(i0);
+    const uint32_t tie_at = ties + __popc(m.y & below);
+    const uint32_t taken = min(tie_at, need) - min(ties, need);   // equal ones before this lane that stay
+    if ((m.x >> lane & 1u) || ((m.y >> lane & 1u) && tie_at < need)) {
+      const uint32_t pos = out + __popc(m.x & below) + taken;
+      kept[pos] = i0 + lane;
+      nw[pos] = w[i0 + lane];
+    }
+    const uint32_t ties_after = ties + __popc(m.y);
+    out += __popc(m.x) + min(ties_after, need) - min(ties, need);
+    ties = ties_after;
+  }
+  cluster.sync();          // the other CTAs have read this one's counts
 }
 
-// Grid (destination pages per sequence, kv heads, 2 B: keys / values).
+// Grid (destination pages per sequence, kv heads, B).  The first half of a
+// CTA's threads moves the page's keys, the second its values.
 __global__ void __launch_bounds__(512) kv8_compact_kernel(EvictParams p) {
   __shared__ uint32_t slots[16];
-  __shared__ int64_t s_src[128];
-  __shared__ float s_scale[128];
+  __shared__ int64_t s_src[128];       // element offset of the token's row, -1: not a page of the pool
+  __shared__ float s_scale[2][128];
   const Kv8View& c = p.c;
-  const int b = blockIdx.z >> 1, which = blockIdx.z & 1, h = blockIdx.y, blk = blockIdx.x;
+  const int b = blockIdx.z, h = blockIdx.y, blk = blockIdx.x;
   const int page = 1 << c.page_shift;
   const int n = min(kv8_len(c, p.lens[b]), p.budget);
   const int cnt = min(page, n - blk * page);
@@ -405,55 +517,72 @@ __global__ void __launch_bounds__(512) kv8_compact_kernel(EvictParams p) {
     if (threadIdx.x == 0) report_error(kErrBadPage);
     return;
   }
-  const int8_t* codes = which ? c.v_codes : c.k_codes;
-  const float* scales = which ? c.v_scale : c.k_scale;
   const int32_t* kept = p.kept + ((int64_t)b * c.kv_heads + h) * p.budget + blk * page;
   for (int t = threadIdx.x; t < cnt; t += blockDim.x) {
     const int tok = kept[t];
     const int src = kv8_page(c, b, tok >> c.page_shift);
     s_src[t] = src < 0 ? -1 : kv8_base(c, src, h) + (int64_t)(tok & (page - 1)) * c.dim;
-    s_scale[t] = src < 0 ? 0.f : scales[(int64_t)src * c.kv_heads + h];
+    s_scale[0][t] = src < 0 ? 0.f : c.k_scale[(int64_t)src * c.kv_heads + h];
+    s_scale[1][t] = src < 0 ? 0.f : c.v_scale[(int64_t)src * c.kv_heads + h];
   }
   __syncthreads();
-  const int per_tok = c.dim >> 3;
-  uint2 v[kVpt];
+  const int half = blockDim.x >> 1, which = threadIdx.x >= half, tid = threadIdx.x - (which ? half : 0);
+  const int8_t* codes = which ? c.v_codes : c.k_codes;
+  const int per_tok = c.dim >> 4;
+  uint4 v[kVpt];
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < kVpt; ++i) {
-    const int e = i * blockDim.x + threadIdx.x, tok = e / per_tok, d = (e - tok * per_tok) * 8;
-    v[i] = make_uint2(0u, 0u);
-    if (tok < cnt && s_src[tok] >= 0) v[i] = *reinterpret_cast<const uint2*>(codes + s_src[tok] + d);
+    const int e = i * half + tid, tok = e / per_tok, d = (e - tok * per_tok) * 16;
+    v[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (tok < cnt && s_src[tok] >= 0) v[i] = *reinterpret_cast<const uint4*>(codes + s_src[tok] + d);
   }
 #pragma unroll
   for (int i = 0; i < kVpt; ++i) {
-    const int tok = (i * blockDim.x + threadIdx.x) / per_tok;
+    const int tok = (i * half + tid) / per_tok;
     if (tok < cnt) {
-      float f[8];
-      unpack_codes8(v[i], f);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(fabsf(__fmul_rn(f[k], s_scale[tok]))));
+      // |code * scale| is largest where |code| is
+      const uint32_t a = __vmaxu4(__vabs4(v[i].x), __vabs4(v[i].y)), bb = __vmaxu4(__vabs4(v[i].z), __vabs4(v[i].w));
+      uint32_t m = __vmaxu4(a, bb);
+      m = max(max(m & 0xffu, (m >> 8) & 0xffu), max((m >> 16) & 0xffu, m >> 24));
+      top = max(top, __float_as_uint(fabsf(__fmul_rn((float)m, s_scale[which][tok]))));
     }
   }
-  const float s = __fdiv_rn(block_absmax(top, slots), kKv8Max);
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = top;
+  __syncthreads();
+  const int warps = half >> 5;
+  for (int x = 0; x < warps; ++x) top = max(top, slots[which * warps + x]);
+  const float s = __fdiv_rn(__uint_as_float(top), kKv8Max);
   int8_t* dst = (which ? c.v_codes : c.k_codes) + kv8_base(c, id, h);
-  if (threadIdx.x == 0) (which ? c.v_scale : c.k_scale)[(int64_t)id * c.kv_heads + h] = s;
+  if (tid == 0) (which ? c.v_scale : c.k_scale)[(int64_t)id * c.kv_heads + h] = s;
 #pragma unroll
   for (int i = 0; i < kVpt; ++i) {
-    const int e = i * blockDim.x + threadIdx.x, tok = e / per_tok;
+    const int e = i * half + tid, tok = e / per_tok;
     if (tok >= cnt) continue;
-    float f[8];
-    int q[8];
-    unpack_codes8(v[i], f);
+    float f[16];
+    uint32_t q[4];
+    unpack_codes16(v[i], f);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) q[k] = kv8_code(__fmul_rn(f[k], s_scale[tok]), s);
-    *reinterpret_cast<uint2*>(dst + (int64_t)e * 8) = make_uint2(pack4(q), pack4(q + 4));
+    for (int k = 0; k < 16; ++k) f[k] = __fmul_rn(f[k], s_scale[which][tok]);
+    codes_of(f, s, q);
+    *reinterpret_cast<uint4*>(dst + (int64_t)e * 16) = make_uint4(q[0], q[1], q[2], q[3]);
   }
 }
 
 // ---------------------------------------------------------------------------
 // launches
 // ---------------------------------------------------------------------------
+// Threads that hold a (page, head) tile: kVpt vectors of 8 elements each, or,
+// for keys and values together, of 16.
 static int tile_threads(const Kv8View& c) { return (c.dim << c.page_shift) / (8 * kVpt); }
+
+static int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return 148;
+  return n;
+}
 
 cudaError_t launch_kv8_append(const Kv8View& c, const void* k, const void* v, int dtype, const int64_t* strides,
                               const int32_t* cu, const int32_t* starts, int B, int64_t rows, cudaStream_t st) {
@@ -474,10 +603,9 @@ cudaError_t launch_kv8_gather(const Kv8View& c, const int32_t* starts, const int
   GatherParams p{c, starts, cu, B, rows, {k, v}};
   const int64_t blocks = (rows + kGatherRows - 1) / kGatherRows;
   if (blocks > 0x7FFFFFFF) return cudaErrorInvalidValue;
-  const dim3 grid((unsigned)blocks, 2);
-  if (dtype == PARO_BF16) kv8_gather_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p);
-  else if (dtype == PARO_F16) kv8_gather_kernel<__half><<<grid, 256, 0, st>>>(p);
-  else kv8_gather_kernel<float><<<grid, 256, 0, st>>>(p);
+  if (dtype == PARO_BF16) kv8_gather_kernel<__nv_bfloat16><<<(unsigned)blocks, kGatherThreads, 0, st>>>(p);
+  else if (dtype == PARO_F16) kv8_gather_kernel<__half><<<(unsigned)blocks, kGatherThreads, 0, st>>>(p);
+  else kv8_gather_kernel<float><<<(unsigned)blocks, kGatherThreads, 0, st>>>(p);
   return cudaGetLastError();
 }
 
@@ -485,10 +613,33 @@ cudaError_t launch_kv8_evict(const Kv8View& c, const float* weights, int64_t cap
                              int budget, int sink, int recent, int32_t* kept, float* new_weights, int32_t* new_lens,
                              const int32_t* out_table, int out_width, cudaStream_t st) {
   EvictParams p{c, weights, cap, lens, budget, sink, recent, kept, new_weights, new_lens, out_table, out_width};
-  kv8_select_kernel<<<(unsigned)(B * c.kv_heads), kSelThreads, 0, st>>>(p);
-  if (cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
+  // CTAs to a (sequence, head): as many as the GPU holds at once (four of 512
+  // threads to an SM), at most 8
+  int cs = 1;
+  while (cs < 8 && (int64_t)B * c.kv_heads * cs * 2 <= 4 * sm_count()) cs *= 2;
+  // as many keys in shared memory as a CTA can get, up to 160 KB of them,
+  // and the masks of its run (8 bytes per 32 tokens) up to 40 KB; a longer
+  // run makes them twice
+  const int64_t most = (((int64_t)c.table_width << c.page_shift) + cs * 32 - 1) / (cs * 32) * 32;
+  const int cached = (int)(most < kSelCached ? most : kSelCached);
+  const int with_masks = most / 32 * 8 <= 40 * 1024;
+  const int64_t smem = (int64_t)cached * 4 + (with_masks ? most / 32 * 8 : 0);
+  cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(kv8_select_kernel), (int)smem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(B * c.kv_heads * cs));
+  cfg.blockDim = dim3(kSelThreads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim = {(unsigned)cs, 1, 1};
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  if ((e = cudaLaunchKernelEx(&cfg, kv8_select_kernel, p, cached, with_masks)) != cudaSuccess) return e;
   const int blocks = (budget + (1 << c.page_shift) - 1) >> c.page_shift;
-  kv8_compact_kernel<<<dim3((unsigned)blocks, (unsigned)c.kv_heads, (unsigned)(2 * B)), tile_threads(c), 0, st>>>(p);
+  kv8_compact_kernel<<<dim3((unsigned)blocks, (unsigned)c.kv_heads, (unsigned)B),
+                       tile_threads(c) < 64 ? 64 : tile_threads(c), 0, st>>>(p);   // whole warps for each half
   return cudaGetLastError();
 }
 

@@ -281,3 +281,30 @@ def test_evict_refusals_and_bad_pages():
             bad()
     ops.kv8_evict(w, *cache, table, n, R.i32([[-1, 10 ** 6]]), 20, 0, 0)
     assert ops.device_error_word() & 8
+
+
+@pytest.mark.parametrize("lens,kv_heads", [([45000, 300], 1), ([9000] * 20, 8)])
+def test_evict_split_over_several_blocks_and_not(lens, kv_heads):
+    # few (sequence, head)s share their tokens out to several blocks, many do not
+    g = torch.Generator().manual_seed(60)
+    run_evict(lens, 128, kv_heads, 64, 130, 5, 9,
+              lambda b, h, n: torch.randint(0, 400, (h, n), generator=g).float(), 61)
+
+
+def test_append_codes_are_the_rounded_quotients():
+    # the quotient of every pair of a bf16 value and a page maximum, divided and rounded in float32
+    import alpamayo_b200.ops as ops
+    page = 128
+    g = torch.Generator().manual_seed(62)
+    n = 40 * page
+    *cache, table = R.make_pool([n], page, 1, 128, 63)
+    x = torch.randn(n, 1, 128, generator=g).to(BF16)
+    top = x.view(40, page * 128).abs().amax(-1).float()
+    x.view(40, page, 128)[:, 1, :64] = (top / 127)[:, None].to(BF16) * torch.arange(64).to(BF16)
+    x.view(40, page, 128)[:, 2, 0] = (top * 0.5).to(BF16)
+    ops.kv8_append(x.cuda(), x.cuda(), R.cu([n]), R.i32([0]), *cache, table)
+    s = (x.view(40, page, 128).float().abs().amax((1, 2)) / torch.full((40,), 127.0))
+    want = torch.round(x.view(40, page, 128).float() / s[:, None, None]).to(torch.int8)
+    got = cache[0][table[0].long(), 0].cpu()
+    assert torch.equal(cache[2][table[0].long(), 0].cpu(), s)
+    assert torch.equal(got, want)
