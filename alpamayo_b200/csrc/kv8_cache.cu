@@ -68,34 +68,73 @@ __device__ __forceinline__ void unpack_codes8(uint2 u, float (&f)[8]) {
   }
 }
 
+// Four elements' codes by division, out of line: 16 of these inline per piece
+// of the compaction filled the instruction cache (its largest stall).
+__device__ __noinline__ uint32_t codes_div(float a, float b, float c, float d, float scale) {
+  return (uint32_t)(kv8_code(a, scale) & 0xff) | ((uint32_t)(kv8_code(b, scale) & 0xff) << 8) |
+         ((uint32_t)(kv8_code(c, scale) & 0xff) << 16) | ((uint32_t)(kv8_code(d, scale) & 0xff) << 24);
+}
+
 // Codes of N elements under `scale`, as kv8_code gives them, without a
-// division each: x times the reciprocal is within 2.3e-5 of the rounded
-// quotient (three units in the last place below 128), so both round to the
+// division each: x times the reciprocal is within 1.6e-5 of the rounded
+// quotient (two units in the last place below 128), so both round to the
 // same integer unless the product is that close to the middle between two;
-// those few are divided.  Adding 1.5 * 2^23 rounds to an integer (ties to
-// even) that stands in the low bits.
+// where one is, all N are divided.  Adding 1.5 * 2^23 rounds to an integer
+// (ties to even) that stands in the low bits.
+struct CodeScale {
+  float scale, inv;
+  bool slow;       // reciprocal or quotients out of range, zero, not finite
+  __device__ __forceinline__ explicit CodeScale(float s) : scale(s) {
+    slow = !(s > 1e-30f && s < 1e30f);
+    inv = slow ? 0.f : __fdiv_rn(1.f, s);
+  }
+};
 template <int N>
-__device__ __forceinline__ void codes_of(const float (&x)[N], float scale, uint32_t (&out)[N / 4]) {
-  uint32_t q[N];
-  bool slow = !(scale > 1e-30f && scale < 1e30f);   // reciprocal or quotients out of range, zero, not finite
-  if (!slow) {
-    const float inv = __fdiv_rn(1.f, scale);
-    float far = 0.f;
+__device__ __forceinline__ void codes_of(const float (&x)[N], const CodeScale& cs, uint32_t (&out)[N / 4]) {
+  const float2 inv2 = make_float2(cs.inv, cs.inv), magic = make_float2(12582912.f, 12582912.f);
+  float far = 0.f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float y = __fmul_rn(x[i], inv), z = __fadd_rn(y, 12582912.f);
-      q[i] = __float_as_uint(z);
-      far = fmaxf(far, fabsf(__fadd_rn(y, -__fadd_rn(z, -12582912.f))));
+  for (int i = 0; i < N; i += 4) {
+    uint32_t q[4];
+#pragma unroll
+    for (int k = 0; k < 4; k += 2) {
+      const float2 v = make_float2(x[i + k], x[i + k + 1]);
+      const float2 z = __ffma2_rn(v, inv2, magic);
+      const float2 d = __ffma2_rn(v, inv2, __ffma2_rn(z, make_float2(-1.f, -1.f), magic));   // from the integer
+      q[k] = __float_as_uint(z.x);
+      q[k + 1] = __float_as_uint(z.y);
+      far = fmaxf(far, fmaxf(fabsf(d.x), fabsf(d.y)));
     }
-    slow = far > 0.49996f;
+    out[i / 4] = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
   }
-  if (slow) {
+  if (cs.slow || far > 0.49996f) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) q[i] = (uint32_t)kv8_code(x[i], scale);
+    for (int i = 0; i < N; i += 4) out[i / 4] = codes_div(x[i], x[i + 1], x[i + 2], x[i + 3], cs.scale);
   }
+}
+
+// Running maximum of |x|: of 16-bit types as two 16-bit lanes of a word (the
+// bits of non-negative floats are ordered as integers, NaN above infinity,
+// so a NaN shows in the result), of float32 as a word.
+__device__ __forceinline__ uint32_t absmax8(uint32_t top, const uint4& w) {
+  constexpr uint32_t kAbs = 0x7fff7fffu;
+  return __vmaxu2(__vmaxu2(__vmaxu2(top, w.x & kAbs), __vmaxu2(w.y & kAbs, w.z & kAbs)), w.w & kAbs);
+}
+__device__ __forceinline__ uint32_t absmax(uint32_t top, const Vec8<__nv_bfloat16>& v) { return absmax8(top, v.w); }
+__device__ __forceinline__ uint32_t absmax(uint32_t top, const Vec8<__half>& v) { return absmax8(top, v.w); }
+__device__ __forceinline__ uint32_t absmax(uint32_t top, const Vec8<float>& v) {
+  constexpr uint32_t kAbs = 0x7fffffffu;
 #pragma unroll
-  for (int i = 0; i < N; i += 4)
-    out[i / 4] = __byte_perm(__byte_perm(q[i], q[i + 1], 0x0040), __byte_perm(q[i + 2], q[i + 3], 0x0040), 0x5410);
+  for (int i = 0; i < 2; ++i)
+    top = max(max(max(top, v.w[i].x & kAbs), max(v.w[i].y & kAbs, v.w[i].z & kAbs)), v.w[i].w & kAbs);
+  return top;
+}
+// The same as the bits of a float32.
+template <typename T> __device__ __forceinline__ uint32_t absmax_f32(uint32_t top);
+template <> __device__ __forceinline__ uint32_t absmax_f32<float>(uint32_t top) { return top; }
+template <> __device__ __forceinline__ uint32_t absmax_f32<__nv_bfloat16>(uint32_t top) { return max(top & 0xffffu, top >> 16) << 16; }
+template <> __device__ __forceinline__ uint32_t absmax_f32<__half>(uint32_t top) {
+  return __float_as_uint(fabsf(half_bits_to_f32((uint16_t)max(top & 0xffffu, top >> 16))));
 }
 
 __device__ __forceinline__ uint32_t pack4(const int* c) {
@@ -154,7 +193,7 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(AppendParams p) {
   const int64_t t0 = blk << c.page_shift;               // first token of the page
   const int old = (int)max((int64_t)0, start - t0);     // its tokens that were there before
   const int end = (int)min((int64_t)page, (int64_t)start + n - t0);
-  const int per_tok = c.dim >> 3;                        // vectors per token (8 or 16)
+  const int tok_shift = c.dim == 128 ? 4 : 3;            // 16 or 8 vectors per token
   const T* src = static_cast<const T*>(which ? p.src[1] : p.src[0]);
   const int64_t st = which ? p.stride_t[1] : p.stride_t[0], sh = which ? p.stride_h[1] : p.stride_h[0];
   const int64_t row0 = (int64_t)p.cu[b] + (t0 - start);  // source row of the page's token 0
@@ -163,7 +202,7 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(AppendParams p) {
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < kVpt; ++i) {
-    const int e = i * blockDim.x + threadIdx.x, tok = e / per_tok, d = (e - tok * per_tok) * 8;
+    const int e = i * blockDim.x + threadIdx.x, tok = e >> tok_shift, d = (e - (tok << tok_shift)) * 8;
     if (tok >= old && tok < end) load8(v[i], src + (row0 + tok) * st + h * sh + d);
   }
   if (id < 0 || id >= c.num_pages) {
@@ -176,33 +215,29 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(AppendParams p) {
 #pragma unroll
   for (int i = 0; i < kVpt; ++i) {
     const int e = i * blockDim.x + threadIdx.x;
-    if (e / per_tok < old) prev[i] = *reinterpret_cast<const uint2*>(codes + (int64_t)e * 8);
+    if (e >> tok_shift < old) prev[i] = *reinterpret_cast<const uint2*>(codes + (int64_t)e * 8);
   }
 #pragma unroll
   for (int i = 0; i < kVpt; ++i) {
-    const int tok = (i * blockDim.x + threadIdx.x) / per_tok;
-    if (tok >= old && tok < end) {
-      float f[8];
-      unpack(v[i], f);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(fabsf(f[k])));
-    }
+    const int tok = (i * blockDim.x + threadIdx.x) >> tok_shift;
+    if (tok >= old && tok < end) top = absmax(top, v[i]);
   }
-  float s = __fdiv_rn(block_absmax(top, slots), kKv8Max);
+  float s = __fdiv_rn(block_absmax(absmax_f32<T>(top), slots), kKv8Max);
   // every thread read the prior scale before the barrier inside
   // block_absmax, so thread 0 may overwrite it now
   if (old && !(s > prior) && !isnan(s)) s = prior;
   const float ratio = s > 0.f ? __fdiv_rn(prior, s) : 0.f;
+  const CodeScale cs(s);
   if (threadIdx.x == 0) *scale_at = s;
 #pragma unroll
   for (int i = 0; i < kVpt; ++i) {
-    const int e = i * blockDim.x + threadIdx.x, tok = e / per_tok;
+    const int e = i * blockDim.x + threadIdx.x, tok = e >> tok_shift;
     if (tok >= end) continue;
     float f[8];
     uint32_t q[2];
     if (tok >= old) {
       unpack(v[i], f);
-      codes_of(f, s, q);
+      codes_of(f, cs, q);
     } else {
       if (ratio == 1.f) continue;
       unpack_codes8(prev[i], f);
@@ -233,6 +268,28 @@ __device__ __forceinline__ void unpack_codes16(const uint4& u, float (&f)[16]) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
   for (int i = 0; i < 16; ++i) f[i] = (float)(int8_t)(w[i >> 2] >> (8 * (i & 3)));
+}
+
+__device__ __forceinline__ uint32_t max_s16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.s16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t min_s16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("min.s16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// Largest |code| of 16.  As signed 16-bit lanes a word orders by its odd
+// bytes, shifted left by 8 by its even ones (the byte below only breaks ties).
+__device__ __forceinline__ int code_absmax(const uint4& v) {
+  const uint32_t e[4] = {v.x << 8, v.y << 8, v.z << 8, v.w << 8};
+  const uint32_t hi = max_s16x2(max_s16x2(max_s16x2(v.x, v.y), max_s16x2(v.z, v.w)),
+                                max_s16x2(max_s16x2(e[0], e[1]), max_s16x2(e[2], e[3])));
+  const uint32_t lo = min_s16x2(min_s16x2(min_s16x2(v.x, v.y), min_s16x2(v.z, v.w)),
+                                min_s16x2(min_s16x2(e[0], e[1]), min_s16x2(e[2], e[3])));
+  const int up = max((int)hi >> 24, (int)(hi << 16) >> 24), down = min((int)lo >> 24, (int)(lo << 16) >> 24);
+  return max(up, -down);
 }
 
 template <typename T>
@@ -273,7 +330,7 @@ __global__ void __launch_bounds__(kGatherThreads) kv8_gather_kernel(GatherParams
     s_at[threadIdx.x] = at;
   }
   __syncthreads();
-  const int per_head = c.dim >> 4, per_tok = c.kv_heads * per_head;
+  const int head_shift = c.dim == 128 ? 3 : 2, per_tok = c.kv_heads << head_shift;   // pieces of a head, of a token
   const int rows = (int)min((int64_t)kGatherRows, p.rows - r0), side = rows * per_tok;
   for (int e0 = threadIdx.x; e0 < 2 * side; e0 += kGatherFlight * kGatherThreads) {
     uint4 w[kGatherFlight];
@@ -285,7 +342,7 @@ __global__ void __launch_bounds__(kGatherThreads) kv8_gather_kernel(GatherParams
       s[x] = 0.f;
       if (e < 2 * side) {
         const int which = e >= side, i = e - (which ? side : 0), r = i / per_tok, in_tok = i - r * per_tok;
-        const int h = in_tok / per_head, d = (in_tok - h * per_head) * 16, page = s_page[r];
+        const int h = in_tok >> head_shift, d = (in_tok - (h << head_shift)) * 16, page = s_page[r];
         if (page >= 0) {
           w[x] = *reinterpret_cast<const uint4*>((which ? c.v_codes : c.k_codes) + kv8_base(c, page, h) + s_at[r] * c.dim + d);
           s[x] = (which ? c.v_scale : c.k_scale)[(int64_t)page * c.kv_heads + h];
@@ -500,81 +557,112 @@ __global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(EvictParams p, 
   cluster.sync();          // the other CTAs have read this one's counts
 }
 
-// Grid (destination pages per sequence, kv heads, B).  The first half of a
-// CTA's threads moves the page's keys, the second its values.
-__global__ void __launch_bounds__(512) kv8_compact_kernel(EvictParams p) {
-  __shared__ uint32_t slots[16];
-  __shared__ int64_t s_src[128];       // element offset of the token's row, -1: not a page of the pool
-  __shared__ float s_scale[2][128];
+// One task per (destination page, keys or values, head, sequence), taken by
+// a team of as many warps as its pieces of 16 codes need at 8 to a lane, all
+// of them in flight at once.  With a block of 256 threads per task, an index
+// list in shared memory and two barriers, the same work took 90 us instead of
+// 62 for 64 sequences cut to 2048 tokens.
+constexpr int kCmpThreads = 128;
+constexpr int kCmpPieces = 8;
+
+template <int D>
+__global__ void __launch_bounds__(kCmpThreads) kv8_compact_kernel(EvictParams p, int pages) {
+  constexpr int kShift = D == 128 ? 3 : 2;       // 8 or 4 pieces per token
+  constexpr int kTok = kCmpPieces >> kShift;     // tokens per lane
+  constexpr int kPer = 32 >> kShift;             // tokens per piece index
+  __shared__ uint32_t s_top[kCmpThreads / 32];
   const Kv8View& c = p.c;
-  const int b = blockIdx.z, h = blockIdx.y, blk = blockIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int page = 1 << c.page_shift;
-  const int n = min(kv8_len(c, p.lens[b]), p.budget);
-  const int cnt = min(page, n - blk * page);
-  if (cnt <= 0) return;
-  const int id = p.out_table[(int64_t)b * p.out_width + blk];
-  if (id < 0 || id >= c.num_pages) {
-    if (threadIdx.x == 0) report_error(kErrBadPage);
-    return;
-  }
-  const int32_t* kept = p.kept + ((int64_t)b * c.kv_heads + h) * p.budget + blk * page;
-  for (int t = threadIdx.x; t < cnt; t += blockDim.x) {
-    const int tok = kept[t];
-    const int src = kv8_page(c, b, tok >> c.page_shift);
-    s_src[t] = src < 0 ? -1 : kv8_base(c, src, h) + (int64_t)(tok & (page - 1)) * c.dim;
-    s_scale[0][t] = src < 0 ? 0.f : c.k_scale[(int64_t)src * c.kv_heads + h];
-    s_scale[1][t] = src < 0 ? 0.f : c.v_scale[(int64_t)src * c.kv_heads + h];
-  }
-  __syncthreads();
-  const int half = blockDim.x >> 1, which = threadIdx.x >= half, tid = threadIdx.x - (which ? half : 0);
-  const int8_t* codes = which ? c.v_codes : c.k_codes;
-  const int per_tok = c.dim >> 4;
-  uint4 v[kVpt];
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < kVpt; ++i) {
-    const int e = i * half + tid, tok = e / per_tok, d = (e - tok * per_tok) * 16;
-    v[i] = make_uint4(0u, 0u, 0u, 0u);
-    if (tok < cnt && s_src[tok] >= 0) v[i] = *reinterpret_cast<const uint4*>(codes + s_src[tok] + d);
-  }
-#pragma unroll
-  for (int i = 0; i < kVpt; ++i) {
-    const int tok = (i * half + tid) / per_tok;
-    if (tok < cnt) {
-      // |code * scale| is largest where |code| is
-      const uint32_t a = __vmaxu4(__vabs4(v[i].x), __vabs4(v[i].y)), bb = __vmaxu4(__vabs4(v[i].z), __vabs4(v[i].w));
-      uint32_t m = __vmaxu4(a, bb);
-      m = max(max(m & 0xffu, (m >> 8) & 0xffu), max((m >> 16) & 0xffu, m >> 24));
-      top = max(top, __float_as_uint(fabsf(__fmul_rn((float)m, s_scale[which][tok]))));
+  // log2 of the warps to a task: 1, 2 or 4 of them
+  const int team_shift = max(0, c.page_shift + kShift - 8), team = 1 << team_shift;
+  static_assert(32 * kCmpPieces == 256, "2^8 pieces to a warp");
+  const int task = (blockIdx.x * (kCmpThreads / 32) + warp) >> team_shift, which = task & 1, blk = task >> 1;
+  const int h = blockIdx.y, b = blockIdx.z, bh = b * c.kv_heads + h;
+  int cnt = 0, id = -1;
+  if (blk < pages) {
+    id = p.out_table[(int64_t)b * p.out_width + blk];
+    cnt = min(page, min(kv8_len(c, p.lens[b]), p.budget) - blk * page);
+    if (cnt > 0 && (id < 0 || id >= c.num_pages)) {
+      report_error(kErrBadPage);
+      cnt = 0;
     }
   }
-  top = __reduce_max_sync(0xffffffffu, top);
-  if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = top;
-  __syncthreads();
-  const int warps = half >> 5;
-  for (int x = 0; x < warps; ++x) top = max(top, slots[which * warps + x]);
-  const float s = __fdiv_rn(__uint_as_float(top), kKv8Max);
-  int8_t* dst = (which ? c.v_codes : c.k_codes) + kv8_base(c, id, h);
-  if (tid == 0) (which ? c.v_scale : c.k_scale)[(int64_t)id * c.kv_heads + h] = s;
+  const int share = page >> team_shift, first = (warp & (team - 1)) * share;             // this warp's tokens of the page
+  const int mine = max(0, min(share, cnt - first));
+  const float* scales = which ? c.v_scale : c.k_scale;
+  const int8_t* codes = which ? c.v_codes : c.k_codes;
+  // lane l knows the source rows of the warp's tokens l, l + 32, ...
+  int src_page[kTok], src_at[kTok];
+  float src_scale[kTok];
 #pragma unroll
-  for (int i = 0; i < kVpt; ++i) {
-    const int e = i * half + tid, tok = e / per_tok;
-    if (tok >= cnt) continue;
+  for (int x = 0; x < kTok; ++x) {
+    const int t = x * 32 + lane;
+    src_at[x] = t < mine ? p.kept[(int64_t)bh * p.budget + blk * page + first + t] : 0;
+  }
+#pragma unroll
+  for (int x = 0; x < kTok; ++x) {
+    src_page[x] = x * 32 + lane < mine ? kv8_page(c, b, src_at[x] >> c.page_shift) : -1;
+    src_at[x] &= page - 1;
+  }
+#pragma unroll
+  for (int x = 0; x < kTok; ++x)
+    src_scale[x] = src_page[x] >= 0 ? scales[(int64_t)src_page[x] * c.kv_heads + h] : 0.f;
+  // piece i of a lane belongs to token (i * 32 + lane) >> kShift, known to
+  // lane (token & 31) as its token x(i)
+  auto owner = [&](int i) { return ((i * 32 + lane) >> kShift) & 31; };
+  uint4 v[kCmpPieces];
+#pragma unroll
+  for (int i = 0; i < kCmpPieces; ++i) {
+    v[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (i * kPer >= share) continue;
+    const int x = i * kPer / 32;
+    const int pg = __shfl_sync(0xffffffffu, src_page[x], owner(i)), at = __shfl_sync(0xffffffffu, src_at[x], owner(i));
+    if (pg >= 0)
+      v[i] = *reinterpret_cast<const uint4*>(codes + kv8_base(c, pg, h) + at * D + (lane & ((1 << kShift) - 1)) * 16);
+  }
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < kCmpPieces; ++i) {
+    if (i * kPer >= share) break;
+    const float sc = __shfl_sync(0xffffffffu, src_scale[i * kPer / 32], owner(i));
+    // |code * scale| is largest where |code| is
+    top = max(top, __float_as_uint(fabsf(__fmul_rn((float)code_absmax(v[i]), sc))));
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (team > 1) {
+    if (lane == 0) s_top[warp] = top;
+    named_barrier(1 + (warp >> team_shift), 32 * team);
+    for (int x = 0; x < team; ++x) top = max(top, s_top[(warp & ~(team - 1)) + x]);
+  }
+  if (cnt <= 0) return;
+  const float s = __fdiv_rn(__uint_as_float(top), kKv8Max);
+  const CodeScale cs(s);
+  int8_t* dst = (which ? c.v_codes : c.k_codes) + kv8_base(c, id, h) + (int64_t)first * D;
+  if (lane == 0 && first == 0) (which ? c.v_scale : c.k_scale)[(int64_t)id * c.kv_heads + h] = s;
+#pragma unroll
+  for (int i = 0; i < kCmpPieces; ++i) {
+    if (i * kPer >= share) break;
+    const float sc = __shfl_sync(0xffffffffu, src_scale[i * kPer / 32], owner(i));
     float f[16];
     uint32_t q[4];
     unpack_codes16(v[i], f);
 #pragma unroll
-    for (int k = 0; k < 16; ++k) f[k] = __fmul_rn(f[k], s_scale[which][tok]);
-    codes_of(f, s, q);
-    *reinterpret_cast<uint4*>(dst + (int64_t)e * 16) = make_uint4(q[0], q[1], q[2], q[3]);
+    for (int k = 0; k < 16; k += 2) {
+      const float2 y = __fmul2_rn(make_float2(f[k], f[k + 1]), make_float2(sc, sc));
+      f[k] = y.x;
+      f[k + 1] = y.y;
+    }
+    codes_of(f, cs, q);
+    if ((i * 32 + lane) >> kShift < mine)
+      *reinterpret_cast<uint4*>(dst + (int64_t)(i * 32 + lane) * 16) = make_uint4(q[0], q[1], q[2], q[3]);
   }
 }
 
 // ---------------------------------------------------------------------------
 // launches
 // ---------------------------------------------------------------------------
-// Threads that hold a (page, head) tile: kVpt vectors of 8 elements each, or,
-// for keys and values together, of 16.
+// Threads that hold a (page, head) tile, kVpt vectors of 8 elements each.
 static int tile_threads(const Kv8View& c) { return (c.dim << c.page_shift) / (8 * kVpt); }
 
 static int sm_count() {
@@ -613,10 +701,10 @@ cudaError_t launch_kv8_evict(const Kv8View& c, const float* weights, int64_t cap
                              int budget, int sink, int recent, int32_t* kept, float* new_weights, int32_t* new_lens,
                              const int32_t* out_table, int out_width, cudaStream_t st) {
   EvictParams p{c, weights, cap, lens, budget, sink, recent, kept, new_weights, new_lens, out_table, out_width};
-  // CTAs to a (sequence, head): as many as the GPU holds at once (four of 512
-  // threads to an SM), at most 8
+  // CTAs to a (sequence, head): as many as the GPU holds at once (two to an
+  // SM, by registers), at most 8
   int cs = 1;
-  while (cs < 8 && (int64_t)B * c.kv_heads * cs * 2 <= 4 * sm_count()) cs *= 2;
+  while (cs < 8 && (int64_t)B * c.kv_heads * cs * 2 <= 2 * sm_count()) cs *= 2;
   // as many keys in shared memory as a CTA can get, up to 160 KB of them,
   // and the masks of its run (8 bytes per 32 tokens) up to 40 KB; a longer
   // run makes them twice
@@ -638,8 +726,11 @@ cudaError_t launch_kv8_evict(const Kv8View& c, const float* weights, int64_t cap
   cfg.numAttrs = 1;
   if ((e = cudaLaunchKernelEx(&cfg, kv8_select_kernel, p, cached, with_masks)) != cudaSuccess) return e;
   const int blocks = (budget + (1 << c.page_shift) - 1) >> c.page_shift;
-  kv8_compact_kernel<<<dim3((unsigned)blocks, (unsigned)c.kv_heads, (unsigned)B),
-                       tile_threads(c) < 64 ? 64 : tile_threads(c), 0, st>>>(p);   // whole warps for each half
+  const int pieces = (c.dim << c.page_shift) / 16, team = pieces > 32 * kCmpPieces ? pieces / (32 * kCmpPieces) : 1;
+  const int64_t ctas = ((int64_t)blocks * 2 * team + kCmpThreads / 32 - 1) / (kCmpThreads / 32);
+  const dim3 grid((unsigned)ctas, (unsigned)c.kv_heads, (unsigned)B);
+  if (c.dim == 128) kv8_compact_kernel<128><<<grid, kCmpThreads, 0, st>>>(p, blocks);
+  else kv8_compact_kernel<64><<<grid, kCmpThreads, 0, st>>>(p, blocks);
   return cudaGetLastError();
 }
 
