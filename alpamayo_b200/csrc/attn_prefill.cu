@@ -41,6 +41,7 @@ PARO_DEFINE_ERROR_ACCESSOR(attn)
 
 constexpr int kPfRows = 128;       // query rows per tile, keys per tile
 constexpr int kPfThreads = 384;
+constexpr int kPolyOf32 = 0;       // exponentials of 32 that go through the FMA units (an even number)
 constexpr int kPfMasked = 3;       // key tiles that a CTA's rows see in part, at most
 
 struct PrefillParams {
@@ -77,27 +78,50 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32
       "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]), "r"(taddr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+      ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+      "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// The MMA warp runs as a whole and issues under a predicate that one lane
+// has: in code that only one lane executes, every descriptor has to be moved
+// to the uniform registers that tcgen05 instructions take, some 100 clocks
+// per MMA (measured), against the 64 that it executes for.
+
 // D[tmem] (+)= A[smem] * B[smem], one CTA
-__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc,
+                                           uint32_t leader) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(leader)
       : "memory");
 }
 // D[tmem] (+)= A[tmem] * B[smem]
-__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc,
+                                           uint32_t leader) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(
-          d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(leader)
       : "memory");
 }
-// Arrives on `bar` when every tcgen05 operation issued so far by this thread is done.
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
+// Arrives on `bar` when every tcgen05 operation issued so far by the leader is done.
+__device__ __forceinline__ void umma_commit(uint64_t* bar, uint32_t leader) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar)),
+      "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(r));
+  return r;
 }
 
 // MN-major operand with 128-byte swizzle: 64 columns (128 bytes) by 8 rows
@@ -106,6 +130,29 @@ __device__ __forceinline__ void umma_commit(uint64_t* bar) {
 __device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t saddr) {
   return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)((kPfRows * 128) >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
          ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+// 2^x of a pair without the exp2 unit, for x <= 15: x = n + f with n the
+// nearest integer (it stands in the low bits of x + 1.5 * 2^23) and |f| <=
+// 1/2; 2^f by the polynomial of degree 4 with value 1 at 0 whose largest
+// relative error is smallest (2.9e-6 in float32 arithmetic; coefficients from
+// a Lawson iteration on a fine grid); n is added to the exponent.  Below
+// -127 the result is +0.
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+  x.x = fmaxf(x.x, -127.f);
+  x.y = fmaxf(x.y, -127.f);
+  const float2 magic = make_float2(12582912.f, 12582912.f);
+  const float2 t = __fadd2_rn(x, magic);
+  const float2 n = __ffma2_rn(t, make_float2(-1.f, -1.f), magic);   // minus the integer
+  const float2 f = __fadd2_rn(x, n);
+  float2 r = __ffma2_rn(f, make_float2(0.009582854807376862f, 0.009582854807376862f),
+                        make_float2(0.05590642988681793f, 0.05590642988681793f));
+  r = __ffma2_rn(r, f, make_float2(0.24024099111557007f, 0.24024099111557007f));
+  r = __ffma2_rn(r, f, make_float2(0.6931241750717163f, 0.6931241750717163f));
+  r = __ffma2_rn(r, f, make_float2(1.f, 1.f));
+  r.x = __uint_as_float(__float_as_uint(r.x) + (__float_as_uint(t.x) << 23));
+  r.y = __uint_as_float(__float_as_uint(r.y) + (__float_as_uint(t.y) << 23));
+  return r;
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -157,8 +204,8 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
   uint64_t* full = q_full + 2;                                        // [slots] a K or V tile has landed
   uint64_t* empty = full + C::kSlots;                                 // [slots] its MMAs are done
   uint64_t* s_full = empty + C::kSlots;                               // [2] scores ready (and O up to date)
-  uint64_t* p_ready = s_full + 2;                                     // [2] probabilities written
-  uint64_t* o_full = p_ready + 2;                                     // [2] output complete
+  uint64_t* p_ready = s_full + 2;                                     // [2][2] half a tile's probabilities written
+  uint64_t* o_full = p_ready + 4;                                     // [2] output complete
   uint64_t* v_full = o_full + 2;                                      // [3] partly seen value tile has landed
   uint64_t* v_ok = v_full + kPfMasked;                                // [3] ... and is cleaned
   uint64_t* done = v_ok + kPfMasked;                                  // [1] every MMA is done
@@ -231,7 +278,8 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
     for (int s = 0; s < 2; ++s) {
       mbar_init(&q_full[s], 1);
       mbar_init(&s_full[s], 1);
-      mbar_init(&p_ready[s], 4);
+      mbar_init(&p_ready[2 * s], 4);
+      mbar_init(&p_ready[2 * s + 1], 4);
       mbar_init(&o_full[s], 1);
     }
     for (int i = 0; i < C::kSlots; ++i) {
@@ -288,57 +336,90 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
                   (i & 1) && (i >> 1) >= jm ? 0 : (i / C::kSlots) & 1);
       if (nk[0]) mbar_wait(&q_full[0], 0);
       if (nk[1] && n > 0) mbar_wait(&q_full[1], 0);
-    } else if (warp == 9 && lane == 0) {
+    } else if (warp == 9) {
       constexpr uint32_t kFmt = (1u << 4) | (Type16<T>::kFmt << 7) | (Type16<T>::kFmt << 10) |
                                 ((uint32_t)(kPfRows >> 4) << 24);
       constexpr uint32_t kIdS = kFmt | ((uint32_t)(kPfRows >> 3) << 17);
       constexpr uint32_t kIdO = kFmt | (1u << 16) | ((uint32_t)(D >> 3) << 17);   // B is MN-major
-      const uint32_t q_at = smem_u32(smem), kv_at = smem_u32(smem + C::kOffKv);
-      auto scores = [&](int s, int j) {        // S_s = Q_s K_j^T
-        const uint64_t da = umma_desc_sw128(q_at + s * C::kTileBytes);
-        const uint64_t db = umma_desc_sw128(kv_at + ((2 * j) % C::kSlots) * C::kTileBytes);
+      const uint32_t leader = elect_one();
+      // warp-uniform copies of what the loop depends on
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), base = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
+      const int un[2] = {__shfl_sync(0xffffffffu, nk[0], 0), __shfl_sync(0xffffffffu, nk[1], 0)};
+      const int umax = max(un[0], un[1]), um = __shfl_sync(0xffffffffu, jm, 0);
+      const uint64_t dq = umma_desc_sw128(base), dk = umma_desc_sw128(base + C::kOffKv), dv = umma_desc_mn_sw128(base + C::kOffKv);
+      constexpr uint32_t kStep = C::kTileBytes >> 4;
+      auto scores = [&](int s, uint32_t slot) {            // S_s = Q_s K^T, K in ring slot `slot`
+        const uint64_t da = dq + s * kStep, db = dk + slot * kStep;
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const uint32_t o = ((k >> 2) * (kPfRows * 128) + (k & 3) * 32) >> 4;
-          mma_f16_ss(tmem + s * kPfRows, da + o, db + o, kIdS, k > 0);
+          mma_f16_ss(tm + s * kPfRows, da + o, db + o, kIdS, k > 0, leader);
         }
-        umma_commit(&s_full[s]);
+        umma_commit(&s_full[s], leader);
       };
-      auto values = [&](int s, int j) {        // O_s += P_s V_j
-        const uint64_t db = umma_desc_mn_sw128(kv_at + ((2 * j + 1) % C::kSlots) * C::kTileBytes);
+      auto values = [&](int s, uint32_t slot, int half, uint32_t acc) {   // O_s += P_s V, one half of the keys
+        const uint64_t db = dv + slot * kStep;
 #pragma unroll
-        for (int k = 0; k < kPfRows / 16; ++k)
-          mma_f16_ts(tmem + C::kTmemO + s * 128, tmem + s * kPfRows + k * 8, db + k * (2048 >> 4), kIdO, j > 0 || k > 0);
+        for (int i = 0; i < kPfRows / 32; ++i) {
+          const int k = half * (kPfRows / 32) + i;
+          mma_f16_ts(tm + C::kTmemO + s * 128, tm + s * kPfRows + k * 8, db + k * (2048 >> 4), kIdO, acc | (k > 0), leader);
+        }
       };
-      auto landed = [&](int n) { return mbar_wait(&full[n % C::kSlots], (n / C::kSlots) & 1); };
-      if (!landed(0)) failed = true;
-      for (int s = 0; s < 2 && !failed; ++s) {
-        if (!nk[s]) continue;
-        if (!mbar_wait(&q_full[s], 0)) failed = true;
-        else scores(s, 0);
-      }
-      if (!failed) umma_commit(&empty[0]);
-      for (int j = 0; j < nmax && !failed; ++j) {
-        if (!(j < jm ? landed(2 * j + 1) : mbar_wait(&v_ok[j - jm], 0)) || (j + 1 < nmax && !landed(2 * j + 2))) {
-          failed = true;
-          break;
+      // ring slot and phase of the tile that is waited for next
+      uint32_t slot = 0, phase = 0;
+      auto advance = [&]() {
+        if (++slot == (uint32_t)C::kSlots) {
+          slot = 0;
+          phase ^= 1;
         }
+      };
+      // V_j and, unless it is the last, K_(j + 1) are in their slots
+      uint32_t vslot = 0, kslot = 0;
+      auto landed = [&](int j, uint32_t& v, uint32_t& k) {
+        v = slot;
+        bool r = j < um ? mbar_wait(&full[slot], phase) : mbar_wait(&v_ok[j - um], 0);
+        advance();
+        k = slot;
+        if (r && j + 1 < umax) r = mbar_wait(&full[slot], phase);
+        advance();
+        return r;
+      };
+      bool ok = mbar_wait(&full[0], 0);
+      advance();
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (ok && un[s]) {
+          ok = mbar_wait(&q_full[s], 0);
+          if (ok) scores(s, 0);
+        }
+      if (ok) umma_commit(&empty[0], leader);
+      ok = ok && landed(0, vslot, kslot);
+      for (int j = 0; j < umax && ok; ++j) {
+        uint32_t vnext = 0, knext = 0;
+#pragma unroll
         for (int s = 0; s < 2; ++s) {
-          if (j >= nk[s]) continue;
-          if (!mbar_wait(&p_ready[s], j & 1)) {
-            failed = true;
-            break;
+          if (j < un[s] && ok) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              ok = ok && mbar_wait(&p_ready[2 * s + half], j & 1);
+              tc_fence_after();
+              if (ok) values(s, vslot, half, j > 0);
+            }
+            if (ok) {
+              if (j + 1 < un[s]) scores(s, kslot);
+              else umma_commit(&o_full[s], leader);
+            }
           }
-          tc_fence_after();
-          values(s, j);
-          if (j + 1 < nk[s]) scores(s, j + 1);
-          else umma_commit(&o_full[s]);
+          // the next tiles are waited for while the tensor core is busy
+          if (s == 0 && ok && j + 1 < umax) ok = landed(j + 1, vnext, knext);
         }
-        if (failed) break;
-        umma_commit(&empty[(2 * j + 1) % C::kSlots]);
-        if (j + 1 < nmax) umma_commit(&empty[(2 * j + 2) % C::kSlots]);
+        if (!ok) break;
+        umma_commit(&empty[vslot], leader);
+        if (j + 1 < umax) umma_commit(&empty[kslot], leader);
+        vslot = vnext;
+        kslot = knext;
       }
-      umma_commit(done);                       // the tensor memory is not freed under an MMA
+      umma_commit(done, leader);               // the tensor memory is not freed under an MMA
       mbar_wait(done, 0);
     } else if (warp >= 10) {
       for (int j = jm; j < nmax; ++j) {
@@ -389,22 +470,25 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
       }
       tc_fence_after();
       uint32_t x[4][32];
+      const int here = see - j * kPfRows;
+      const bool masked = (j + 1) * kPfRows > seen_by_all;
+      float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, x[c]);
       tmem_wait_ld();
-      const int here = see - j * kPfRows;
-      if ((j + 1) * kPfRows > seen_by_all) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+      for (int c = 0; c < 4; ++c) {
+        if (masked) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) x[c][i] = c * 32 + i < here ? x[c][i] : 0xff800000u;
+        }
+#pragma unroll
+        for (int i = 0; i < 32; i += 8)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            top4[k] = fmaxf(fmaxf(top4[k], __uint_as_float(x[c][i + 2 * k])), __uint_as_float(x[c][i + 2 * k + 1]));
       }
-      float top = -INFINITY;
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int i = 0; i < 32; i += 2)
-          top = fmaxf(fmaxf(top, __uint_as_float(x[c][i])), __uint_as_float(x[c][i + 1]));
+      const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
       // a new reference maximum where the terms would pass 2^8
       const bool grow = top > m && (m == -INFINITY || (top - m) * scale > 8.f);
       if (__any_sync(0xffffffffu, grow)) {
@@ -414,19 +498,22 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
           sum *= a;
         }
         if (j > 0) {
-#pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(t_o + c * 32, o);
+#pragma unroll 1
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld16(t_o + c * 16, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
-            tmem_st32(t_o + c * 32, o);
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
+            tmem_st16(t_o + c * 16, o);
           }
         }
       }
       const float neg = m == -INFINITY ? 0.f : Type16<T>::kShift - m * scale;
-      float part[4] = {0.f, 0.f, 0.f, 0.f};
+      const float2 scale2 = make_float2(scale, scale), neg2 = make_float2(neg, neg);
+      float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      // the first half of the keys goes to the tensor core while the second
+      // half's exponentials are computed
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         uint32_t w[32];
@@ -434,19 +521,19 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
         for (int c = 0; c < 2; ++c)
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
-            const float e0 = ex2(fmaf(__uint_as_float(x[half * 2 + c][i]), scale, neg));
-            const float e1 = ex2(fmaf(__uint_as_float(x[half * 2 + c][i + 1]), scale, neg));
-            part[(i >> 1) & 1] += e0;
-            part[2 + ((i >> 1) & 1)] += e1;
-            w[c * 16 + (i >> 1)] = pack16<T>(e0, e1);
+            const float2 v = __ffma2_rn(
+                make_float2(__uint_as_float(x[half * 2 + c][i]), __uint_as_float(x[half * 2 + c][i + 1])), scale2, neg2);
+            const float2 e = i % 32 < kPolyOf32 ? ex2_poly(v) : make_float2(ex2(v.x), ex2(v.y));
+            part[(i >> 1) & 1] = __fadd2_rn(part[(i >> 1) & 1], e);
+            w[c * 16 + (i >> 1)] = pack16<T>(e.x, e.y);
           }
         tmem_st32(t_s + half * 32, w);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_ready[2 * s + half]);
       }
-      sum += (part[0] + part[1]) + (part[2] + part[3]);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_ready[s]);
+      sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
     }
     const bool live = row < lq;
     T* dst = out + ((int64_t)(q0 + row) * p.heads + h) * D;
