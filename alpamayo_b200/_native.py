@@ -95,6 +95,9 @@ def capi() -> ctypes.CDLL:
         "paro_silu_mul": (i32, [vp, i64, i32, vp, vp]),
         "paro_attention_prefill": (i32, [vp, vp, vp, i32, vp, vp, vp, i32, i64, i64, i32, i32, i32, ctypes.c_float,
                                          vp, vp]),
+        "paro_attention_prefill_workspace_size": (sz, [i32, i64, i64, i32, i32]),
+        "paro_attention_prefill_ws": (i32, [vp, vp, vp, i32, vp, vp, vp, i32, i64, i64, i32, i32, i32, ctypes.c_float,
+                                            vp, vp, sz, vp]),
         "paro_kv8_append": (i32, [vp, vp, i32, vp, vp, i32, vp, vp, vp, i32, i64, vp]),
         "paro_kv8_gather": (i32, [vp, vp, i32, vp, vp, i32, i64, vp, vp, i32, vp]),
         "paro_attention_kv8_workspace_size": (sz, [vp, i32, i32, i32, i32, i32]),

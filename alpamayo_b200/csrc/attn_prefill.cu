@@ -41,7 +41,7 @@ PARO_DEFINE_ERROR_ACCESSOR(attn)
 
 constexpr int kPfRows = 128;       // query rows per tile, keys per tile
 constexpr int kPfThreads = 384;
-constexpr int kPolyOf32 = 0;       // exponentials of 32 that go through the FMA units (an even number)
+constexpr int kPfSplits = 8;       // splits of an item's keys, at most
 constexpr int kPfMasked = 3;       // key tiles that a CTA's rows see in part, at most
 
 struct PrefillParams {
@@ -53,6 +53,9 @@ struct PrefillParams {
   void* out;
   const void* v;                   // for the values that are not finite
   int64_t sv_t, sv_h;
+  int splits;                      // CTAs that share the keys of one item; > 1: partial results
+  float* part_o;                   // [splits][rows][heads][dim] sums of terms times values
+  float2* part_ml;                 // [splits][rows][heads] (reference maximum, sum of terms), in log2 units
 };
 
 template <int D>
@@ -132,29 +135,6 @@ __device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t saddr) {
          ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
-// 2^x of a pair without the exp2 unit, for x <= 15: x = n + f with n the
-// nearest integer (it stands in the low bits of x + 1.5 * 2^23) and |f| <=
-// 1/2; 2^f by the polynomial of degree 4 with value 1 at 0 whose largest
-// relative error is smallest (2.9e-6 in float32 arithmetic; coefficients from
-// a Lawson iteration on a fine grid); n is added to the exponent.  Below
-// -127 the result is +0.
-__device__ __forceinline__ float2 ex2_poly(float2 x) {
-  x.x = fmaxf(x.x, -127.f);
-  x.y = fmaxf(x.y, -127.f);
-  const float2 magic = make_float2(12582912.f, 12582912.f);
-  const float2 t = __fadd2_rn(x, magic);
-  const float2 n = __ffma2_rn(t, make_float2(-1.f, -1.f), magic);   // minus the integer
-  const float2 f = __fadd2_rn(x, n);
-  float2 r = __ffma2_rn(f, make_float2(0.009582854807376862f, 0.009582854807376862f),
-                        make_float2(0.05590642988681793f, 0.05590642988681793f));
-  r = __ffma2_rn(r, f, make_float2(0.24024099111557007f, 0.24024099111557007f));
-  r = __ffma2_rn(r, f, make_float2(0.6931241750717163f, 0.6931241750717163f));
-  r = __ffma2_rn(r, f, make_float2(1.f, 1.f));
-  r.x = __uint_as_float(__float_as_uint(r.x) + (__float_as_uint(t.x) << 23));
-  r.y = __uint_as_float(__float_as_uint(r.y) + (__float_as_uint(t.y) << 23));
-  return r;
-}
-
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -211,50 +191,69 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
   uint64_t* done = v_ok + kPfMasked;                                  // [1] every MMA is done
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   uint32_t* poison = tmem_slot + 1;                                   // [3][4] keys with values that are not finite
+  // the item, for the softmax warps: read where it is used, so that it takes
+  // no registers in their loop (a few spilled ones there cost 4 %)
+  volatile int* ctx = reinterpret_cast<volatile int*>(poison + 4 * kPfMasked);
+  enum { kCtxQ0, kCtxLq, kCtxR0, kCtxH, kCtxOff, kCtxLk, kCtxJm, kCtxK0, kCtxNk };
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int h = blockIdx.x % p.heads, hk = h / p.group;
-  const int slot = blockIdx.x / p.heads;
-
-  // this CTA's rows: sequence b, rows r0 .. of it, the last ones first (the
-  // longest work starts earliest); b = B: rows behind the last sequence
-  int64_t first = 0;
-  int b = -1;
+  if (threadIdx.x == 256) {   // the tensor maps' descriptors, fetched while the item is found
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&qmap) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
+  }
+  // This CTA's item: rows r0 .. of sequence b, head h.  Items are taken in
+  // order of the tile's place in its sequence, the last places of all
+  // sequences first (they see the most keys, and the longest work starts
+  // earliest).  left(t) items lie at place t or later; b = B stands for the
+  // rows behind the last sequence.
+  const int split = blockIdx.x % p.splits;
+  const int item = blockIdx.x / p.splits;
+  auto tiles_of = [&](int i) {
+    if (i > p.B) return 0;
+    const int lo = min(max(p.cu_q[i], 0), p.rows), hi = i < p.B ? min(max(p.cu_q[i + 1], lo), p.rows) : p.rows;
+    return (hi - lo + 2 * kPfRows - 1) / (2 * kPfRows);
+  };
+  const int mine0 = tiles_of(lane);            // sequences 0 .. 31 are kept in registers
+  auto left = [&](int t) {
+    int n = max(0, mine0 - t);
+    for (int b0 = 32; b0 <= p.B; b0 += 32) n += max(0, tiles_of(b0 + lane) - t);
+    return __reduce_add_sync(0xffffffffu, n);
+  };
+  int place = 0, b = -1, h = 0;
   {
-    int64_t before = 0;
+    if (item >= left(0) * p.heads) return;
+    int most = mine0;
+    for (int b0 = 32; b0 <= p.B; b0 += 32) most = max(most, tiles_of(b0 + lane));
+    int hi = __reduce_max_sync(0xffffffffu, most);   // left(hi) = 0
+    while (hi - place > 1) {                         // the largest place with left(place) * heads > item
+      const int mid = (place + hi) >> 1;
+      if (left(mid) * p.heads > item) place = mid;
+      else hi = mid;
+    }
+    const int rest = item - left(place + 1) * p.heads;
+    int nth = rest / p.heads;                        // of the sequences that have such a place
+    h = rest - nth * p.heads;
     for (int b0 = 0; b0 <= p.B && b < 0; b0 += 32) {
-      const int i = b0 + lane;
-      int64_t mine = 0;
-      if (i <= p.B) {
-        const int lo = min(max(p.cu_q[i], 0), p.rows), hi = i < p.B ? min(max(p.cu_q[i + 1], lo), p.rows) : p.rows;
-        mine = (hi - lo + 2 * kPfRows - 1) / (2 * kPfRows);
+      unsigned has = __ballot_sync(0xffffffffu, (b0 ? tiles_of(b0 + lane) : mine0) > place);
+      if (nth >= __popc(has)) {
+        nth -= __popc(has);
+        continue;
       }
-      int64_t incl = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += up;
-      }
-      const unsigned hit = __ballot_sync(0xffffffffu, before + incl > slot);
-      if (hit) {
-        const int src = __ffs(hit) - 1;
-        b = b0 + src;
-        first = before + __shfl_sync(0xffffffffu, incl - mine, src);
-      }
-      before += __shfl_sync(0xffffffffu, incl, 31);
+      for (; nth > 0; --nth) has &= has - 1;
+      b = b0 + __ffs(has) - 1;
     }
   }
-  if (b < 0) return;
+  const int hk = h / p.group;
   const int q0 = min(max(p.cu_q[b], 0), p.rows);
   const int lq = (b < p.B ? min(max(p.cu_q[b + 1], q0), p.rows) : p.rows) - q0;
-  const int k0 = b < p.B ? min(max(p.cu_k[b], 0), p.k_rows) : 0;
-  const int lk = b < p.B ? min(max(p.cu_k[b + 1], k0), p.k_rows) - k0 : 0;
+  int k0 = b < p.B ? min(max(p.cu_k[b], 0), p.k_rows) : 0;
+  int lk = b < p.B ? min(max(p.cu_k[b + 1], k0), p.k_rows) - k0 : 0;
   if (threadIdx.x == 0 && b < p.B && (q0 != p.cu_q[b] || lq != p.cu_q[b + 1] - q0 || k0 != p.cu_k[b] ||
                                       lk != p.cu_k[b + 1] - k0))
     report_error(kErrBadPage);
-  const int tiles_q = (lq + 2 * kPfRows - 1) / (2 * kPfRows);
-  const int r0 = (tiles_q - 1 - (int)(slot - first)) * 2 * kPfRows;
-  const int off = lk - lq;                                 // row i sees keys j <= i + off
+  const int r0 = place * 2 * kPfRows;
+  int off = lk - lq;                                 // row i sees keys j <= i + off
   // key tiles of each row tile (0: no rows, or none that sees a key)
   int nk[2];
 #pragma unroll
@@ -262,11 +261,25 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
     const int begin = r0 + s * kPfRows, end = min(lq, begin + kPfRows);
     nk[s] = begin < lq && end + off > 0 ? (end + off + kPfRows - 1) / kPfRows : 0;
   }
+  T* out = static_cast<T*>(p.out);
+  // this split's key tiles are j0 .. : from here on keys are counted from there
+  if (p.splits > 1) {
+    const int all = max(nk[0], nk[1]), share = (all + p.splits - 1) / p.splits, j0 = min(all, split * share);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) nk[s] = max(0, min(nk[s], j0 + share) - j0);
+    k0 += j0 * kPfRows;
+    lk -= j0 * kPfRows;
+    off -= j0 * kPfRows;
+  }
   const int nmax = max(nk[0], nk[1]);
   const int jm = min(nmax, max(0, (r0 + off + 1) / kPfRows));   // tiles from jm on are seen in part by some row
-  T* out = static_cast<T*>(p.out);
   if (nmax == 0) {                                         // nothing to see: zeros
     const int n = min(2 * kPfRows, lq - r0);
+    if (p.splits > 1) {
+      for (int r = threadIdx.x; r < n; r += kPfThreads)
+        p.part_ml[((int64_t)split * p.rows + q0 + r0 + r) * p.heads + h] = make_float2(-INFINITY, 0.f);
+      return;
+    }
     for (int e = threadIdx.x; e < n * (D / 8); e += kPfThreads) {
       const int r = e / (D / 8), d = (e - r * (D / 8)) * 8;
       *reinterpret_cast<uint4*>(out + ((int64_t)(q0 + r0 + r) * p.heads + h) * D + d) = make_uint4(0u, 0u, 0u, 0u);
@@ -274,7 +287,14 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
     return;
   }
 
-  if (threadIdx.x == 0) {
+  // the loader's thread sets up the barriers and starts the first copies
+  // before the CTA meets
+  auto load = [&](const CUtensorMap* map, uint8_t* dst, int head, int row, uint64_t* bar) {
+    mbar_arrive_expect_tx(bar, C::kTileBytes);
+#pragma unroll
+    for (int a = 0; a < C::kAtoms; ++a) tma_load_3d(dst + a * kPfRows * 128, map, a * 64, head, row, bar);
+  };
+  if (threadIdx.x == 256) {
     for (int s = 0; s < 2; ++s) {
       mbar_init(&q_full[s], 1);
       mbar_init(&s_full[s], 1);
@@ -292,8 +312,23 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
     }
     mbar_init(done, 1);
     fence_mbar_init();
+    if (nk[0]) load(&qmap, smem, h, q0 + r0, &q_full[0]);
+    load(&kmap, smem + C::kOffKv, hk, k0, &full[0]);
+    if (nk[1]) load(&qmap, smem + C::kTileBytes, h, q0 + r0 + kPfRows, &q_full[1]);
   }
   if (threadIdx.x < 4 * kPfMasked) poison[threadIdx.x] = 0u;
+  if (threadIdx.x == 0) {
+    ctx[kCtxQ0] = q0;
+    ctx[kCtxLq] = lq;
+    ctx[kCtxR0] = r0;
+    ctx[kCtxH] = h;
+    ctx[kCtxOff] = off;
+    ctx[kCtxLk] = lk;
+    ctx[kCtxJm] = jm;
+    ctx[kCtxK0] = k0;
+    ctx[kCtxNk] = nk[0];
+    ctx[kCtxNk + 1] = nk[1];
+  }
   if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "n"(512)
                  : "memory");
@@ -303,39 +338,29 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  bool failed = false;
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp == 8 && lane == 0) {
-      // loader: ring position 2 j holds K_j, 2 j + 1 holds V_j
-      auto load = [&](const CUtensorMap* map, uint8_t* dst, int head, int row, uint64_t* bar) {
-        mbar_arrive_expect_tx(bar, C::kTileBytes);
-#pragma unroll
-        for (int a = 0; a < C::kAtoms; ++a) tma_load_3d(dst + a * kPfRows * 128, map, a * 64, head, row, bar);
-      };
-      if (nk[0]) load(&qmap, smem, h, q0 + r0, &q_full[0]);
-      int n = 0;
+      // loader: ring position 2 j holds K_j, 2 j + 1 holds V_j; K_0 and the
+      // queries are on their way
+      int n = 1;
       for (; n < 2 * nmax; ++n) {
         const int s = n % C::kSlots;
-        if (n >= C::kSlots && !mbar_wait(&empty[s], ((n / C::kSlots) - 1) & 1)) {
-          failed = true;
-          break;
-        }
+        if (n >= C::kSlots && !mbar_wait(&empty[s], ((n / C::kSlots) - 1) & 1)) break;
         // a partly seen value tile goes to the cleaning warps: it has a
         // barrier of its own, and the slot's passes on to the next phase
         const bool masked = (n & 1) && (n >> 1) >= jm;
         if (masked) mbar_arrive(&full[s]);
         load((n & 1) ? &vmap : &kmap, smem + C::kOffKv + s * C::kTileBytes, hk, k0 + (n >> 1) * kPfRows,
              masked ? &v_full[(n >> 1) - jm] : &full[s]);
-        if (n == 0 && nk[1]) load(&qmap, smem + C::kTileBytes, h, q0 + r0 + kPfRows, &q_full[1]);
       }
       // no copy is left in flight, whatever became of its readers
       for (int i = max(0, n - C::kSlots); i < n; ++i)
         mbar_wait((i & 1) && (i >> 1) >= jm ? &v_full[(i >> 1) - jm] : &full[i % C::kSlots],
                   (i & 1) && (i >> 1) >= jm ? 0 : (i / C::kSlots) & 1);
       if (nk[0]) mbar_wait(&q_full[0], 0);
-      if (nk[1] && n > 0) mbar_wait(&q_full[1], 0);
+      if (nk[1]) mbar_wait(&q_full[1], 0);
     } else if (warp == 9) {
       constexpr uint32_t kFmt = (1u << 4) | (Type16<T>::kFmt << 7) | (Type16<T>::kFmt << 10) |
                                 ((uint32_t)(kPfRows >> 4) << 24);
@@ -427,24 +452,39 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
         if (!__all_sync(0xffffffffu, mbar_wait(&v_full[j - jm], 0))) break;
         uint8_t* tile = smem + C::kOffKv + (n % C::kSlots) * C::kTileBytes;
         const int keys = min(kPfRows, lk - j * kPfRows);
-        for (int c = threadIdx.x - 320; c < C::kTileBytes / 16; c += 64) {   // 16-byte pieces, 8 to a 128-byte row
-          uint4* at = reinterpret_cast<uint4*>(tile) + c;
-          const int key = (c >> 3) % kPfRows;
-          if (key >= keys) {
-            *at = make_uint4(0u, 0u, 0u, 0u);
-            continue;
-          }
-          uint4 w = *at;
-          if (not_finite<T>(w.x) | not_finite<T>(w.y) | not_finite<T>(w.z) | not_finite<T>(w.w)) {
-            atomicOr(&poison[(j - jm) * 4 + (key >> 5)], 1u << (key & 31));
-            uint32_t* x = &w.x;
+        // 16-byte pieces, 8 to a 128-byte row, eight of them at a time: one
+        // by one this took longer than a tile's MMAs and softmax
+        constexpr int kBatch = 8;
+        uint4* at = reinterpret_cast<uint4*>(tile) + (threadIdx.x - 320);
+#pragma unroll 1
+        for (int c0 = 0; c0 < C::kTileBytes / 16; c0 += 64 * kBatch, at += 64 * kBatch) {
+          uint4 w[kBatch];
+          uint32_t bad = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t bad = not_finite<T>(x[i]);
-              if (bad & 0x8000u) x[i] &= 0xffff0000u;
-              if (bad & 0x80000000u) x[i] &= 0x0000ffffu;
+          for (int i = 0; i < kBatch; ++i) w[i] = at[i * 64];
+          auto key_of = [&](int i) { return ((c0 + i * 64 + (int)threadIdx.x - 320) >> 3) % kPfRows; };
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) {
+            const uint32_t b = not_finite<T>(w[i].x) | not_finite<T>(w[i].y) | not_finite<T>(w[i].z) | not_finite<T>(w[i].w);
+            if (key_of(i) < keys) bad |= b;
+            else at[i * 64] = make_uint4(0u, 0u, 0u, 0u);
+          }
+          if (bad) {
+#pragma unroll 1
+            for (int i = 0; i < kBatch; ++i) {
+              const int key = key_of(i);
+              uint4 v = at[i * 64];
+              if (key >= keys || !(not_finite<T>(v.x) | not_finite<T>(v.y) | not_finite<T>(v.z) | not_finite<T>(v.w))) continue;
+              atomicOr(&poison[(j - jm) * 4 + (key >> 5)], 1u << (key & 31));
+              uint32_t* x = &v.x;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const uint32_t b = not_finite<T>(x[k]);
+                if (b & 0x8000u) x[k] &= 0xffff0000u;
+                if (b & 0x80000000u) x[k] &= 0x0000ffffu;
+              }
+              at[i * 64] = v;
             }
-            *at = w;
           }
         }
         fence_proxy_async_smem();
@@ -455,11 +495,12 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int s = warp >> 2, quarter = warp & 3;
-    const int row = r0 + s * kPfRows + quarter * 32 + lane;      // within the sequence
     const uint32_t t_s = tmem + s * kPfRows + ((uint32_t)(quarter * 32) << 16);
     const uint32_t t_o = tmem + C::kTmemO + s * 128 + ((uint32_t)(quarter * 32) << 16);
-    const int n = nk[s], see = min(lk, row + off + 1);           // keys this row sees
-    const int seen_by_all = r0 + s * kPfRows + off + 1;          // keys the tile's first row sees
+    const int n = ctx[kCtxNk + s];
+    // keys this row sees, and the tile's first row
+    const int seen_by_all = ctx[kCtxR0] + s * kPfRows + ctx[kCtxOff] + 1;
+    const int see = min(ctx[kCtxLk], seen_by_all + quarter * 32 + lane);
     float m = -INFINITY, sum = 0.f;                              // reference maximum of the raw scores, sum of terms
     const float scale = p.scale_log2;
     bool fail = false;
@@ -523,7 +564,7 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
           for (int i = 0; i < 32; i += 2) {
             const float2 v = __ffma2_rn(
                 make_float2(__uint_as_float(x[half * 2 + c][i]), __uint_as_float(x[half * 2 + c][i + 1])), scale2, neg2);
-            const float2 e = i % 32 < kPolyOf32 ? ex2_poly(v) : make_float2(ex2(v.x), ex2(v.y));
+            const float2 e = make_float2(ex2(v.x), ex2(v.y));
             part[(i >> 1) & 1] = __fadd2_rn(part[(i >> 1) & 1], e);
             w[c * 16 + (i >> 1)] = pack16<T>(e.x, e.y);
           }
@@ -535,11 +576,22 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
       }
       sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
     }
-    const bool live = row < lq;
-    T* dst = out + ((int64_t)(q0 + row) * p.heads + h) * D;
+    const int e_q0 = ctx[kCtxQ0], e_lq = ctx[kCtxLq], e_h = ctx[kCtxH], e_k0 = ctx[kCtxK0], e_jm = ctx[kCtxJm];
+    const int first = ctx[kCtxR0] + s * kPfRows + quarter * 32, row = first + lane;   // within the sequence
+    const bool live = row < e_lq;
+    const int64_t at = ((int64_t)(blockIdx.x % p.splits) * p.rows + e_q0 + row) * p.heads + e_h;   // splits: partial row
+    T* dst = static_cast<T*>(p.out) + ((int64_t)(e_q0 + row) * p.heads + e_h) * D;
     if (n && !fail && __all_sync(0xffffffffu, mbar_wait(&o_full[s], 0))) {
       tc_fence_after();
-      const float inv = see > 0 ? 1.f / sum : 0.f;
+      // The rows go through shared memory (the tile's queries have been
+      // used), so that a store instruction writes whole rows: one row per lane
+      // is one line per lane, and the stores took 2 us per CTA.
+      constexpr int kPieces = D / 8;
+      uint4* stage = reinterpret_cast<uint4*>(smem + s * C::kTileBytes) + quarter * 32 * kPieces;
+      // a split leaves its sums as they are, to be joined
+      const bool whole = p.splits == 1;
+      const float inv = !whole ? 1.f : see > 0 ? 1.f / sum : 0.f;
+      if (!whole && live) p.part_ml[at] = make_float2(sum == 0.f ? -INFINITY : m * scale, sum);
       uint32_t any = 0;
 #pragma unroll
       for (int i = 0; i < 4 * kPfMasked; ++i) any |= poison[i];
@@ -555,10 +607,10 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
           for (int i = 0; i < 4 * kPfMasked; ++i) {
             uint32_t bits = poison[i];
             while (bits) {
-              const int key = jm * kPfRows + i * 32 + __ffs(bits) - 1;
+              const int key = e_jm * kPfRows + i * 32 + __ffs(bits) - 1;
               bits &= bits - 1;
               if (key >= see) continue;
-              const T* vr = static_cast<const T*>(p.v) + (int64_t)(k0 + key) * p.sv_t + (int64_t)hk * p.sv_h + c * 32;
+              const T* vr = static_cast<const T*>(p.v) + (int64_t)(e_k0 + key) * p.sv_t + (int64_t)(e_h / p.group) * p.sv_h + c * 32;
 #pragma unroll
               for (int d = 0; d < 32; ++d) {
                 const float v = to_f32(vr[d]);
@@ -567,15 +619,31 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
             }
           }
         }
-        if (live) {
+        if (live && !whole) {
+          float* po = p.part_o + at * D + c * 32;
 #pragma unroll
-          for (int i = 0; i < 32; i += 8)
-            *reinterpret_cast<uint4*>(dst + c * 32 + i) =
-                make_uint4(pack16<T>(f[i], f[i + 1]), pack16<T>(f[i + 2], f[i + 3]), pack16<T>(f[i + 4], f[i + 5]),
-                           pack16<T>(f[i + 6], f[i + 7]));
+          for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(po + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+        } else if (whole) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            stage[lane * kPieces + ((c * 4 + i) ^ (lane & 7))] =
+                make_uint4(pack16<T>(f[8 * i], f[8 * i + 1]), pack16<T>(f[8 * i + 2], f[8 * i + 3]),
+                           pack16<T>(f[8 * i + 4], f[8 * i + 5]), pack16<T>(f[8 * i + 6], f[8 * i + 7]));
         }
       }
-    } else if (!n && live) {                                     // this tile's rows see nothing
+      if (whole) {
+        __syncwarp();
+        const int rows = min(32, e_lq - first);
+#pragma unroll 4
+        for (int i = lane; i < rows * kPieces; i += 32) {
+          const int r = i / kPieces, c = i - r * kPieces;
+          *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + ((int64_t)(e_q0 + first + r) * p.heads + e_h) * D + c * 8) =
+              stage[r * kPieces + (c ^ (r & 7))];
+        }
+      }
+    } else if (!n && live && p.splits > 1) {                     // this tile's rows see nothing here
+      p.part_ml[at] = make_float2(-INFINITY, 0.f);
+    } else if (!n && live) {
 #pragma unroll 1
       for (int d = 0; d < D; d += 8) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0u, 0u, 0u, 0u);
     }
@@ -586,11 +654,50 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
   if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512));
 }
 
+// Joins the splits' partial results: one thread per four columns.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) attn_prefill_join_kernel(const __grid_constant__ PrefillParams p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int64_t n = (int64_t)p.rows * p.heads, e = (int64_t)blockIdx.x * 256 + threadIdx.x, at = e / (D / 4);
+  if (at >= n) return;
+  const int d = (int)(e - at * (D / 4)) * 4;
+  float2 ml[kPfSplits];
+  float mx = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kPfSplits; ++i) {
+    ml[i] = i < p.splits ? p.part_ml[i * n + at] : make_float2(-INFINITY, 0.f);
+    mx = fmaxf(mx, ml[i].x);
+  }
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kPfSplits; ++i) {
+    if (ml[i].y == 0.f) continue;                          // this split saw nothing (its values are not set)
+    const float4 v = *reinterpret_cast<const float4*>(p.part_o + (i * n + at) * D + d);
+    const float f = exp2f(ml[i].x - mx);
+    acc.x = fmaf(v.x, f, acc.x);
+    acc.y = fmaf(v.y, f, acc.y);
+    acc.z = fmaf(v.z, f, acc.z);
+    acc.w = fmaf(v.w, f, acc.w);
+    sum = fmaf(ml[i].y, f, sum);
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const T o[4] = {from_f32<T>(acc.x * inv), from_f32<T>(acc.y * inv), from_f32<T>(acc.z * inv), from_f32<T>(acc.w * inv)};
+  *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at * D + d) = *reinterpret_cast<const uint2*>(o);
+}
+
 // ---------------------------------------------------------------------------
 // launch
 // ---------------------------------------------------------------------------
 // [tokens][heads][dim] with the given element strides; boxes of 128 tokens
 // by 64 columns of one head.
+static int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return 148;
+  return n;
+}
+
 static bool encode_rows(CUtensorMap* map, const void* base, int dtype, int64_t rows, int heads, int dim, int64_t st_t,
                         int64_t st_h) {
   auto encode = get_encode();
@@ -610,15 +717,45 @@ static bool encode_rows(CUtensorMap* map, const void* base, int dtype, int64_t r
 template <typename T, int D>
 static cudaError_t launch_prefill(const CUtensorMap* maps, const PrefillParams& p, int64_t slots, cudaStream_t st) {
   using C = PrefillTile<D>;
-  const cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(attn_prefill_kernel<T, D>), C::kSmem);
+  cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(attn_prefill_kernel<T, D>), C::kSmem);
   if (e != cudaSuccess) return e;
-  attn_prefill_kernel<T, D><<<(unsigned)(slots * p.heads), kPfThreads, C::kSmem, st>>>(maps[0], maps[1], maps[2], p);
-  return cudaGetLastError();
+  attn_prefill_kernel<T, D><<<(unsigned)(slots * p.heads * p.splits), kPfThreads, C::kSmem, st>>>(maps[0], maps[1],
+                                                                                                  maps[2], p);
+  if ((e = cudaGetLastError()) != cudaSuccess || p.splits == 1) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(((int64_t)p.rows * p.heads * (D / 4) + 255) / 256));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, attn_prefill_join_kernel<T, D>, p);
+}
+
+// Into how many CTAs an item's keys are split.  An item (256 rows of one
+// head) takes as long as its keys whatever the number of rows, so where the
+// items do not fill the SMs and the sequences are long, sharing the keys out
+// shortens the call; the number of items is estimated as one per 256 rows and
+// half a one more per sequence.  Two calls at 16 heads of 64: 901 queries
+// behind 6596 keys 66 us unsplit, 39 us in two.
+static int prefill_splits(int B, int64_t rows, int64_t k_rows, int heads) {
+  const int64_t items = (rows / (2 * kPfRows) + (B + 1) / 2) * heads;
+  const int64_t by_sms = items > 0 ? (sm_count() + sm_count() / 4) / items : 1;
+  const int64_t by_keys = B > 0 ? k_rows / B / (4 * kPfRows) : 1;      // at least four key tiles each
+  const int64_t n = by_sms < by_keys ? by_sms : by_keys;
+  return n < 1 ? 1 : n > kPfSplits ? kPfSplits : (int)n;
+}
+
+size_t attn_prefill_workspace(int B, int64_t rows, int64_t k_rows, int heads, int dim) {
+  const int n = prefill_splits(B, rows, k_rows, heads);
+  return n == 1 ? 0 : (size_t)n * rows * heads * (dim * 4 + 8);
 }
 
 cudaError_t launch_attn_prefill(const void* q, const void* k, const void* v, int dtype, const int64_t* s,
                                 const int32_t* cu_q, const int32_t* cu_k, int B, int64_t rows, int64_t k_rows,
-                                int heads, int kv_heads, int dim, float scale, void* out, cudaStream_t st) {
+                                int heads, int kv_heads, int dim, float scale, void* out, void* workspace, cudaStream_t st) {
   if (k_rows == 0) return cudaMemsetAsync(out, 0, (size_t)rows * heads * dim * 2, st);
   CUtensorMap maps[3];
   if (!encode_rows(&maps[0], q, dtype, rows, heads, dim, s[0], s[1]) ||
@@ -627,11 +764,14 @@ cudaError_t launch_attn_prefill(const void* q, const void* k, const void* v, int
     return cudaErrorInvalidValue;
   // a scale of zero still has to leave -infinity where a key is not seen
   const float scale_log2 = fmaxf(scale * 1.4426950408889634f, 1e-37f);
-  const PrefillParams p{cu_q, cu_k, B, heads, heads / kv_heads, (int)rows, (int)k_rows, scale_log2, out, v, s[4], s[5]};
-  // at most one tile more than whole ones per sequence (and for the rows behind the last)
+  const int splits = workspace ? prefill_splits(B, rows, k_rows, heads) : 1;
+  float* po = static_cast<float*>(workspace);
+  const PrefillParams p{cu_q, cu_k, B, heads, heads / kv_heads, (int)rows, (int)k_rows, scale_log2, out, v, s[4], s[5],
+                        splits, po, reinterpret_cast<float2*>(po + (size_t)splits * rows * heads * dim)};
+  // at most one item more than whole ones per sequence (and for the rows behind the last)
   int64_t slots = rows / (2 * kPfRows) + B + 1;
   if (slots > rows) slots = rows;
-  if (slots * heads > 0x7FFFFFFF) return cudaErrorInvalidValue;
+  if (slots * heads * splits > 0x7FFFFFFF || rows * heads * (dim / 4) / 256 >= 0x7FFFFFFF) return cudaErrorInvalidValue;
   if (dtype == PARO_BF16)
     return dim == 128 ? launch_prefill<__nv_bfloat16, 128>(maps, p, slots, st)
                       : launch_prefill<__nv_bfloat16, 64>(maps, p, slots, st);

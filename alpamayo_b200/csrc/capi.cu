@@ -66,7 +66,9 @@ cudaError_t launch_gemm_tc_sets(const int8_t* xq, const float* xscale, int64_t M
 int gemm_tc_sets_ok(int T, const int* tab_nb);
 cudaError_t launch_attn_prefill(const void* q, const void* k, const void* v, int dtype, const int64_t* strides,
                                 const int32_t* cu_q, const int32_t* cu_k, int B, int64_t rows, int64_t k_rows,
-                                int heads, int kv_heads, int dim, float scale, void* out, cudaStream_t st);
+                                int heads, int kv_heads, int dim, float scale, void* out, void* workspace,
+                                cudaStream_t st);
+size_t attn_prefill_workspace(int B, int64_t rows, int64_t k_rows, int heads, int dim);
 cudaError_t launch_kv8_append(const Kv8View& c, const void* k, const void* v, int dtype, const int64_t* strides,
                               const int32_t* cu, const int32_t* starts, int B, int64_t rows, cudaStream_t st);
 cudaError_t launch_kv8_gather(const Kv8View& c, const int32_t* starts, const int32_t* cu, int B, int64_t rows, void* k,
@@ -831,9 +833,15 @@ size_t paro_attention_kv8_workspace_size(const paro_kv8_cache* cache, int table_
   return kv8_attn_workspace(c, B, T, heads, with_weights);
 }
 
-int paro_attention_prefill(const void* q, const void* k, const void* v, int dtype, const int64_t* strides,
-                           const int32_t* cu_q, const int32_t* cu_k, int B, int64_t rows, int64_t k_rows, int heads,
-                           int kv_heads, int head_dim, float scale, void* out, paro_stream_t stream) {
+size_t paro_attention_prefill_workspace_size(int B, int64_t rows, int64_t k_rows, int heads, int head_dim) {
+  if (B <= 0 || rows <= 0 || k_rows <= 0 || heads <= 0 || (head_dim != 64 && head_dim != 128)) return 0;
+  return attn_prefill_workspace(B, rows, k_rows, heads, head_dim);
+}
+
+int paro_attention_prefill_ws(const void* q, const void* k, const void* v, int dtype, const int64_t* strides,
+                              const int32_t* cu_q, const int32_t* cu_k, int B, int64_t rows, int64_t k_rows, int heads,
+                              int kv_heads, int head_dim, float scale, void* out, void* workspace,
+                              size_t workspace_bytes, paro_stream_t stream) {
   if (rows < 0 || k_rows < 0 || B < 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return PARO_ERR_INVALID_ARGUMENT;
   if (dtype != PARO_BF16 && dtype != PARO_F16) return PARO_ERR_UNSUPPORTED;
   if (heads % kv_heads || (head_dim != 64 && head_dim != 128)) return PARO_ERR_SHAPE;
@@ -842,13 +850,22 @@ int paro_attention_prefill(const void* q, const void* k, const void* v, int dtyp
   if (rows == 0) return PARO_OK;
   if (!q || !out || !strides || !cu_q || !cu_k || (k_rows > 0 && (!k || !v))) return PARO_ERR_INVALID_ARGUMENT;
   if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16) || !aligned(cu_q, 4) ||
-      !aligned(cu_k, 4))
+      !aligned(cu_k, 4) || !aligned(workspace, 256))
     return PARO_ERR_MISALIGNED;
   for (int i = 0; i < 6; ++i)
     if (strides[i] < 0 || strides[i] % 8) return PARO_ERR_MISALIGNED;
+  const size_t need = paro_attention_prefill_workspace_size(B, rows, k_rows, heads, head_dim);
+  if (workspace && workspace_bytes < need) return PARO_ERR_WORKSPACE;
   if (int d = device_check()) return d;
   return cuda_status(launch_attn_prefill(q, k, v, dtype, strides, cu_q, cu_k, B, rows, k_rows, heads, kv_heads,
-                                         head_dim, scale, out, (cudaStream_t)stream));
+                                         head_dim, scale, out, need ? workspace : nullptr, (cudaStream_t)stream));
+}
+
+int paro_attention_prefill(const void* q, const void* k, const void* v, int dtype, const int64_t* strides,
+                           const int32_t* cu_q, const int32_t* cu_k, int B, int64_t rows, int64_t k_rows, int heads,
+                           int kv_heads, int head_dim, float scale, void* out, paro_stream_t stream) {
+  return paro_attention_prefill_ws(q, k, v, dtype, strides, cu_q, cu_k, B, rows, k_rows, heads, kv_heads, head_dim,
+                                   scale, out, nullptr, 0, stream);
 }
 
 int paro_kv8_append(const paro_kv8_cache* cache, const int32_t* page_table, int table_width, const void* k,

@@ -104,10 +104,14 @@ at::Tensor attention_prefill(const at::Tensor& q, const at::Tensor& k, const at:
   at::Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
   const int64_t strides[6] = {stride_of(q, 0), stride_of(q, 1), stride_of(k, 0), stride_of(k, 1), stride_of(v, 0),
                               stride_of(v, 1)};
-  check_status(paro_attention_prefill(q.data_ptr(), k.data_ptr(), v.data_ptr(), dt, strides, cu.data_ptr<int32_t>(),
-                                      cu_k.data_ptr<int32_t>(), (int)cu.size(0) - 1, q.size(0), k.size(0),
-                                      (int)q.size(1), (int)k.size(1), (int)q.size(2), (float)scale, out.data_ptr(),
-                                      cur_stream()),
+  const int B = (int)cu.size(0) - 1;
+  const size_t wsb = paro_attention_prefill_workspace_size(B, q.size(0), k.size(0), (int)q.size(1), (int)q.size(2));
+  at::Tensor ws;   // allocations start on 512-byte boundaries
+  if (wsb) ws = at::empty({(int64_t)wsb}, q.options().dtype(at::kByte));
+  check_status(paro_attention_prefill_ws(q.data_ptr(), k.data_ptr(), v.data_ptr(), dt, strides, cu.data_ptr<int32_t>(),
+                                         cu_k.data_ptr<int32_t>(), B, q.size(0), k.size(0), (int)q.size(1),
+                                         (int)k.size(1), (int)q.size(2), (float)scale, out.data_ptr(),
+                                         wsb ? ws.data_ptr() : nullptr, wsb, cur_stream()),
                "attention_prefill");
   return out;
 }

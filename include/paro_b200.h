@@ -536,6 +536,17 @@ int paro_attention_prefill(const void* q, const void* k, const void* v, int dtyp
                            paro_stream_t stream);
 
 /*
+ * The same with a workspace (256-byte aligned, of any content) in which few
+ * queries over long sequences may be shared out over the keys; a size of 0
+ * says that the call would not use one.
+ */
+size_t paro_attention_prefill_workspace_size(int B, int64_t rows, int64_t k_rows, int heads, int head_dim);
+int paro_attention_prefill_ws(const void* q, const void* k, const void* v, int dtype, const int64_t* strides,
+                              const int32_t* cu_q, const int32_t* cu_k, int B, int64_t rows, int64_t k_rows,
+                              int heads, int kv_heads, int head_dim, float scale, void* out, void* workspace,
+                              size_t workspace_bytes, paro_stream_t stream);
+
+/*
  * Writes new tokens' keys and values into the cache: sequence b's rows
  * cu[b] .. cu[b + 1] - 1 become its tokens starts[b], starts[b] + 1, ...
  * Per page and head: scale = max|x| / 127 over the page's tokens, code = the

@@ -64,6 +64,47 @@ def test_prefill_behind_history(q_lens, k_lens, dim, dtype):
         a += n
 
 
+@pytest.mark.parametrize("dtype,dim", [(BF16, 128), (F16, 64)])
+@pytest.mark.parametrize("q_lens,k_lens", [([5, 100], [3000, 1111]), ([1], [5000]), ([300], [2500]), ([3, 0, 700, 2], [9, 0, 700, 6000])])
+def test_prefill_keys_shared_out(q_lens, k_lens, dim, dtype):
+    # few rows over long sequences: several blocks share a row's keys
+    import alpamayo_b200.ops as ops
+    from alpamayo_b200 import _native
+    assert _native.capi().paro_attention_prefill_workspace_size(len(q_lens), sum(q_lens), sum(k_lens), 2, dim) > 0
+    q, k, v = packed(q_lens, k_lens, 2, 1, dim, dtype, 40)
+    out = ops.attention_prefill(q.cuda(), k.cuda(), v.cuda(), R.cu(q_lens), R.cu(k_lens))
+    a = b = 0
+    for n, m in zip(q_lens, k_lens):
+        for i in sorted({0, n // 3, n // 2, n - 1} - {-1}) if n else []:
+            see = i + 1 + m - n
+            ref, _, size, sb = R.attend(q[a + i:a + i + 1].double(), k[b:b + see].double(), v[b:b + see].double(), dim ** -0.5)
+            bound = R.out_bound(ref, size, sb, dtype, R.UNIT[dtype]) + (2.0 ** -25 if dtype == F16 else 0.0)
+            assert R.max_excess(out[a + i:a + i + 1], ref, bound) <= 1.0, (n, m, i)
+        a, b = a + n, b + m
+    # a value that is not finite, seen by some of the last sequence's rows only
+    n, m = q_lens[-1], k_lens[-1]
+    v2 = v.clone()
+    v2[-1, 0, 5] = float("inf")
+    got = ops.attention_prefill(q.cuda(), k.cuda(), v2.cuda(), R.cu(q_lens), R.cu(k_lens))
+    assert torch.equal(got[:-1], out[:-1]) and not torch.isfinite(got[-1, :, 5]).any()
+    rest = torch.arange(dim) != 5
+    assert torch.equal(got[-1][:, rest], out[-1][:, rest])
+
+
+def test_prefill_many_sequences_in_order_of_place():
+    # over 32 sequences, of all numbers of tiles
+    import alpamayo_b200.ops as ops
+    lens = [(i * 37) % 520 if i % 5 else 0 for i in range(70)]
+    q, k, v = packed(lens, lens, 2, 2, 64, BF16, 41)
+    out = ops.attention_prefill(q.cuda(), k.cuda(), v.cuda(), R.cu(lens))
+    a = 0
+    for n in lens:
+        for i in sorted({0, n // 2, n - 1} - {-1}) if n else []:
+            ref, _, size, sb = R.attend(q[a + i:a + i + 1].double(), k[a:a + i + 1].double(), v[a:a + i + 1].double(), 0.125)
+            assert R.max_excess(out[a + i:a + i + 1], ref, R.out_bound(ref, size, sb, BF16, R.UNIT[BF16])) <= 1.0, (n, i)
+        a += n
+
+
 def test_prefill_long_rows_and_large_scores():
     import alpamayo_b200.ops as ops
     lens = [1500]
