@@ -691,13 +691,6 @@ __global__ void __launch_bounds__(256) attn_prefill_join_kernel(const __grid_con
 // ---------------------------------------------------------------------------
 // [tokens][heads][dim] with the given element strides; boxes of 128 tokens
 // by 64 columns of one head.
-static int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return 148;
-  return n;
-}
-
 static bool encode_rows(CUtensorMap* map, const void* base, int dtype, int64_t rows, int heads, int dim, int64_t st_t,
                         int64_t st_h) {
   auto encode = get_encode();

@@ -6,6 +6,7 @@
 // then launches asynchronously on the caller's stream.  Nothing here
 // allocates device memory or synchronises.
 #include <algorithm>
+#include <atomic>
 #include <cstring>
 #include <string>
 
@@ -94,6 +95,16 @@ uint32_t error_word_rows(int clear);
 uint32_t error_word_kv8(int clear);
 uint32_t error_word_kv8a(int clear);
 uint32_t error_word_attn(int clear);
+
+int sm_count() {
+  static std::atomic<int> known[64];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if ((n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+  known[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
 
 cudaError_t ensure_smem_limit(const void* kernel, int bytes) {
   static std::mutex mu;

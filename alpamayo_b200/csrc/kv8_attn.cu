@@ -57,7 +57,9 @@ struct DecodeParams {
   float* part_o;               // [row blocks][slots][RB][dim]
   float2* part_ml;             // [row blocks][slots][RB] (M, sum)
   int slots;                   // B * kv_heads + ctas
-  int lanes, out_blocks;       // second kernel: threads per output column group, blocks of output rows
+  int lanes, out_blocks;       // second kernel: threads per output column group, blocks of output rows,
+  int row_groups;              // threads that share a weight's rows
+  int2* range;                 // [B * kv_heads] first and last CTA with a partial
   float* scores;               // [B * kv_heads][rows][score_cap] log2-scaled scores, or null
   int64_t score_cap;
   const float* weights;        // [B][kv_heads][cap] or null
@@ -158,8 +160,8 @@ struct DecodeTile {
   static constexpr int kWarpRows = RB / kWr;             // 8 or 16
   static constexpr int kSlots = D / 8;                   // 16-byte slots per lane and stage (K and V)
   static constexpr int kStage = kSlots * 512 + 32;       // + the unit's four scales
-  static constexpr int kCtas = RB == 8 ? 3 : 2;          // CTAs per SM
-  static constexpr int kStages = RB == 8 ? (D == 128 ? 2 : 4) : kWr == 1 ? (D == 128 ? 3 : 4) : 4;
+  static constexpr int kCtas = 3;                        // CTAs per SM
+  static constexpr int kStages = kWr == 4 ? 4 : kWr == 2 ? 3 : D == 128 ? 2 : 4;
   static constexpr int kRing = kTeams * kStages * kStage;
   static constexpr int kComb = kTeams > 1 ? RB * D * 4 + RB * 32 : 0;   // one team's partial on its way to the next
   static constexpr int kSmem = kRing + kComb;
@@ -312,6 +314,11 @@ __global__ void __launch_bounds__(kDecWarps * 32, (DecodeTile<D, RB>::kCtas)) kv
 
   while (seg0 < u1) {
     const int seg1 = min(u1, seg_first + su);
+    if (threadIdx.x == 0 && blockIdx.y == 0) {
+      int* at = reinterpret_cast<int*>(p.range + b * c.kv_heads + h);
+      if (seg0 == seg_first) at[0] = blockIdx.x;
+      if (seg1 == seg_first + su) at[1] = blockIdx.x;
+    }
     const int len = kv8_len(c, p.lens[b]);
     // query fragments and row state
 #pragma unroll
@@ -587,7 +594,8 @@ __global__ void __launch_bounds__(kDecWarps * 32, (DecodeTile<D, RB>::kCtas)) kv
 // partial of the same group (a long sequence has one partial per CTA of the
 // first kernel, and reading them one after the other would cost more than
 // the attention).  A weight block turns the scores of kJoinTokens tokens
-// into weights.
+// into weights (where there are many rows, of fewer tokens, with several
+// threads to share a token's rows).
 constexpr int kJoinTokens = 1024;
 constexpr int kJoinThreads = 256;
 constexpr int kJoinRows = 8;                  // rows of scores in flight per thread
@@ -609,20 +617,15 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const __grid_con
   __shared__ float4 s_part[kJoinThreads];
   constexpr int kCols = D / 4;                // column groups of a row
   const Kv8View& c = p.c;
-  const int lane = threadIdx.x & 31;
   const int bh = blockIdx.x, b = bh / c.kv_heads, h = bh - b * c.kv_heads;
   const int chunk = (int)blockIdx.y - p.out_blocks;
   const int len = kv8_len(c, p.lens[b]);
-  if (chunk >= 0 && (int64_t)chunk * kJoinTokens >= len) return;
-  // the CTAs of the first kernel that hold partials of (b, h): c0 .. c1
-  int total;
-  const int per = units_per_cta(p, &total);
-  int before = 0;
-  for (int i = lane; i < b; i += 32) before += seq_units(p, i);
-  before = __reduce_add_sync(0xffffffffu, before);
-  const int su = seq_units(p, b), ub = before * c.kv_heads + h * su;
-  const int c0 = ub / per, c1 = su ? (ub + su - 1) / per : c0 - 1;
+  const int tokens = kJoinTokens / p.row_groups;   // a weight block's
+  if (chunk >= 0 && (int64_t)chunk * tokens >= len) return;
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  // the CTAs of the first kernel that hold partials of (b, h): c0 .. c1
+  const int2 range = len > 0 ? p.range[bh] : make_int2(0, -1);
+  const int c0 = range.x, c1 = range.y;
 
   if (chunk < 0) {
     const int groups = kJoinThreads / p.lanes;
@@ -683,23 +686,26 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const __grid_con
     }
     return;
   }
-  // Four tokens per thread.  The first rows' scores and the old weights are
-  // on their way while the statistics are joined; a masked or padded score is
-  // loaded (inside its row) but never used.
-  const int tok = chunk * kJoinTokens + threadIdx.x * 4;
+  // Four tokens per thread, and every row_groups-th row.  The first rows'
+  // scores and the old weights are on their way while the statistics are
+  // joined; a masked or padded score is loaded (inside its row) but never
+  // used.
+  const int quads = tokens / 4, rg = threadIdx.x / quads, tok = chunk * tokens + threadIdx.x % quads * 4;
   const bool live = tok < len;
   const float* s = p.scores + (int64_t)bh * p.rows * p.score_cap + tok;
   const int64_t wat = (int64_t)bh * p.cap + tok;
   float4 v[kJoinRows];
   auto fetch = [&](int r0) {
 #pragma unroll
-    for (int r = 0; r < kJoinRows; ++r)
-      if (live && r0 + r < p.rows) v[r] = *reinterpret_cast<const float4*>(s + (int64_t)(r0 + r) * p.score_cap);
+    for (int i = 0; i < kJoinRows; ++i) {
+      const int r = r0 + i * p.row_groups + rg;
+      if (live && r < p.rows) v[i] = *reinterpret_cast<const float4*>(s + (int64_t)r * p.score_cap);
+    }
   };
   fetch(0);
   float w[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) w[e] = tok + e < len ? p.weights[wat + e] : 0.f;
+  for (int e = 0; e < 4; ++e) w[e] = rg == 0 && tok + e < len ? p.weights[wat + e] : 0.f;
   // `per_row` lanes join a row's statistics
   int per_row = 32;
   while (per_row > 1 && kJoinThreads / per_row < p.rows) per_row >>= 1;
@@ -721,21 +727,34 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const __grid_con
     if (r < p.rows && threadIdx.x % per_row == 0) s_ml[r] = make_float2(m, l == 0.f ? 0.f : 1.f / l);
   }
   __syncthreads();
-  if (!live) return;
   float mass[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int r0 = 0; r0 < p.rows; r0 += kJoinRows) {
+  for (int r0 = 0; r0 < p.rows; r0 += kJoinRows * p.row_groups) {
     if (r0) fetch(r0);
 #pragma unroll
-    for (int r = 0; r < kJoinRows; ++r) {
-      if (r0 + r >= p.rows) break;
-      const float2 row = s_ml[r0 + r];
-      const int see = row.y == 0.f ? 0 : len - p.T + (r0 + r) / p.group + 1;
-      const float x[4] = {v[r].x, v[r].y, v[r].z, v[r].w};
+    for (int i = 0; i < kJoinRows; ++i) {
+      const int r = r0 + i * p.row_groups + rg;
+      if (r >= p.rows) break;
+      const float2 row = s_ml[r];
+      const int see = row.y == 0.f ? 0 : len - p.T + r / p.group + 1;
+      const float x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (tok + e < see) mass[e] = fmaf(ex2(x[e] - row.x), row.y, mass[e]);
     }
   }
+  if (p.row_groups > 1) {
+    s_part[threadIdx.x] = make_float4(mass[0], mass[1], mass[2], mass[3]);
+    __syncthreads();
+    if (rg == 0)
+      for (int i = 1; i < p.row_groups; ++i) {
+        const float4 o = s_part[threadIdx.x + i * quads];
+        mass[0] += o.x;
+        mass[1] += o.y;
+        mass[2] += o.z;
+        mass[3] += o.w;
+      }
+  }
+  if (rg) return;
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     if (tok + e < len) p.weights_out[wat + e] = w[e] + mass[e];
@@ -747,19 +766,12 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const __grid_con
 // Rows per CTA; beyond 64 the cache is read once for each 64.
 static int row_block(int rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
 
-static int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return 148;
-  return n;
-}
-
 // Workspace: partials, their (M, sum), and the scores where weights are kept.
 static void decode_plan(DecodeParams& p, size_t* bytes) {
   const int rb = row_block(p.rows), blocks = (p.rows + rb - 1) / rb;
   const int64_t cap_units = (((int64_t)p.c.table_width << p.c.page_shift) + kUnit - 1) / kUnit;
   const int64_t most = (cap_units * p.B * p.c.kv_heads + kMinUnits - 1) / kMinUnits;
-  int64_t ctas = (int64_t)sm_count() * (rb == 8 ? 3 : 2);   // DecodeTile's kCtas
+  int64_t ctas = (int64_t)sm_count() * 3;                    // DecodeTile's kCtas
   ctas = (ctas + blocks - 1) / blocks;
   p.ctas = (int)(most < ctas ? most : ctas);
   if (p.ctas < 1) p.ctas = 1;
@@ -772,6 +784,7 @@ static void decode_plan(DecodeParams& p, size_t* bytes) {
   while (p.lanes < 32 && p.lanes * p.B * p.c.kv_heads * 2 <= p.ctas &&
          (int64_t)p.lanes * 2 * p.B * p.c.kv_heads * p.rows * (p.c.dim / 4) <= (int64_t)kJoinThreads * 4 * sm_count())
     p.lanes *= 2;
+  p.row_groups = p.rows <= 8 ? 1 : p.rows <= 16 ? 2 : 4;
   const int groups = kJoinThreads / p.lanes;
   p.out_blocks = (p.rows * (p.c.dim / 4) + groups - 1) / groups;
   const size_t part_rows = (size_t)blocks * p.slots * rb;
@@ -780,6 +793,8 @@ static void decode_plan(DecodeParams& p, size_t* bytes) {
   size_t off = al(part_rows * p.c.dim * 4);
   p.part_ml = reinterpret_cast<float2*>(w + off);
   off += al(part_rows * 8);
+  p.range = reinterpret_cast<int2*>(w + off);
+  off += al((size_t)p.B * p.c.kv_heads * 8);
   p.scores = p.weights ? reinterpret_cast<float*>(w + off) : nullptr;
   if (p.weights) off += (size_t)p.B * p.c.kv_heads * p.rows * p.score_cap * 4;
   *bytes = off;
@@ -811,7 +826,7 @@ static cudaError_t launch_decode(const DecodeParams& p, cudaStream_t st) {
   kv8_attn_kernel<T, D, RB><<<dim3((unsigned)p.ctas, (unsigned)blocks), kDecWarps * 32, C::kSmem, st>>>(p);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   const int64_t cap = (int64_t)p.c.table_width << p.c.page_shift;
-  const int64_t chunks = p.weights ? (cap + kJoinTokens - 1) / kJoinTokens : 0;
+  const int64_t chunks = p.weights ? (cap * p.row_groups + kJoinTokens - 1) / kJoinTokens : 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(p.B * p.c.kv_heads), (unsigned)(p.out_blocks + chunks));
   cfg.blockDim = dim3(kJoinThreads);

@@ -665,13 +665,6 @@ __global__ void __launch_bounds__(kCmpThreads) kv8_compact_kernel(EvictParams p,
 // Threads that hold a (page, head) tile, kVpt vectors of 8 elements each.
 static int tile_threads(const Kv8View& c) { return (c.dim << c.page_shift) / (8 * kVpt); }
 
-static int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return 148;
-  return n;
-}
-
 cudaError_t launch_kv8_append(const Kv8View& c, const void* k, const void* v, int dtype, const int64_t* strides,
                               const int32_t* cu, const int32_t* starts, int B, int64_t rows, cudaStream_t st) {
   AppendParams p{c, {k, v}, {strides[0], strides[2]}, {strides[1], strides[3]}, cu, starts, B, rows};

@@ -174,6 +174,9 @@ struct RotTables {
 // device); later calls are a map lookup instead of a driver call.
 cudaError_t ensure_smem_limit(const void* kernel, int bytes);
 
+// SMs of the current device, asked for once per device.
+int sm_count();
+
 // ---------------------------------------------------------------------------
 // small PTX wrappers
 // ---------------------------------------------------------------------------
