@@ -614,6 +614,7 @@ __device__ __forceinline__ void join_stats(float& m, float& l, float m2, float l
 template <typename T, int D, int RB>
 __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const __grid_constant__ DecodeParams p) {
   __shared__ float2 s_ml[kMaxRows];           // weights: (M - kPShift, 1 / sum) per row; 0: the row sees nothing
+  __shared__ int s_see[kMaxRows];             // tokens the row sees
   __shared__ float4 s_part[kJoinThreads];
   constexpr int kCols = D / 4;                // column groups of a row
   const Kv8View& c = p.c;
@@ -696,19 +697,20 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const __grid_con
   const int64_t wat = (int64_t)bh * p.cap + tok;
   float4 v[kJoinRows];
   auto fetch = [&](int r0) {
+    const float* at = s + (int64_t)(r0 + rg) * p.score_cap;
+    const int64_t step = (int64_t)p.row_groups * p.score_cap;
 #pragma unroll
-    for (int i = 0; i < kJoinRows; ++i) {
-      const int r = r0 + i * p.row_groups + rg;
-      if (live && r < p.rows) v[i] = *reinterpret_cast<const float4*>(s + (int64_t)r * p.score_cap);
-    }
+    for (int i = 0; i < kJoinRows; ++i, at += step)
+      if (live && r0 + i * p.row_groups + rg < p.rows) v[i] = *reinterpret_cast<const float4*>(at);
   };
   fetch(0);
   float w[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) w[e] = rg == 0 && tok + e < len ? p.weights[wat + e] : 0.f;
-  // `per_row` lanes join a row's statistics
-  int per_row = 32;
-  while (per_row > 1 && kJoinThreads / per_row < p.rows) per_row >>= 1;
+  // `per_row` lanes join a row's statistics: no more than there are partials,
+  // nor than let the block take all rows at once
+  int per_row = 1;
+  while (per_row < 32 && per_row < c1 - c0 + 1 && kJoinThreads / (2 * per_row) >= p.rows) per_row <<= 1;
   for (int r0 = 0; r0 < p.rows; r0 += kJoinThreads / per_row) {
     const int r = r0 + threadIdx.x / per_row;
     float m = -INFINITY, l = 0.f, f, f2;
@@ -724,7 +726,10 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const __grid_con
       const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o);
       join_stats(m, l, m2, l2, f, f2);
     }
-    if (r < p.rows && threadIdx.x % per_row == 0) s_ml[r] = make_float2(m, l == 0.f ? 0.f : 1.f / l);
+    if (r < p.rows && threadIdx.x % per_row == 0) {
+      s_ml[r] = make_float2(m, l == 0.f ? 0.f : 1.f / l);
+      s_see[r] = l == 0.f ? 0 : len - p.T + r / p.group + 1;
+    }
   }
   __syncthreads();
   float mass[4] = {0.f, 0.f, 0.f, 0.f};
@@ -735,7 +740,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const __grid_con
       const int r = r0 + i * p.row_groups + rg;
       if (r >= p.rows) break;
       const float2 row = s_ml[r];
-      const int see = row.y == 0.f ? 0 : len - p.T + r / p.group + 1;
+      const int see = s_see[r];
       const float x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
       for (int e = 0; e < 4; ++e)
