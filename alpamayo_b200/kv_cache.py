@@ -1,0 +1,216 @@
+"""The int8 paged key/value cache as a program holds it, and the attention of
+a decoder stack over it.
+
+* KV8Cache — one layer's pool of pages: int8 codes with one float32 scale per
+  (page, KV head) for keys and for values, and the operators on it.
+* ClipCache — the caches of all layers for a batch of clips: which pages each
+  clip has, how many tokens it holds, and the attention between a layer's qkv
+  and o projections for prompts (whole or in chunks), decode steps,
+  speculative verification and, where attention totals are kept, eviction.
+
+The reference keeps bf16 keys and values in a StaticCache and calls
+scaled_dot_product_attention on it (src/alpamayo_r1/utils/system/patches.py:
+381-548); rotary embedding and the query/key norms happen before, in the
+caller's `position` function here.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import ops
+
+PAGE_SIZES, HEAD_DIMS = (16, 32, 64, 128), (64, 128)
+
+
+class KV8Cache:
+    """One layer's pages.  A page holds `page_size` tokens of one sequence for
+    every KV head; an element stands for code * scale."""
+
+    def __init__(self, pages, kv_heads, head_dim, page_size=64, device="cuda"):
+        if page_size not in PAGE_SIZES or head_dim not in HEAD_DIMS:
+            raise ValueError(f"page_size must be one of {PAGE_SIZES} and head_dim one of {HEAD_DIMS}")
+        shape = (pages, kv_heads, page_size, head_dim)
+        self.page_size = page_size
+        self.k_codes = torch.zeros(shape, dtype=torch.int8, device=device)
+        self.v_codes = torch.zeros(shape, dtype=torch.int8, device=device)
+        self.k_scale = torch.zeros(shape[:2], device=device)
+        self.v_scale = torch.zeros(shape[:2], device=device)
+
+    @property
+    def tensors(self):
+        """(k_codes, v_codes, k_scale, v_scale), as the operators take them."""
+        return self.k_codes, self.v_codes, self.k_scale, self.v_scale
+
+    def append(self, k, v, cu_seqlens, starts, page_table):
+        """Write new tokens behind starts[b] tokens (ops.kv8_append)."""
+        ops.kv8_append(k, v, cu_seqlens, starts, *self.tensors, page_table)
+
+    def gather(self, page_table, starts, cu_seqlens, rows, dtype=torch.bfloat16):
+        """Token ranges back as (k, v) [rows, kv_heads, head_dim] (ops.kv8_gather)."""
+        return ops.kv8_gather(*self.tensors, page_table, starts, cu_seqlens, rows, dtype)
+
+    def attend(self, q, page_table, seq_lens, scale=None, weights=None, weights_out=None):
+        """Attention of the newest tokens q [B, T, heads, head_dim] (ops.attention_kv8)."""
+        return ops.attention_kv8(q, *self.tensors, page_table, seq_lens, scale, weights, weights_out)
+
+    def evict(self, weights, page_table, seq_lens, out_table, budget, sink=4, recent=0):
+        """Keep `budget` tokens per sequence and KV head, in other pages (ops.kv8_evict)."""
+        return ops.kv8_evict(weights, *self.tensors, page_table, seq_lens, out_table, budget, sink, recent)
+
+
+def _offsets(lens, device):
+    cu = [0]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    return torch.tensor(cu, dtype=torch.int32, device=device)
+
+
+class ClipCache:
+    """Key/value caches of `layers` decoder layers for `clips` sequences of up
+    to `capacity` tokens.
+
+    prompt(), step() and verify() return the attention of the next forward
+    pass, a callable (layer, qkv) -> attention output for
+    ``DecoderStack.forward(x, attention=...)``, with qkv [rows, (heads + 2 *
+    kv_heads) * head_dim].  Lengths and pages are counted on the host; nothing
+    synchronises.  With ``totals`` the softmax weight of every cached token is
+    accumulated by step() and verify(), which evict() needs.  `spare` tokens of
+    pages per clip are held free for evict()."""
+
+    def __init__(self, layers, clips, capacity, heads, kv_heads, head_dim=128, page_size=64, totals=False, spare=0,
+                 position=None, device="cuda"):
+        self.heads, self.kv_heads, self.head_dim, self.page_size = heads, kv_heads, head_dim, page_size
+        self.device, self.position = device, position
+        self.width = -(-capacity // page_size)
+        pages = clips * (self.width + -(-spare // page_size))
+        self.caches = [KV8Cache(pages, kv_heads, head_dim, page_size, device) for _ in range(layers)]
+        self.free = list(range(pages))
+        self.pages = [[] for _ in range(clips)]
+        self.lens = [0] * clips
+        cap = self.width * page_size
+        self.totals = [torch.zeros(clips, kv_heads, cap, device=device) for _ in range(layers)] if totals else None
+        self._state()
+
+    def _state(self):
+        rows = [p + [-1] * (self.width - len(p)) for p in self.pages]
+        self.table = torch.tensor(rows, dtype=torch.int32, device=self.device)
+        self.seq_lens = torch.tensor(self.lens, dtype=torch.int32, device=self.device)
+
+    def _take(self, n):
+        if n > len(self.free):
+            raise RuntimeError(f"key/value cache is out of pages ({n} wanted, {len(self.free)} free)")
+        return [self.free.pop() for _ in range(n)]
+
+    def _grow(self, new):
+        """Room for new[b] more tokens of each clip; returns the lengths before."""
+        if len(new) != len(self.lens):
+            raise ValueError(f"{len(new)} lengths for {len(self.lens)} clips")
+        before = list(self.lens)
+        after = [n + m for n, m in zip(before, new)]
+        need = [-(-n // self.page_size) - len(p) for n, p in zip(after, self.pages)]
+        if any(n < 0 for n in new) or any(n > self.width * self.page_size for n in after):
+            raise ValueError("a clip would pass the cache's capacity (or a length is negative)")
+        if sum(max(0, n) for n in need) > len(self.free):
+            raise RuntimeError("key/value cache is out of pages")
+        for p, n in zip(self.pages, need):
+            p += self._take(max(0, n))
+        self.lens = after
+        self._state()
+        return before
+
+    def _split(self, qkv):
+        x = qkv.view(-1, self.heads + 2 * self.kv_heads, self.head_dim)
+        q, k, v = x.split((self.heads, self.kv_heads, self.kv_heads), dim=1)
+        if self.position is not None:
+            q, k = self.position(q, k)
+        return q, k, v
+
+    def prompt(self, lens):
+        """Attention for lens[b] packed new tokens of each clip: causal among
+        themselves and, where the clip has cached tokens, over those too (read
+        back from the cache)."""
+        before = self._grow(list(lens))
+        cu = _offsets(lens, self.device)
+        starts = torch.tensor(before, dtype=torch.int32, device=self.device)
+        table, behind = self.table, any(n and m for n, m in zip(before, lens))
+        if behind:
+            # only clips with new tokens need their keys
+            ends = [n if m else 0 for n, m in zip(self.lens, lens)]
+            cu_k, rows, zero = _offsets(ends, self.device), sum(ends), torch.zeros_like(starts)
+
+        def attention(layer, qkv):
+            q, k, v = self._split(qkv)
+            cache = self.caches[layer]
+            cache.append(k, v, cu, starts, table)
+            if behind:
+                kk, vv = cache.gather(table, zero, cu_k, rows, q.dtype)
+                out = ops.attention_prefill(q, kk, vv, cu, cu_k)
+            else:
+                out = ops.attention_prefill(q, k, v, cu)
+            return out.view(-1, self.heads * self.head_dim)
+
+        return attention
+
+    def verify(self, new):
+        """Attention for `new` tokens of every clip (rows clip by clip), as a
+        draft's verification runs them; accept() says how many of them stay."""
+        clips = len(self.lens)
+        before = self._grow([new] * clips)
+        cu = _offsets([new] * clips, self.device)
+        starts = torch.tensor(before, dtype=torch.int32, device=self.device)
+        table, seq_lens = self.table, self.seq_lens
+
+        def attention(layer, qkv):
+            q, k, v = self._split(qkv)
+            cache = self.caches[layer]
+            cache.append(k, v, cu, starts, table)
+            out = cache.attend(q.view(clips, new, self.heads, self.head_dim) if q.is_contiguous()
+                               else q.unflatten(0, (clips, new)), table, seq_lens,
+                               weights=self.totals[layer] if self.totals else None)
+            return out.view(-1, self.heads * self.head_dim)
+
+        return attention
+
+    def step(self):
+        """Attention for one new token of every clip."""
+        return self.verify(1)
+
+    def accept(self, rejected):
+        """Take back the last rejected[b] tokens of each clip; their places are
+        written again by the next call.  (Page scales that they raised stay,
+        and so do the totals that they added to other tokens.)"""
+        if len(rejected) != len(self.lens) or any(r < 0 or r > n for r, n in zip(rejected, self.lens)):
+            raise ValueError("rejected: one count per clip, at most its length")
+        self.lens = [n - r for n, r in zip(self.lens, rejected)]
+        for b, n in enumerate(self.lens):
+            keep = -(-n // self.page_size)
+            self.free += self.pages[b][keep:]
+            del self.pages[b][keep:]
+            if self.totals and rejected[b]:
+                for t in self.totals:
+                    t[b, :, n:] = 0
+        self._state()
+
+    def evict(self, budget, sink=4, recent=0):
+        """Cut every clip to its `budget` most attended tokens per KV head (and
+        layer), its first `sink` and last `recent` ones among them.  Returns
+        the tokens kept, per layer."""
+        if self.totals is None:
+            raise RuntimeError("eviction needs a ClipCache with totals=True")
+        width = -(-budget // self.page_size)
+        if width > self.width:
+            raise ValueError("budget is larger than the cache's capacity")
+        fresh = [self._take(-(-min(n, budget) // self.page_size)) for n in self.lens]
+        out_table = torch.tensor([p + [-1] * (width - len(p)) for p in fresh], dtype=torch.int32, device=self.device)
+        kept = []
+        for i, cache in enumerate(self.caches):
+            tokens, totals, _ = cache.evict(self.totals[i], self.table, self.seq_lens, out_table, budget, sink, recent)
+            kept.append(tokens)
+            self.totals[i].zero_()
+            self.totals[i][:, :, :budget] = totals
+        for b in range(len(self.lens)):
+            self.free += self.pages[b]
+            self.pages[b] = fresh[b]
+            self.lens[b] = min(self.lens[b], budget)
+        self._state()
+        return kept

@@ -7,7 +7,9 @@
   residual add + RMSNorm -> gate_up -> SiLU * up -> down_proj.  Seeded
   random-init weights, quantised with the reference's recipe.  Independent
   clips shard across GPUs with no collective: every rank holds the whole
-  stack and runs its share of the tokens.
+  stack and runs its share of the tokens.  forward(x, attention=...) puts a
+  real attention between qkv and o_proj, such as kv_cache.ClipCache's over
+  an int8 paged cache.
 * ColumnShardedLinear — the sharded-prefill workload:
   one rotated linear whose output columns are split across the ranks of a
   process group; each rank computes its [M, N / world] block and a gather
@@ -141,8 +143,11 @@ class DecoderStack:
         return sum(syn.weight_stream_bytes(L[k]["N"], L[k]["K"]) for L in self.layers
                    for k in ("qkv", "o", "gate_up", "down"))
 
-    def forward(self, x, fused=True):
+    def forward(self, x, fused=True, attention=None):
         """x: bf16 [M, 3584] (one token per clip) -> bf16 [M, 3584].
+
+        attention: (layer, qkv [M, 4608]) -> [M, 3584]; None is the identity
+        on the query heads.
 
         fused: the residual add + RMSNorm before qkv and gate_up and the
         SiLU * up before down run inside those linears' activation kernels
@@ -150,7 +155,7 @@ class DecoderStack:
         kernels (add_rmsnorm, silu_mul).  Both give the same bits."""
         res = None
         mlp_out = x
-        for L in self.layers:
+        for i, L in enumerate(self.layers):
             if self.per_projection:
                 qkv, res = group_rmsnorm(L["qkv"], mlp_out, res, L["in_norm"], self.eps, fused)
             elif fused:
@@ -158,7 +163,10 @@ class DecoderStack:
             else:
                 h, res = ops.add_rmsnorm(mlp_out, res, L["in_norm"], self.eps)
                 qkv = linear(L["qkv"], h)
-            attn = qkv[:, :HEADS * HEAD_DIM].contiguous()   # identity attention
+            if attention is None:
+                attn = qkv[:, :HEADS * HEAD_DIM].contiguous()   # identity attention
+            else:
+                attn = attention(i, qkv)
             o = linear(L["o"], attn)
             if self.per_projection:
                 gu, res = group_rmsnorm(L["gate_up"], o, res, L["post_norm"], self.eps, fused)
