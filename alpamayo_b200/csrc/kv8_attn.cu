@@ -162,7 +162,12 @@ struct DecodeTile {
   static constexpr int kStage = kSlots * 512 + 32;       // + the unit's four scales
   static constexpr int kCtas = 3;                        // CTAs per SM
   static constexpr int kStages = kWr == 4 ? 4 : kWr == 2 ? 3 : D == 128 ? 2 : 4;
-  static constexpr int kRing = kTeams * kStages * kStage;
+  // Teams of four: the expanded codes, shared by the team, as the 16-byte
+  // fragments of the products ([K, V][16 or 8 slots][lanes]) and the scales;
+  // two buffers, so that one barrier per unit will do.
+  static constexpr bool kShare = kWr == 4;
+  static constexpr int kFrag = 2 * (D / 8) * 512 + 32;
+  static constexpr int kRing = kTeams * kStages * kStage + (kShare ? 2 * kFrag : 0);
   static constexpr int kComb = kTeams > 1 ? RB * D * 4 + RB * 32 : 0;   // one team's partial on its way to the next
   static constexpr int kSmem = kRing + kComb;
 };
@@ -183,6 +188,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, (DecodeTile<D, RB>::kCtas)) kv
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int team = warp / C::kWr, wr = warp % C::kWr;
   uint8_t* ring = smem + team * (C::kStages * C::kStage);
+  [[maybe_unused]] uint8_t* frags = smem + C::kTeams * C::kStages * C::kStage;
   float4* comb = reinterpret_cast<float4*>(smem + C::kRing) + wr * (NT * 32);   // [NT][lanes]
   float2* comb_ml = reinterpret_cast<float2*>(smem + C::kRing + RB * D * 4) + wr * (kHalves * 32);
   const Kv8View& c = p.c;
@@ -260,15 +266,27 @@ __global__ void __launch_bounds__(kDecWarps * 32, (DecodeTile<D, RB>::kCtas)) kv
                      c.k_codes + kb[j >> 1] + ((j & 1) * 8 + g) * D + i * 64 + t * 16);
       }
       // V: slot (kk, x) = token 16 kk + {2t, 2t + 1, 2t + 8, 2t + 9}[x], bytes of lane g's D / 8 columns
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk)
+      if constexpr (C::kShare) {
+        // what this warp will expand: one kk, half of the columns
+        const int kk = wr >> 1;
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          if ((kk * 4 + x) % C::kWr != wr) continue;
-          const int64_t off = kb[kk] + (2 * t + (x & 1) + (x >> 1) * 8) * D + g * (D / 8);
-          if constexpr (D == 128) cp_async16(dst + (D / 16 + kk * 4 + x) * 512, c.v_codes + off);
-          else cp_async8(at + 4 * 512 + (kk * 4 + x) * 256 + lane * 8, c.v_codes + off);
+          const int64_t off = (kk ? kb[1] : kb[0]) + (2 * t + (x & 1) + (x >> 1) * 8) * D + g * (D / 8) + (wr & 1) * (D / 16);
+          const uint32_t to = at + (D / 16) * 512 + (wr * 4 + x) * (2 * D) + lane * (D / 16);
+          if constexpr (D == 128) cp_async8(to, c.v_codes + off);
+          else cp_async4(to, c.v_codes + off);
         }
+      } else {
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            if ((kk * 4 + x) % C::kWr != wr) continue;
+            const int64_t off = kb[kk] + (2 * t + (x & 1) + (x >> 1) * 8) * D + g * (D / 8);
+            if constexpr (D == 128) cp_async16(dst + (D / 16 + kk * 4 + x) * 512, c.v_codes + off);
+            else cp_async8(at + 4 * 512 + (kk * 4 + x) * 256 + lane * 8, c.v_codes + off);
+          }
+      }
       if (lane < 4 && wr == 0) {
         const float* sc = (lane < 2 ? c.k_scale : c.v_scale) + (int64_t)((lane & 1) ? n.id[1] : n.id[0]) * c.kv_heads + n.head;
         cp_async4(at + C::kSlots * 512 + lane * 4, sc);
@@ -278,9 +296,9 @@ __global__ void __launch_bounds__(kDecWarps * 32, (DecodeTile<D, RB>::kCtas)) kv
   };
   ahead[0] = look_up();
   ahead[1] = look_up();
-  // A team of one warp refills a stage when it has used it; a larger team
-  // when the barrier of the next unit says that all of it has.
-  constexpr bool kAlone = C::kWr == 1;
+  // A warp that reads its own copies alone refills a stage when it has used
+  // it; otherwise when the barrier of the next unit says that the team has.
+  constexpr bool kAlone = C::kWr == 1 || C::kShare;
 #pragma unroll
   for (int s = 0; s < C::kStages - (kAlone ? 0 : 1); ++s) issue(s);
 
@@ -308,6 +326,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, (DecodeTile<D, RB>::kCtas)) kv
     }
   };
   int stage = 0;
+  [[maybe_unused]] int buf = 0;
   int cu = u0 + team;                       // this team's next unit
   int seg0 = u0;                            // current segment: units [seg0, seg1) of (b, h)
   int seg_first = u0 - unit0;               // flat index of (b, h)'s unit 0
@@ -373,14 +392,62 @@ __global__ void __launch_bounds__(kDecWarps * 32, (DecodeTile<D, RB>::kCtas)) kv
     for (; cu < seg1; cu += C::kTeams) {
       // the other lanes' copies (the scales) and the other warps' are in
       cp_wait<C::kStages - (kAlone ? 1 : 2)>();
-      if constexpr (kAlone) {
+      if constexpr (C::kShare) {
+        // this warp's quarter of the unit, expanded once for the team
+        const uint8_t* raw = ring + stage * C::kStage;
+        uint4* fk = reinterpret_cast<uint4*>(frags + buf * C::kFrag) + lane;
+        uint4* fv = fk + (D / 8) * 32;
+        __syncwarp();                        // the scales are other lanes' copies
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) {
+          const uint4 kw = *reinterpret_cast<const uint4*>(raw + (wr * (D / 64) + i) * 512 + lane * 16);
+          const uint32_t w4[4] = {kw.x ^ 0x80808080u, kw.y ^ 0x80808080u, kw.z ^ 0x80808080u, kw.w ^ 0x80808080u};
+#pragma unroll
+          for (int w = 0; w < 4; w += 2)
+            fk[((wr * (D / 64) + i) * 2 + w / 2) * 32] =
+                make_uint4(codes_f16x2(w4[w], 0x4140), codes_f16x2(w4[w], 0x4342), codes_f16x2(w4[w + 1], 0x4140),
+                           codes_f16x2(w4[w + 1], 0x4342));
+        }
+        uint32_t vw[4][VW / 2];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const uint8_t* from = raw + (D / 16) * 512 + (wr * 4 + x) * (2 * D) + lane * (D / 16);
+          if constexpr (D == 128) {
+            const uint2 w = *reinterpret_cast<const uint2*>(from);
+            vw[x][0] = w.x;
+            vw[x][1] = w.y;
+          } else {
+            vw[x][0] = *reinterpret_cast<const uint32_t*>(from);
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < VW / 2; ++w) {
+          const uint32_t a_lo = __byte_perm(vw[0][w], vw[1][w], 0x5140) ^ 0x80808080u;
+          const uint32_t a_hi = __byte_perm(vw[0][w], vw[1][w], 0x7362) ^ 0x80808080u;
+          const uint32_t c_lo = __byte_perm(vw[2][w], vw[3][w], 0x5140) ^ 0x80808080u;
+          const uint32_t c_hi = __byte_perm(vw[2][w], vw[3][w], 0x7362) ^ 0x80808080u;
+          const int slot = ((wr >> 1) * VW + (wr & 1) * (VW / 2) + w) * 2;
+          fv[slot * 32] = make_uint4(codes_f16x2(a_lo, 0x4140), codes_f16x2(c_lo, 0x4140), codes_f16x2(a_lo, 0x4342),
+                                     codes_f16x2(c_lo, 0x4342));
+          fv[(slot + 1) * 32] = make_uint4(codes_f16x2(a_hi, 0x4140), codes_f16x2(c_hi, 0x4140),
+                                           codes_f16x2(a_hi, 0x4342), codes_f16x2(c_hi, 0x4342));
+        }
+        if (wr == 0 && lane < 4)
+          reinterpret_cast<float*>(frags + buf * C::kFrag + 2 * (D / 8) * 512)[lane] =
+              reinterpret_cast<const float*>(raw + C::kSlots * 512)[lane];
+        __syncwarp();
+        issue(stage);
+        named_barrier(1 + team, C::kWr * 32);
+      } else if constexpr (kAlone) {
         __syncwarp();
       } else {
         named_barrier(1 + team, C::kWr * 32);
         issue(stage == 0 ? C::kStages - 1 : stage - 1);
       }
       const uint8_t* st = ring + stage * C::kStage;
-      const float* sc = reinterpret_cast<const float*>(st + C::kSlots * 512);
+      const float* sc = reinterpret_cast<const float*>(C::kShare ? frags + buf * C::kFrag + 2 * (D / 8) * 512
+                                                                 : st + C::kSlots * 512);
+      [[maybe_unused]] const uint4* fk = reinterpret_cast<const uint4*>(frags + buf * C::kFrag) + lane;
       const float ks[2] = {sc[0], sc[1]}, vs[2] = {sc[2], sc[3]};
       const int tok0 = (cu - seg_first) * kUnit;
       // scores
@@ -389,14 +456,23 @@ __global__ void __launch_bounds__(kDecWarps * 32, (DecodeTile<D, RB>::kCtas)) kv
       for (int j = 0; j < 4; ++j) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[j][e] = 0.f;
+        if constexpr (C::kShare) {
 #pragma unroll
-        for (int i = 0; i < D / 64; ++i) {
-          const uint4 kw = *reinterpret_cast<const uint4*>(st + (j * (D / 64) + i) * 512 + lane * 16);
-          const uint32_t w4[4] = {kw.x, kw.y, kw.z, kw.w};
+          for (int w = 0; w < D / 32; ++w) {
+            const uint4 f = fk[(j * (D / 32) + w) * 32];
+            mma_f16(s[j], qf[2 * w], f.x, f.y);
+            mma_f16(s[j], qf[2 * w + 1], f.z, f.w);
+          }
+        } else {
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const uint32_t bi = w4[w] ^ 0x80808080u;
-            mma_f16(s[j], qf[i * 4 + w], codes_f16x2(bi, 0x4140), codes_f16x2(bi, 0x4342));
+          for (int i = 0; i < D / 64; ++i) {
+            const uint4 kw = *reinterpret_cast<const uint4*>(st + (j * (D / 64) + i) * 512 + lane * 16);
+            const uint32_t w4[4] = {kw.x, kw.y, kw.z, kw.w};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const uint32_t bi = w4[w] ^ 0x80808080u;
+              mma_f16(s[j], qf[i * 4 + w], codes_f16x2(bi, 0x4140), codes_f16x2(bi, 0x4342));
+            }
           }
         }
       }
@@ -456,43 +532,54 @@ __global__ void __launch_bounds__(kDecWarps * 32, (DecodeTile<D, RB>::kCtas)) kv
       // values
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
-        uint32_t vw[4][VW];
+        if constexpr (C::kShare) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          if constexpr (D == 128) {
-            const uint4 w = *reinterpret_cast<const uint4*>(st + (D / 16 + kk * 4 + x) * 512 + lane * 16);
-            vw[x][0] = w.x;
-            vw[x][1] = w.y;
-            vw[x][2] = w.z;
-            vw[x][3] = w.w;
-          } else {
-            const uint2 w = *reinterpret_cast<const uint2*>(st + 4 * 512 + (kk * 4 + x) * 256 + lane * 8);
-            vw[x][0] = w.x;
-            vw[x][1] = w.y;
+          for (int w = 0; w < VW * 2; ++w) {
+            const uint4 f = fk[(D / 8 + kk * VW * 2 + w) * 32];
+            mma_f16(o[2 * w], pa[kk], f.x, f.y);
+            mma_f16(o[2 * w + 1], pa[kk], f.z, f.w);
           }
-        }
+        } else {
+          uint32_t vw[4][VW];
 #pragma unroll
-        for (int w = 0; w < VW; ++w) {
-          [[maybe_unused]] uint32_t va[4];
-          const uint32_t a_lo = __byte_perm(vw[0][w], vw[1][w], 0x5140) ^ 0x80808080u;
-          const uint32_t a_hi = __byte_perm(vw[0][w], vw[1][w], 0x7362) ^ 0x80808080u;
-          const uint32_t c_lo = __byte_perm(vw[2][w], vw[3][w], 0x5140) ^ 0x80808080u;
-          const uint32_t c_hi = __byte_perm(vw[2][w], vw[3][w], 0x7362) ^ 0x80808080u;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t b0 = codes_f16x2(e < 2 ? a_lo : a_hi, (e & 1) ? 0x4342 : 0x4140);
-            const uint32_t b1 = codes_f16x2(e < 2 ? c_lo : c_hi, (e & 1) ? 0x4342 : 0x4140);
-            if constexpr (kUpper) {
-              mma_f16(o[w * 4 + e], pa[kk], b0, b1);
+          for (int x = 0; x < 4; ++x) {
+            if constexpr (D == 128) {
+              const uint4 w = *reinterpret_cast<const uint4*>(st + (D / 16 + kk * 4 + x) * 512 + lane * 16);
+              vw[x][0] = w.x;
+              vw[x][1] = w.y;
+              vw[x][2] = w.z;
+              vw[x][3] = w.w;
             } else {
-              va[(e & 1)] = b0;
-              va[2 + (e & 1)] = b1;
-              if (e & 1) mma_f16(o[w * 2 + (e >> 1)], va, pa[kk][0], pa[kk][2]);
+              const uint2 w = *reinterpret_cast<const uint2*>(st + 4 * 512 + (kk * 4 + x) * 256 + lane * 8);
+              vw[x][0] = w.x;
+              vw[x][1] = w.y;
+            }
+          }
+#pragma unroll
+          for (int w = 0; w < VW; ++w) {
+            [[maybe_unused]] uint32_t va[4];
+            const uint32_t a_lo = __byte_perm(vw[0][w], vw[1][w], 0x5140) ^ 0x80808080u;
+            const uint32_t a_hi = __byte_perm(vw[0][w], vw[1][w], 0x7362) ^ 0x80808080u;
+            const uint32_t c_lo = __byte_perm(vw[2][w], vw[3][w], 0x5140) ^ 0x80808080u;
+            const uint32_t c_hi = __byte_perm(vw[2][w], vw[3][w], 0x7362) ^ 0x80808080u;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t b0 = codes_f16x2(e < 2 ? a_lo : a_hi, (e & 1) ? 0x4342 : 0x4140);
+              const uint32_t b1 = codes_f16x2(e < 2 ? c_lo : c_hi, (e & 1) ? 0x4342 : 0x4140);
+              if constexpr (kUpper) {
+                mma_f16(o[w * 4 + e], pa[kk], b0, b1);
+              } else {
+                va[(e & 1)] = b0;
+                va[2 + (e & 1)] = b1;
+                if (e & 1) mma_f16(o[w * 2 + (e >> 1)], va, pa[kk][0], pa[kk][2]);
+              }
             }
           }
         }
       }
-      if constexpr (kAlone) {
+      if constexpr (C::kShare) {
+        buf ^= 1;
+      } else if constexpr (kAlone) {
         __syncwarp();                        // every lane has read the stage's scales
         issue(stage);
       }

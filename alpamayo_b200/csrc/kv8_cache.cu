@@ -113,6 +113,35 @@ __device__ __forceinline__ void codes_of(const float (&x)[N], const CodeScale& c
   }
 }
 
+// Codes under `cs` of 16 old codes c under the scale `sc`: those of the
+// float32 products c * sc, as codes_of gives them.  c times fl(sc / s) is
+// within 3.1e-5 of their rounded quotient.
+__device__ __forceinline__ void recodes_of(const float (&c)[16], float sc, const CodeScale& cs, uint32_t (&out)[4]) {
+  const float r = __fmul_rn(sc, cs.inv);
+  const float2 r2 = make_float2(r, r), magic = make_float2(12582912.f, 12582912.f);
+  float far = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; i += 4) {
+    uint32_t q[4];
+#pragma unroll
+    for (int k = 0; k < 4; k += 2) {
+      const float2 v = make_float2(c[i + k], c[i + k + 1]);
+      const float2 z = __ffma2_rn(v, r2, magic);
+      const float2 d = __ffma2_rn(v, r2, __ffma2_rn(z, make_float2(-1.f, -1.f), magic));   // from the integer
+      q[k] = __float_as_uint(z.x);
+      q[k + 1] = __float_as_uint(z.y);
+      far = fmaxf(far, fmaxf(fabsf(d.x), fabsf(d.y)));
+    }
+    out[i / 4] = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+  }
+  if (cs.slow || !(far <= 0.4999f) || !(r < 1e30f)) {
+#pragma unroll
+    for (int i = 0; i < 16; i += 4)
+      out[i / 4] = codes_div(__fmul_rn(c[i], sc), __fmul_rn(c[i + 1], sc), __fmul_rn(c[i + 2], sc),
+                             __fmul_rn(c[i + 3], sc), cs.scale);
+  }
+}
+
 // Running maximum of |x|: of 16-bit types as two 16-bit lanes of a word (the
 // bits of non-negative floats are ordered as integers, NaN above infinity,
 // so a NaN shows in the result), of float32 as a word.
@@ -561,8 +590,9 @@ __global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(EvictParams p, 
 // a team of as many warps as its pieces of 16 codes need at 8 to a lane, all
 // of them in flight at once.  With a block of 256 threads per task, an index
 // list in shared memory and two barriers, the same work took 90 us instead of
-// 62 for 64 sequences cut to 2048 tokens.
-constexpr int kCmpThreads = 128;
+// 78 for 64 sequences cut to 2048 tokens (warps in blocks of 128: 89, of 512:
+// 107; teams that walk the tasks with the grid's stride: 117).
+constexpr int kCmpThreads = 256;
 constexpr int kCmpPieces = 8;
 
 template <int D>
@@ -647,13 +677,7 @@ __global__ void __launch_bounds__(kCmpThreads) kv8_compact_kernel(EvictParams p,
     float f[16];
     uint32_t q[4];
     unpack_codes16(v[i], f);
-#pragma unroll
-    for (int k = 0; k < 16; k += 2) {
-      const float2 y = __fmul2_rn(make_float2(f[k], f[k + 1]), make_float2(sc, sc));
-      f[k] = y.x;
-      f[k + 1] = y.y;
-    }
-    codes_of(f, cs, q);
+    recodes_of(f, sc, cs, q);
     if ((i * 32 + lane) >> kShift < mine)
       *reinterpret_cast<uint4*>(dst + (int64_t)(i * 32 + lane) * 16) = make_uint4(q[0], q[1], q[2], q[3]);
   }
