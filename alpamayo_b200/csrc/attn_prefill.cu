@@ -3,7 +3,7 @@
 //
 //   o_i = sum_{j <= i + Lk - Lq} softmax_j(scale * q_i . k_j) v_j
 //
-// One CTA per (256 query rows of one sequence, head): two tiles of 128 rows
+// An item is 256 query rows of one sequence and head: two tiles of 128 rows
 // that share every key/value tile of 128 tokens, walked with a running
 // maximum and sum.  Bound by the tensor cores (4 * dim flops per pair) and,
 // nearly as much, by the exponentials: a 128 x 128 tile takes 2 * 512 clocks
@@ -15,7 +15,16 @@
 //    The output is rescaled only when a row's maximum has grown by more than
 //    2^8 since the reference maximum in use (any exact common factor of
 //    terms and sum cancels), so nearly never.
-//  * warp 8: TMA loads, K_0 V_0 K_1 V_1 ... through one ring of tiles.
+//  * warp 8: finds the items and loads their tiles with TMA, K_0 V_0 K_1 V_1
+//    ... through one ring that runs on from item to item.  The launch has a
+//    CTA per item; one that is running takes over the items of those that
+//    have not started (the hardware's cancel request), so the next item's
+//    queries, first keys and first scores are under way while the softmax
+//    warps store the last one's output.  28 heads, 8 prompts of 1 to 1500
+//    tokens (560 items of 1 to 12 tiles): 61 us with an item per CTA, 58 with
+//    the items shared out evenly beforehand, 53 like this; one prompt of 8192
+//    gains 1 %; one of 37, whose items have a CTA each either way, takes 7.9
+//    us for 7.5 (the hand-over of its description).
 //  * warp 9: MMAs, one thread: S = Q K^T (both K-major in shared memory) and
 //    O += P V (P in tensor memory, V with its columns contiguous, i.e.
 //    MN-major).  In issue order ... O_0 += P_0(j) V_j, S_0 = Q_0 K_(j+1),
@@ -44,6 +53,18 @@ constexpr int kPfThreads = 384;
 constexpr int kPfSplits = 8;       // splits of an item's keys, at most
 constexpr int kPfMasked = 3;       // key tiles that a CTA's rows see in part, at most
 
+// Division of 0 .. 2^31 - 1 by a divisor that the host knows: the rounded-up
+// reciprocal gives the quotient or one more.
+struct Divisor {
+  int d;
+  uint64_t inv;                    // ceil(2^32 / d)
+  explicit Divisor(int d) : d(d), inv(((1ull << 32) + d - 1) / d) {}
+  __device__ __forceinline__ int operator()(int n) const {
+    const int q = (int)(((uint64_t)n * inv) >> 32);
+    return q - ((int64_t)q * d > n);
+  }
+};
+
 struct PrefillParams {
   const int32_t* cu_q;
   const int32_t* cu_k;
@@ -53,6 +74,8 @@ struct PrefillParams {
   void* out;
   const void* v;                   // for the values that are not finite
   int64_t sv_t, sv_h;
+  Divisor by_heads, by_group, by_splits;
+  int sms;
   int splits;                      // CTAs that share the keys of one item; > 1: partial results
   float* part_o;                   // [splits][rows][heads][dim] sums of terms times values
   float2* part_ml;                 // [splits][rows][heads] (reference maximum, sum of terms), in log2 units
@@ -62,12 +85,16 @@ template <int D>
 struct PrefillTile {
   static constexpr int kAtoms = D / 64;                    // 128-byte wide columns of a tile
   static constexpr int kTileBytes = kPfRows * D * 2;       // one Q, K or V tile
-  static constexpr int kSlots = 5;
+  static constexpr int kSlots = D == 128 ? 4 : 6;
   static constexpr int kOffKv = 2 * kTileBytes;
-  static constexpr int kOffBar = kOffKv + kSlots * kTileBytes;
-  static constexpr int kSmem = kOffBar + 512 + 1024;
+  static constexpr int kOffStage = kOffKv + kSlots * kTileBytes;   // [8 warps][32 rows][64 columns] output on its way
+  static constexpr int kOffBar = kOffStage + 8 * 32 * 128;
+  static constexpr int kSmem = kOffBar + 768 + 1024;
   static constexpr int kTmemO = 256;                       // S_0, S_1: columns 0 and 128; O_0, O_1: from 256
 };
+
+// An item as the loader hands it to the other warps.
+enum { kCtxStop, kCtxQ0, kCtxLq, kCtxR0, kCtxH, kCtxOff, kCtxLk, kCtxJm, kCtxK0, kCtxNk, kCtxSplit = kCtxNk + 2, kCtxWords };
 
 namespace {
 
@@ -141,6 +168,13 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// 256-row items of sequence i (i = B: the rows behind the last sequence).
+__device__ __forceinline__ int prefill_tiles(const PrefillParams& p, int i) {
+  if (i > p.B) return 0;
+  const int lo = min(max(p.cu_q[i], 0), p.rows), hi = i < p.B ? min(max(p.cu_q[i + 1], lo), p.rows) : p.rows;
+  return (hi - lo + 2 * kPfRows - 1) / (2 * kPfRows);
+}
+
 template <typename T> __device__ __forceinline__ uint32_t pack16(float lo, float hi);
 template <> __device__ __forceinline__ uint32_t pack16<__nv_bfloat16>(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
@@ -180,123 +214,44 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
   using C = PrefillTile<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + C::kOffBar);  // [2]
-  uint64_t* full = q_full + 2;                                        // [slots] a K or V tile has landed
+  uint4* next = reinterpret_cast<uint4*>(smem + C::kOffBar);          // [1] answer to a request for the next item
+  uint64_t* next_full = reinterpret_cast<uint64_t*>(next + 1);        // [1] it has come
+  uint64_t* ctx_full = next_full + 1;                                 // [2] an item's description is written
+  uint64_t* ctx_empty = ctx_full + 2;                                 // [2] every warp is done with the item
+  uint64_t* q_full = ctx_empty + 2;                                   // [2] queries have landed
+  uint64_t* q_empty = q_full + 2;                                     // [2] their last scores are done
+  uint64_t* full = q_empty + 2;                                       // [slots] a K or V tile has landed
   uint64_t* empty = full + C::kSlots;                                 // [slots] its MMAs are done
   uint64_t* s_full = empty + C::kSlots;                               // [2] scores ready (and O up to date)
   uint64_t* p_ready = s_full + 2;                                     // [2][2] half a tile's probabilities written
   uint64_t* o_full = p_ready + 4;                                     // [2] output complete
-  uint64_t* v_full = o_full + 2;                                      // [3] partly seen value tile has landed
-  uint64_t* v_ok = v_full + kPfMasked;                                // [3] ... and is cleaned
-  uint64_t* done = v_ok + kPfMasked;                                  // [1] every MMA is done
+  uint64_t* v_full = o_full + 2;                                      // [2][3] partly seen value tile has landed
+  uint64_t* v_ok = v_full + 2 * kPfMasked;                            // [2][3] ... and is cleaned
+  uint64_t* done = v_ok + 2 * kPfMasked;                              // [1] every MMA is done
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
-  uint32_t* poison = tmem_slot + 1;                                   // [3][4] keys with values that are not finite
-  // the item, for the softmax warps: read where it is used, so that it takes
-  // no registers in their loop (a few spilled ones there cost 4 %)
-  volatile int* ctx = reinterpret_cast<volatile int*>(poison + 4 * kPfMasked);
-  enum { kCtxQ0, kCtxLq, kCtxR0, kCtxH, kCtxOff, kCtxLk, kCtxJm, kCtxK0, kCtxNk };
+  uint32_t* poisons = tmem_slot + 1;                                  // [2][3][4] keys with values that are not finite
+  // The items' descriptions, two deep; the softmax warps read them where they
+  // use them, so that they take no registers in their loop (a few spilled
+  // ones there cost 4 %).
+  volatile int* ctxs = reinterpret_cast<volatile int*>(poisons + 2 * 4 * kPfMasked);   // [2][kCtxWords]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 256) {   // the tensor maps' descriptors, fetched while the item is found
+  // the loader's lanes keep sequences 0 .. 31: offsets of queries and keys, items
+  const int cu_q0 = warp == 8 && lane <= p.B ? p.cu_q[lane] : 0, cu_k0 = warp == 8 && lane <= p.B ? p.cu_k[lane] : 0;
+  const int mine0 = warp == 8 ? prefill_tiles(p, lane) : 0;
+  if (threadIdx.x == 352) {
+    // the tensor maps' descriptors, fetched while the first item is found
     asm volatile("prefetch.tensormap [%0];" ::"l"(&qmap) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
   }
-  // This CTA's item: rows r0 .. of sequence b, head h.  Items are taken in
-  // order of the tile's place in its sequence, the last places of all
-  // sequences first (they see the most keys, and the longest work starts
-  // earliest).  left(t) items lie at place t or later; b = B stands for the
-  // rows behind the last sequence.
-  const int split = blockIdx.x % p.splits;
-  const int item = blockIdx.x / p.splits;
-  auto tiles_of = [&](int i) {
-    if (i > p.B) return 0;
-    const int lo = min(max(p.cu_q[i], 0), p.rows), hi = i < p.B ? min(max(p.cu_q[i + 1], lo), p.rows) : p.rows;
-    return (hi - lo + 2 * kPfRows - 1) / (2 * kPfRows);
-  };
-  const int mine0 = tiles_of(lane);            // sequences 0 .. 31 are kept in registers
-  auto left = [&](int t) {
-    int n = max(0, mine0 - t);
-    for (int b0 = 32; b0 <= p.B; b0 += 32) n += max(0, tiles_of(b0 + lane) - t);
-    return __reduce_add_sync(0xffffffffu, n);
-  };
-  int place = 0, b = -1, h = 0;
-  {
-    if (item >= left(0) * p.heads) return;
-    int most = mine0;
-    for (int b0 = 32; b0 <= p.B; b0 += 32) most = max(most, tiles_of(b0 + lane));
-    int hi = __reduce_max_sync(0xffffffffu, most);   // left(hi) = 0
-    while (hi - place > 1) {                         // the largest place with left(place) * heads > item
-      const int mid = (place + hi) >> 1;
-      if (left(mid) * p.heads > item) place = mid;
-      else hi = mid;
-    }
-    const int rest = item - left(place + 1) * p.heads;
-    int nth = rest / p.heads;                        // of the sequences that have such a place
-    h = rest - nth * p.heads;
-    for (int b0 = 0; b0 <= p.B && b < 0; b0 += 32) {
-      unsigned has = __ballot_sync(0xffffffffu, (b0 ? tiles_of(b0 + lane) : mine0) > place);
-      if (nth >= __popc(has)) {
-        nth -= __popc(has);
-        continue;
-      }
-      for (; nth > 0; --nth) has &= has - 1;
-      b = b0 + __ffs(has) - 1;
-    }
-  }
-  const int hk = h / p.group;
-  const int q0 = min(max(p.cu_q[b], 0), p.rows);
-  const int lq = (b < p.B ? min(max(p.cu_q[b + 1], q0), p.rows) : p.rows) - q0;
-  int k0 = b < p.B ? min(max(p.cu_k[b], 0), p.k_rows) : 0;
-  int lk = b < p.B ? min(max(p.cu_k[b + 1], k0), p.k_rows) - k0 : 0;
-  if (threadIdx.x == 0 && b < p.B && (q0 != p.cu_q[b] || lq != p.cu_q[b + 1] - q0 || k0 != p.cu_k[b] ||
-                                      lk != p.cu_k[b + 1] - k0))
-    report_error(kErrBadPage);
-  const int r0 = place * 2 * kPfRows;
-  int off = lk - lq;                                 // row i sees keys j <= i + off
-  // key tiles of each row tile (0: no rows, or none that sees a key)
-  int nk[2];
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    const int begin = r0 + s * kPfRows, end = min(lq, begin + kPfRows);
-    nk[s] = begin < lq && end + off > 0 ? (end + off + kPfRows - 1) / kPfRows : 0;
-  }
-  T* out = static_cast<T*>(p.out);
-  // this split's key tiles are j0 .. : from here on keys are counted from there
-  if (p.splits > 1) {
-    const int all = max(nk[0], nk[1]), share = (all + p.splits - 1) / p.splits, j0 = min(all, split * share);
-#pragma unroll
-    for (int s = 0; s < 2; ++s) nk[s] = max(0, min(nk[s], j0 + share) - j0);
-    k0 += j0 * kPfRows;
-    lk -= j0 * kPfRows;
-    off -= j0 * kPfRows;
-  }
-  const int nmax = max(nk[0], nk[1]);
-  const int jm = min(nmax, max(0, (r0 + off + 1) / kPfRows));   // tiles from jm on are seen in part by some row
-  if (nmax == 0) {                                         // nothing to see: zeros
-    const int n = min(2 * kPfRows, lq - r0);
-    if (p.splits > 1) {
-      for (int r = threadIdx.x; r < n; r += kPfThreads)
-        p.part_ml[((int64_t)split * p.rows + q0 + r0 + r) * p.heads + h] = make_float2(-INFINITY, 0.f);
-      return;
-    }
-    for (int e = threadIdx.x; e < n * (D / 8); e += kPfThreads) {
-      const int r = e / (D / 8), d = (e - r * (D / 8)) * 8;
-      *reinterpret_cast<uint4*>(out + ((int64_t)(q0 + r0 + r) * p.heads + h) * D + d) = make_uint4(0u, 0u, 0u, 0u);
-    }
-    return;
-  }
-
-  // the loader's thread sets up the barriers and starts the first copies
-  // before the CTA meets
-  auto load = [&](const CUtensorMap* map, uint8_t* dst, int head, int row, uint64_t* bar) {
-    mbar_arrive_expect_tx(bar, C::kTileBytes);
-#pragma unroll
-    for (int a = 0; a < C::kAtoms; ++a) tma_load_3d(dst + a * kPfRows * 128, map, a * 64, head, row, bar);
-  };
-  if (threadIdx.x == 256) {
+  if (threadIdx.x == 320) {
+    mbar_init(next_full, 1);
     for (int s = 0; s < 2; ++s) {
+      mbar_init(&ctx_full[s], 1);
+      mbar_init(&ctx_empty[s], 11);     // 8 softmax warps, the MMA warp, 2 cleaning warps
       mbar_init(&q_full[s], 1);
+      mbar_init(&q_empty[s], 1);
       mbar_init(&s_full[s], 1);
       mbar_init(&p_ready[2 * s], 4);
       mbar_init(&p_ready[2 * s + 1], 4);
@@ -306,61 +261,210 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
-    for (int i = 0; i < kPfMasked; ++i) {
+    for (int i = 0; i < 2 * kPfMasked; ++i) {
       mbar_init(&v_full[i], 1);
       mbar_init(&v_ok[i], 2);
     }
     mbar_init(done, 1);
     fence_mbar_init();
-    if (nk[0]) load(&qmap, smem, h, q0 + r0, &q_full[0]);
-    load(&kmap, smem + C::kOffKv, hk, k0, &full[0]);
-    if (nk[1]) load(&qmap, smem + C::kTileBytes, h, q0 + r0 + kPfRows, &q_full[1]);
   }
-  if (threadIdx.x < 4 * kPfMasked) poison[threadIdx.x] = 0u;
-  if (threadIdx.x == 0) {
-    ctx[kCtxQ0] = q0;
-    ctx[kCtxLq] = lq;
-    ctx[kCtxR0] = r0;
-    ctx[kCtxH] = h;
-    ctx[kCtxOff] = off;
-    ctx[kCtxLk] = lk;
-    ctx[kCtxJm] = jm;
-    ctx[kCtxK0] = k0;
-    ctx[kCtxNk] = nk[0];
-    ctx[kCtxNk + 1] = nk[1];
+  if (warp == 10) {                            // the loader goes on as soon as the barriers are there
+    __syncwarp();
+    asm volatile("bar.arrive 1, 64;" ::: "memory");
   }
   if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "n"(512)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  // 256 x 176 + 128 x 152 = 384 x 168 registers.  The softmax warps need no
+  // more than 176; with 184 to 200 of them the same code took 1 to 3 % longer
+  // or the other warps' spilled.
+  if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 152;");
+  // Every warp meets here but the loader's, which needs nothing of the others
+  // and has begun by now.
+  if (warp == 8) {
+    asm volatile("bar.arrive 2, 384;" ::: "memory");
+    asm volatile("bar.sync 1, 64;" ::: "memory");
+  } else {
+    tc_fence_before();
+    asm volatile("bar.sync 2, 384;" ::: "memory");
+    tc_fence_after();
+  }
+  const uint32_t tmem = warp == 8 ? 0u : *tmem_slot;
+  auto all_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0; };
 
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (warp == 8 && lane == 0) {
-      // loader: ring position 2 j holds K_j, 2 j + 1 holds V_j; K_0 and the
-      // queries are on their way
-      int n = 1;
-      for (; n < 2 * nmax; ++n) {
-        const int s = n % C::kSlots;
-        if (n >= C::kSlots && !mbar_wait(&empty[s], ((n / C::kSlots) - 1) & 1)) break;
-        // a partly seen value tile goes to the cleaning warps: it has a
-        // barrier of its own, and the slot's passes on to the next phase
-        const bool masked = (n & 1) && (n >> 1) >= jm;
-        if (masked) mbar_arrive(&full[s]);
-        load((n & 1) ? &vmap : &kmap, smem + C::kOffKv + s * C::kTileBytes, hk, k0 + (n >> 1) * kPfRows,
-             masked ? &v_full[(n >> 1) - jm] : &full[s]);
+    if (warp == 8) {
+      // Loader.  The whole warp finds the next item; one lane loads.
+      auto left = [&](int t) {                             // items of one head at place t or later
+        int n = max(0, mine0 - t);
+        for (int b0 = 32; b0 <= p.B; b0 += 32) n += max(0, prefill_tiles(p, b0 + lane) - t);
+        return __reduce_add_sync(0xffffffffu, n);
+      };
+      const int total = left(0) * p.heads * p.splits;
+      auto load = [&](const CUtensorMap* map, uint8_t* dst, int head, int row, uint64_t* bar) {
+        mbar_arrive_expect_tx(bar, C::kTileBytes);
+#pragma unroll
+        for (int a = 0; a < C::kAtoms; ++a) tma_load_3d(dst + a * kPfRows * 128, map, a * 64, head, row, bar);
+      };
+      uint32_t slot = 0, phase = 1;                        // ring: a fresh `empty` passes for the first round
+      uint32_t q_phase[2] = {1u, 1u}, v_phase = 0, asked = 0;
+      bool ok = true, open = false;              // open: a request has no answer yet
+      int it = blockIdx.x;
+      for (int n = 0; ok; ++n) {
+        const int c = n & 1;
+        if (n >= 2 && !all_wait(&ctx_empty[c], ((n >> 1) - 1) & 1)) break;
+        // Items in order of their place in their sequence, the last places of
+        // all sequences first (they see the most keys).  A CTA takes over the
+        // items of CTAs that have not started, one while it works on the last.
+        if (n > 0) it = -1;
+        while (n > 0 && total > p.sms) {                // otherwise every item has a CTA of its own
+          if (lane == 0) {
+            mbar_arrive_expect_tx(next_full, 16);
+            asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+                         ::"r"(smem_u32(next)), "r"(smem_u32(next_full)) : "memory");
+          }
+          open = true;
+          if (!all_wait(next_full, asked & 1)) break;
+          open = false;
+          ++asked;
+          uint4 w;
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(smem_u32(next)) : "memory");
+          uint32_t taken = 0, x = 0;
+          asm volatile(
+              "{\n.reg .pred p;\n.reg .b128 a;\n.reg .b64 lo, hi;\n"
+              "mov.b64 lo, {%2, %3};\nmov.b64 hi, {%4, %5};\nmov.b128 a, {lo, hi};\n"
+              "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n"
+              "selp.u32 %0, 1, 0, p;\n"
+              "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, a;\n}"
+              : "=r"(taken), "+r"(x)
+              : "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w));
+          if (!taken) break;
+          fence_proxy_async_smem();                        // this read comes before the next answer
+          __syncwarp();
+          if ((int)x < total) {
+            it = (int)x;
+            break;
+          }
+        }
+        volatile int* ctx = ctxs + c * kCtxWords;
+        if (it < 0 || it >= total) {
+          if (lane == 0) {
+            ctx[kCtxStop] = 1;
+            mbar_arrive(&ctx_full[c]);
+          }
+          break;
+        }
+        const int item = p.by_splits(it), split = it - item * p.splits;
+        int place = 0, hi = p.rows / (2 * kPfRows) + 1, above = 0, b = -1;
+        while (hi - place > 1) {                           // the largest place with left(place) * heads > item
+          const int mid = (place + hi) >> 1, n_mid = left(mid) * p.heads;
+          if (n_mid > item) {
+            place = mid;
+          } else {
+            hi = mid;
+            above = n_mid;                                 // items of later places
+          }
+        }
+        const int rest = item - above;
+        int nth = p.by_heads(rest);                          // of the sequences that have such a place
+        const int h = rest - nth * p.heads, hk = p.by_group(h);
+        for (int b0 = 0; b0 <= p.B && b < 0; b0 += 32) {
+          unsigned has = __ballot_sync(0xffffffffu, (b0 ? prefill_tiles(p, b0 + lane) : mine0) > place);
+          if (nth >= __popc(has)) {
+            nth -= __popc(has);
+            continue;
+          }
+          for (; nth > 0; --nth) has &= has - 1;
+          b = b0 + __ffs(has) - 1;                         // b = B: the rows behind the last sequence
+        }
+        // b < 31: from the lanes that keep them
+        const bool kept = b < 31, last = b == p.B;
+        const int cq0 = __shfl_sync(0xffffffffu, cu_q0, b & 31), cq1 = __shfl_sync(0xffffffffu, cu_q0, (b + 1) & 31);
+        const int ck0 = __shfl_sync(0xffffffffu, cu_k0, b & 31), ck1 = __shfl_sync(0xffffffffu, cu_k0, (b + 1) & 31);
+        const int bq0 = kept ? cq0 : p.cu_q[b], bq1 = last ? p.rows : kept ? cq1 : p.cu_q[b + 1];
+        const int bk0 = last ? 0 : kept ? ck0 : p.cu_k[b], bk1 = last ? 0 : kept ? ck1 : p.cu_k[b + 1];
+        const int q0 = min(max(bq0, 0), p.rows), lq = min(max(bq1, q0), p.rows) - q0;
+        int k0 = min(max(bk0, 0), p.k_rows), lk = min(max(bk1, k0), p.k_rows) - k0;
+        if (lane == 0 && !last && (q0 != bq0 || lq != bq1 - q0 || k0 != bk0 || lk != bk1 - k0)) report_error(kErrBadPage);
+        const int r0 = place * 2 * kPfRows;
+        int off = lk - lq;                                 // row i sees keys j <= i + off
+        // key tiles of each row tile (0: no rows, or none that sees a key)
+        int nk[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const int begin = r0 + s * kPfRows, end = min(lq, begin + kPfRows);
+          nk[s] = begin < lq && end + off > 0 ? (end + off + kPfRows - 1) / kPfRows : 0;
+        }
+        // this split's key tiles are j0 .. : from here on keys are counted from there
+        if (p.splits > 1) {
+          const int all = max(nk[0], nk[1]), share = p.by_splits(all + p.splits - 1), j0 = min(all, split * share);
+#pragma unroll
+          for (int s = 0; s < 2; ++s) nk[s] = max(0, min(nk[s], j0 + share) - j0);
+          k0 += j0 * kPfRows;
+          lk -= j0 * kPfRows;
+          off -= j0 * kPfRows;
+        }
+        const int nmax = max(nk[0], nk[1]);
+        const int jm = min(nmax, max(0, (r0 + off + 1) / kPfRows));   // tiles from jm on are seen in part by some row
+        if (lane < 4 * kPfMasked) poisons[c * 4 * kPfMasked + lane] = 0u;
+        __syncwarp();
+        if (lane == 0) {
+          ctx[kCtxStop] = 0;
+          ctx[kCtxQ0] = q0;
+          ctx[kCtxLq] = lq;
+          ctx[kCtxR0] = r0;
+          ctx[kCtxH] = h;
+          ctx[kCtxOff] = off;
+          ctx[kCtxLk] = lk;
+          ctx[kCtxJm] = jm;
+          ctx[kCtxK0] = k0;
+          ctx[kCtxNk] = nk[0];
+          ctx[kCtxNk + 1] = nk[1];
+          ctx[kCtxSplit] = split;
+          mbar_arrive(&ctx_full[c]);
+          // position 2 j of the item is K_j, 2 j + 1 is V_j; the queries come behind K_0
+#pragma unroll 1
+          for (int i = 0; i < 2 * nmax; ++i) {
+            if (i == 1) {
+#pragma unroll
+              for (int s = 0; s < 2; ++s)
+                if (nk[s] && ok) {
+                  ok = mbar_wait(&q_empty[s], q_phase[s]);
+                  q_phase[s] ^= 1;
+                  if (ok) load(&qmap, smem + s * C::kTileBytes, h, q0 + r0 + s * kPfRows, &q_full[s]);
+                }
+            }
+            if (!(ok = ok && mbar_wait(&empty[slot], phase))) break;
+            // a partly seen value tile goes to the cleaning warps: it has a
+            // barrier of its own, and the slot's passes on to the next phase
+            const int k = (i >> 1) - jm;
+            const bool part = (i & 1) && k >= 0;
+            if (part) mbar_arrive(&full[slot]);
+            load((i & 1) ? &vmap : &kmap, smem + C::kOffKv + slot * C::kTileBytes, hk, k0 + (i >> 1) * kPfRows,
+                 part ? &v_full[c * kPfMasked + k] : &full[slot]);
+            if (part) v_phase ^= 1u << (c * kPfMasked + k);
+            if (++slot == (uint32_t)C::kSlots) {
+              slot = 0;
+              phase ^= 1;
+            }
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
       }
-      // no copy is left in flight, whatever became of its readers
-      for (int i = max(0, n - C::kSlots); i < n; ++i)
-        mbar_wait((i & 1) && (i >> 1) >= jm ? &v_full[(i >> 1) - jm] : &full[i % C::kSlots],
-                  (i & 1) && (i >> 1) >= jm ? 0 : (i / C::kSlots) & 1);
-      if (nk[0]) mbar_wait(&q_full[0], 0);
-      if (nk[1]) mbar_wait(&q_full[1], 0);
+      // No copy is left in flight, whatever became of its readers: everything
+      // that was issued has landed when each barrier's last phase is over.
+      if (lane == 0) {
+        if (open) mbar_wait(next_full, asked & 1);
+        for (int i = 0; i < C::kSlots; ++i) {
+          const uint32_t last = (uint32_t)i < slot ? phase : phase ^ 1;   // the slot's last round, as `empty` counted it
+          mbar_wait(&full[i], last ^ 1);
+        }
+        for (int s = 0; s < 2; ++s) mbar_wait(&q_full[s], q_phase[s]);
+        for (int i = 0; i < 2 * kPfMasked; ++i) mbar_wait(&v_full[i], ((v_phase >> i) & 1) ^ 1);
+      }
     } else if (warp == 9) {
       constexpr uint32_t kFmt = (1u << 4) | (Type16<T>::kFmt << 7) | (Type16<T>::kFmt << 10) |
                                 ((uint32_t)(kPfRows >> 4) << 24);
@@ -369,11 +473,11 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
       const uint32_t leader = elect_one();
       // warp-uniform copies of what the loop depends on
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), base = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
-      const int un[2] = {__shfl_sync(0xffffffffu, nk[0], 0), __shfl_sync(0xffffffffu, nk[1], 0)};
-      const int umax = max(un[0], un[1]), um = __shfl_sync(0xffffffffu, jm, 0);
       const uint64_t dq = umma_desc_sw128(base), dk = umma_desc_sw128(base + C::kOffKv), dv = umma_desc_mn_sw128(base + C::kOffKv);
       constexpr uint32_t kStep = C::kTileBytes >> 4;
-      auto scores = [&](int s, uint32_t slot) {            // S_s = Q_s K^T, K in ring slot `slot`
+      // S_s = Q_s K^T, K in ring slot `slot`; after the item's last ones the
+      // queries' place is free
+      auto scores = [&](int s, uint32_t slot, bool last) {
         const uint64_t da = dq + s * kStep, db = dk + slot * kStep;
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
@@ -381,6 +485,7 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
           mma_f16_ss(tm + s * kPfRows, da + o, db + o, kIdS, k > 0, leader);
         }
         umma_commit(&s_full[s], leader);
+        if (last) umma_commit(&q_empty[s], leader);
       };
       auto values = [&](int s, uint32_t slot, int half, uint32_t acc) {   // O_s += P_s V, one half of the keys
         const uint64_t db = dv + slot * kStep;
@@ -390,268 +495,314 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
           mma_f16_ts(tm + C::kTmemO + s * 128, tm + s * kPfRows + k * 8, db + k * (2048 >> 4), kIdO, acc | (k > 0), leader);
         }
       };
-      // ring slot and phase of the tile that is waited for next
-      uint32_t slot = 0, phase = 0;
+      // ring slot and phase of the tile that is waited for next; phases of
+      // the other barriers
+      uint32_t slot = 0, phase = 0, p_phase[2] = {0u, 0u}, q_phase[2] = {0u, 0u}, v_phase = 0;
       auto advance = [&]() {
         if (++slot == (uint32_t)C::kSlots) {
           slot = 0;
           phase ^= 1;
         }
       };
-      // V_j and, unless it is the last, K_(j + 1) are in their slots
-      uint32_t vslot = 0, kslot = 0;
-      auto landed = [&](int j, uint32_t& v, uint32_t& k) {
-        v = slot;
-        bool r = j < um ? mbar_wait(&full[slot], phase) : mbar_wait(&v_ok[j - um], 0);
-        advance();
-        k = slot;
-        if (r && j + 1 < umax) r = mbar_wait(&full[slot], phase);
-        advance();
-        return r;
-      };
-      bool ok = mbar_wait(&full[0], 0);
-      advance();
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-        if (ok && un[s]) {
-          ok = mbar_wait(&q_full[s], 0);
-          if (ok) scores(s, 0);
-        }
-      if (ok) umma_commit(&empty[0], leader);
-      ok = ok && landed(0, vslot, kslot);
-      for (int j = 0; j < umax && ok; ++j) {
-        uint32_t vnext = 0, knext = 0;
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          if (j < un[s] && ok) {
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              ok = ok && mbar_wait(&p_ready[2 * s + half], j & 1);
-              tc_fence_after();
-              if (ok) values(s, vslot, half, j > 0);
+      bool ok = true;
+      for (int n = 0; ok; ++n) {
+        const int c = n & 1;
+        if (!all_wait(&ctx_full[c], (n >> 1) & 1)) break;
+        volatile int* ctx = ctxs + c * kCtxWords;
+        if (__shfl_sync(0xffffffffu, ctx[kCtxStop], 0)) break;
+        const int un[2] = {__shfl_sync(0xffffffffu, ctx[kCtxNk], 0), __shfl_sync(0xffffffffu, ctx[kCtxNk + 1], 0)};
+        const int umax = max(un[0], un[1]), um = __shfl_sync(0xffffffffu, ctx[kCtxJm], 0);
+        if (umax) {
+          // V_j and, unless it is the last, K_(j + 1) are in their slots
+          uint32_t vslot = 0, kslot = 0;
+          auto landed = [&](int j, uint32_t& v, uint32_t& k) {
+            v = slot;
+            const int i = c * kPfMasked + j - um;
+            bool r = j < um ? mbar_wait(&full[slot], phase) : mbar_wait(&v_ok[i], (v_phase >> i) & 1);
+            if (j >= um) v_phase ^= 1u << i;
+            advance();
+            if (j + 1 < umax) {
+              k = slot;
+              if (r) r = mbar_wait(&full[slot], phase);
+              advance();
             }
-            if (ok) {
-              if (j + 1 < un[s]) scores(s, kslot);
-              else umma_commit(&o_full[s], leader);
+            return r;
+          };
+          const uint32_t first = slot;
+          ok = mbar_wait(&full[slot], phase);
+          advance();
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+            if (ok && un[s]) {
+              ok = mbar_wait(&q_full[s], q_phase[s]);
+              q_phase[s] ^= 1;
+              if (ok) scores(s, first, un[s] == 1);
             }
+          if (ok) umma_commit(&empty[first], leader);
+          ok = ok && landed(0, vslot, kslot);
+          for (int j = 0; j < umax && ok; ++j) {
+            uint32_t vnext = 0, knext = 0;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+              if (j < un[s] && ok) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                  ok = ok && mbar_wait(&p_ready[2 * s + half], p_phase[s]);
+                  tc_fence_after();
+                  if (ok) values(s, vslot, half, j > 0);
+                }
+                p_phase[s] ^= 1;
+                if (ok) {
+                  if (j + 1 < un[s]) scores(s, kslot, j + 2 == un[s]);
+                  else umma_commit(&o_full[s], leader);
+                }
+              }
+              // the next tiles are waited for while the tensor core is busy
+              if (s == 0 && ok && j + 1 < umax) ok = landed(j + 1, vnext, knext);
+            }
+            if (!ok) break;
+            umma_commit(&empty[vslot], leader);
+            if (j + 1 < umax) umma_commit(&empty[kslot], leader);
+            vslot = vnext;
+            kslot = knext;
           }
-          // the next tiles are waited for while the tensor core is busy
-          if (s == 0 && ok && j + 1 < umax) ok = landed(j + 1, vnext, knext);
         }
-        if (!ok) break;
-        umma_commit(&empty[vslot], leader);
-        if (j + 1 < umax) umma_commit(&empty[kslot], leader);
-        vslot = vnext;
-        kslot = knext;
+        ok = __all_sync(0xffffffffu, ok) != 0;
+        if (ok && lane == 0) mbar_arrive(&ctx_empty[c]);
       }
+      __syncwarp();
       umma_commit(done, leader);               // the tensor memory is not freed under an MMA
       mbar_wait(done, 0);
-    } else if (warp >= 10) {
-      for (int j = jm; j < nmax; ++j) {
-        const int n = 2 * j + 1;
-        if (!__all_sync(0xffffffffu, mbar_wait(&v_full[j - jm], 0))) break;
-        uint8_t* tile = smem + C::kOffKv + (n % C::kSlots) * C::kTileBytes;
-        const int keys = min(kPfRows, lk - j * kPfRows);
-        // 16-byte pieces, 8 to a 128-byte row, eight of them at a time: one
-        // by one this took longer than a tile's MMAs and softmax
-        constexpr int kBatch = 8;
-        uint4* at = reinterpret_cast<uint4*>(tile) + (threadIdx.x - 320);
+    } else {
+      uint32_t at_item = 0, v_phase = 0;       // ring position of the item's K_0
+      for (int n = 0;; ++n) {
+        const int c = n & 1;
+        if (!all_wait(&ctx_full[c], (n >> 1) & 1)) break;
+        volatile int* ctx = ctxs + c * kCtxWords;
+        if (ctx[kCtxStop]) break;
+        const int nmax = max(ctx[kCtxNk], ctx[kCtxNk + 1]), jm = ctx[kCtxJm], lk = ctx[kCtxLk];
+        uint32_t* poison = poisons + c * 4 * kPfMasked;
+        bool ok = true;
+        for (int j = jm; j < nmax && ok; ++j) {
+          const int v = c * kPfMasked + j - jm;
+          ok = all_wait(&v_full[v], (v_phase >> v) & 1);
+          v_phase ^= 1u << v;
+          if (!ok) break;
+          uint8_t* tile = smem + C::kOffKv + ((at_item + 2 * j + 1) % C::kSlots) * C::kTileBytes;
+          const int keys = min(kPfRows, lk - j * kPfRows);
+          // 16-byte pieces, 8 to a 128-byte row, eight of them at a time: one
+          // by one this took longer than a tile's MMAs and softmax
+          constexpr int kBatch = 8;
+          uint4* at = reinterpret_cast<uint4*>(tile) + (threadIdx.x - 320);
 #pragma unroll 1
-        for (int c0 = 0; c0 < C::kTileBytes / 16; c0 += 64 * kBatch, at += 64 * kBatch) {
-          uint4 w[kBatch];
-          uint32_t bad = 0;
+          for (int c0 = 0; c0 < C::kTileBytes / 16; c0 += 64 * kBatch, at += 64 * kBatch) {
+            uint4 w[kBatch];
+            uint32_t bad = 0;
 #pragma unroll
-          for (int i = 0; i < kBatch; ++i) w[i] = at[i * 64];
-          auto key_of = [&](int i) { return ((c0 + i * 64 + (int)threadIdx.x - 320) >> 3) % kPfRows; };
+            for (int i = 0; i < kBatch; ++i) w[i] = at[i * 64];
+            auto key_of = [&](int i) { return ((c0 + i * 64 + (int)threadIdx.x - 320) >> 3) % kPfRows; };
 #pragma unroll
-          for (int i = 0; i < kBatch; ++i) {
-            const uint32_t b = not_finite<T>(w[i].x) | not_finite<T>(w[i].y) | not_finite<T>(w[i].z) | not_finite<T>(w[i].w);
-            if (key_of(i) < keys) bad |= b;
-            else at[i * 64] = make_uint4(0u, 0u, 0u, 0u);
-          }
-          if (bad) {
-#pragma unroll 1
             for (int i = 0; i < kBatch; ++i) {
-              const int key = key_of(i);
-              uint4 v = at[i * 64];
-              if (key >= keys || !(not_finite<T>(v.x) | not_finite<T>(v.y) | not_finite<T>(v.z) | not_finite<T>(v.w))) continue;
-              atomicOr(&poison[(j - jm) * 4 + (key >> 5)], 1u << (key & 31));
-              uint32_t* x = &v.x;
+              const uint32_t b = not_finite<T>(w[i].x) | not_finite<T>(w[i].y) | not_finite<T>(w[i].z) | not_finite<T>(w[i].w);
+              if (key_of(i) < keys) bad |= b;
+              else at[i * 64] = make_uint4(0u, 0u, 0u, 0u);
+            }
+            if (bad) {
+#pragma unroll 1
+              for (int i = 0; i < kBatch; ++i) {
+                const int key = key_of(i);
+                uint4 x4 = at[i * 64];
+                if (key >= keys || !(not_finite<T>(x4.x) | not_finite<T>(x4.y) | not_finite<T>(x4.z) | not_finite<T>(x4.w)))
+                  continue;
+                atomicOr(&poison[(j - jm) * 4 + (key >> 5)], 1u << (key & 31));
+                uint32_t* x = &x4.x;
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const uint32_t b = not_finite<T>(x[k]);
-                if (b & 0x8000u) x[k] &= 0xffff0000u;
-                if (b & 0x80000000u) x[k] &= 0x0000ffffu;
+                for (int k = 0; k < 4; ++k) {
+                  const uint32_t b = not_finite<T>(x[k]);
+                  if (b & 0x8000u) x[k] &= 0xffff0000u;
+                  if (b & 0x80000000u) x[k] &= 0x0000ffffu;
+                }
+                at[i * 64] = x4;
               }
-              at[i * 64] = v;
             }
           }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&v_ok[v]);
         }
-        fence_proxy_async_smem();
+        if (!ok) break;
+        at_item += 2 * nmax;
         __syncwarp();
-        if (lane == 0) mbar_arrive(&v_ok[j - jm]);
+        if (lane == 0) mbar_arrive(&ctx_empty[c]);
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
     const int s = warp >> 2, quarter = warp & 3;
     const uint32_t t_s = tmem + s * kPfRows + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t t_o = tmem + C::kTmemO + s * 128 + ((uint32_t)(quarter * 32) << 16);
-    const int n = ctx[kCtxNk + s];
-    // keys this row sees, and the tile's first row
-    const int seen_by_all = ctx[kCtxR0] + s * kPfRows + ctx[kCtxOff] + 1;
-    const int see = min(ctx[kCtxLk], seen_by_all + quarter * 32 + lane);
-    float m = -INFINITY, sum = 0.f;                              // reference maximum of the raw scores, sum of terms
-    const float scale = p.scale_log2;
-    bool fail = false;
-    for (int j = 0; j < n; ++j) {
-      if (!__all_sync(0xffffffffu, mbar_wait(&s_full[s], j & 1))) {
-        fail = true;
-        break;
-      }
-      tc_fence_after();
-      uint32_t x[4][32];
-      const int here = see - j * kPfRows;
-      const bool masked = (j + 1) * kPfRows > seen_by_all;
-      float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, x[c]);
-      tmem_wait_ld();
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        if (masked) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) x[c][i] = c * 32 + i < here ? x[c][i] : 0xff800000u;
+    static_assert(kPfRows == 128);
+    const uint32_t t_o = t_s + C::kTmemO;
+    uint32_t phases = 0;                                         // bit 0: s_full, bit 1: o_full
+    for (int item = 0;; ++item) {
+      volatile int* ctx = ctxs + (item & 1) * kCtxWords;
+      if (!all_wait(&ctx_full[item & 1], (item >> 1) & 1) || ctx[kCtxStop]) break;
+      // keys that the tile's first row sees, and this row
+      const int seen_by_all = ctx[kCtxR0] + ctx[kCtxOff] + s * kPfRows + 1;
+      const int see = min(ctx[kCtxLk], seen_by_all + quarter * 32 + lane), n = ctx[kCtxNk + s];
+      float m = -INFINITY, sum = 0.f;                            // reference maximum of the raw scores, sum of terms
+      const float scale = p.scale_log2;
+      bool fail = false;
+      for (int j = 0; j < n; ++j) {
+        if (!all_wait(&s_full[s], phases & 1)) {
+          fail = true;
+          break;
         }
+        phases ^= 1;
+        tc_fence_after();
+        uint32_t x[4][32];
+        const bool masked = (j + 1) * kPfRows > seen_by_all;
+        const int here = see - j * kPfRows;
+        float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < 32; i += 8)
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            top4[k] = fmaxf(fmaxf(top4[k], __uint_as_float(x[c][i + 2 * k])), __uint_as_float(x[c][i + 2 * k + 1]));
-      }
-      const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
-      // a new reference maximum where the terms would pass 2^8
-      const bool grow = top > m && (m == -INFINITY || (top - m) * scale > 8.f);
-      if (__any_sync(0xffffffffu, grow)) {
-        const float a = grow ? (m == -INFINITY ? 0.f : ex2((m - top) * scale)) : 1.f;
-        if (grow) {
-          m = top;
-          sum *= a;
-        }
-        if (j > 0) {
-#pragma unroll 1
-          for (int c = 0; c < D / 16; ++c) {
-            uint32_t o[16];
-            tmem_ld16(t_o + c * 16, o);
-            tmem_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
-            tmem_st16(t_o + c * 16, o);
-          }
-        }
-      }
-      const float neg = m == -INFINITY ? 0.f : Type16<T>::kShift - m * scale;
-      const float2 scale2 = make_float2(scale, scale), neg2 = make_float2(neg, neg);
-      float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-      // the first half of the keys goes to the tensor core while the second
-      // half's exponentials are computed
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t w[32];
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float2 v = __ffma2_rn(
-                make_float2(__uint_as_float(x[half * 2 + c][i]), __uint_as_float(x[half * 2 + c][i + 1])), scale2, neg2);
-            const float2 e = make_float2(ex2(v.x), ex2(v.y));
-            part[(i >> 1) & 1] = __fadd2_rn(part[(i >> 1) & 1], e);
-            w[c * 16 + (i >> 1)] = pack16<T>(e.x, e.y);
-          }
-        tmem_st32(t_s + half * 32, w);
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_ready[2 * s + half]);
-      }
-      sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
-    }
-    const int e_q0 = ctx[kCtxQ0], e_lq = ctx[kCtxLq], e_h = ctx[kCtxH], e_k0 = ctx[kCtxK0], e_jm = ctx[kCtxJm];
-    const int first = ctx[kCtxR0] + s * kPfRows + quarter * 32, row = first + lane;   // within the sequence
-    const bool live = row < e_lq;
-    const int64_t at = ((int64_t)(blockIdx.x % p.splits) * p.rows + e_q0 + row) * p.heads + e_h;   // splits: partial row
-    T* dst = static_cast<T*>(p.out) + ((int64_t)(e_q0 + row) * p.heads + e_h) * D;
-    if (n && !fail && __all_sync(0xffffffffu, mbar_wait(&o_full[s], 0))) {
-      tc_fence_after();
-      // The rows go through shared memory (the tile's queries have been
-      // used), so that a store instruction writes whole rows: one row per lane
-      // is one line per lane, and the stores took 2 us per CTA.
-      constexpr int kPieces = D / 8;
-      uint4* stage = reinterpret_cast<uint4*>(smem + s * C::kTileBytes) + quarter * 32 * kPieces;
-      // a split leaves its sums as they are, to be joined
-      const bool whole = p.splits == 1;
-      const float inv = !whole ? 1.f : see > 0 ? 1.f / sum : 0.f;
-      if (!whole && live) p.part_ml[at] = make_float2(sum == 0.f ? -INFINITY : m * scale, sum);
-      uint32_t any = 0;
-#pragma unroll
-      for (int i = 0; i < 4 * kPfMasked; ++i) any |= poison[i];
-#pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
-        tmem_ld32(t_o + c * 32, o);
+        for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, x[c]);
         tmem_wait_ld();
-        float f[32];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) f[i] = see > 0 ? __uint_as_float(o[i]) * inv : 0.f;
-        if (any) {
-          for (int i = 0; i < 4 * kPfMasked; ++i) {
-            uint32_t bits = poison[i];
-            while (bits) {
-              const int key = e_jm * kPfRows + i * 32 + __ffs(bits) - 1;
-              bits &= bits - 1;
-              if (key >= see) continue;
-              const T* vr = static_cast<const T*>(p.v) + (int64_t)(e_k0 + key) * p.sv_t + (int64_t)(e_h / p.group) * p.sv_h + c * 32;
+        for (int c = 0; c < 4; ++c) {
+          if (masked) {
 #pragma unroll
-              for (int d = 0; d < 32; ++d) {
-                const float v = to_f32(vr[d]);
-                if (!isfinite(v)) f[d] += v;
-              }
+            for (int i = 0; i < 32; ++i) x[c][i] = c * 32 + i < here ? x[c][i] : 0xff800000u;
+          }
+#pragma unroll
+          for (int i = 0; i < 32; i += 8)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              top4[k] = fmaxf(fmaxf(top4[k], __uint_as_float(x[c][i + 2 * k])), __uint_as_float(x[c][i + 2 * k + 1]));
+        }
+        const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
+        // a new reference maximum where the terms would pass 2^8
+        const bool grow = top > m && (m == -INFINITY || (top - m) * scale > 8.f);
+        if (__any_sync(0xffffffffu, grow)) {
+          const float a = grow ? (m == -INFINITY ? 0.f : ex2((m - top) * scale)) : 1.f;
+          if (grow) {
+            m = top;
+            sum *= a;
+          }
+          if (j > 0) {
+#pragma unroll 1
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t o[16];
+              tmem_ld16(t_o + c * 16, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
+              tmem_st16(t_o + c * 16, o);
             }
           }
         }
-        if (live && !whole) {
-          float* po = p.part_o + at * D + c * 32;
+        const float neg = m == -INFINITY ? 0.f : Type16<T>::kShift - m * scale;
+        const float2 scale2 = make_float2(scale, scale), neg2 = make_float2(neg, neg);
+        float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        // the first half of the keys goes to the tensor core while the second
+        // half's exponentials are computed
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(po + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
-        } else if (whole) {
+        for (int half = 0; half < 2; ++half) {
+          uint32_t w[32];
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            stage[lane * kPieces + ((c * 4 + i) ^ (lane & 7))] =
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const float2 v = __ffma2_rn(
+                  make_float2(__uint_as_float(x[half * 2 + c][i]), __uint_as_float(x[half * 2 + c][i + 1])), scale2, neg2);
+              const float2 e = make_float2(ex2(v.x), ex2(v.y));
+              part[(i >> 1) & 1] = __fadd2_rn(part[(i >> 1) & 1], e);
+              w[c * 16 + (i >> 1)] = pack16<T>(e.x, e.y);
+            }
+          tmem_st32(t_s + half * 32, w);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_ready[2 * s + half]);
+        }
+        sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
+      }
+      if (fail || (n && !all_wait(&o_full[s], phases >> 1))) break;
+      if (n) phases ^= 2;
+      tc_fence_after();
+      const int e_q0 = ctx[kCtxQ0], e_lq = ctx[kCtxLq], e_h = ctx[kCtxH], e_k0 = ctx[kCtxK0], e_jm = ctx[kCtxJm];
+      const int first = ctx[kCtxR0] + s * kPfRows + quarter * 32, row = first + lane;   // within the sequence
+      const bool live = row < e_lq;
+      const int64_t at = ((int64_t)ctx[kCtxSplit] * p.rows + e_q0 + row) * p.heads + e_h;   // splits: partial row
+      // a split leaves its sums as they are, to be joined
+      const bool whole = p.splits == 1;
+      if (!whole && live) p.part_ml[at] = make_float2(sum == 0.f ? -INFINITY : m * scale, sum);
+      if (n || whole) {
+        // The rows go through shared memory, 64 columns at a time, so that a
+        // store instruction writes whole lines: with one row per lane it
+        // touches 32 of them, and the stores took 2 us per item.
+        uint4* stage = reinterpret_cast<uint4*>(smem + C::kOffStage) + warp * 32 * 8;
+        const float inv = !whole ? 1.f : see > 0 && n ? 1.f / sum : 0.f;
+        const uint32_t* poison = poisons + (item & 1) * 4 * kPfMasked;
+        uint32_t any = 0;
+#pragma unroll
+        for (int i = 0; i < 4 * kPfMasked; ++i) any |= poison[i];
+#pragma unroll 1
+        for (int c = 0; c < D; c += 64) {
+          uint32_t o[2][32];
+          tmem_ld32(t_o + c, o[0]);
+          tmem_ld32(t_o + c + 32, o[1]);
+          tmem_wait_ld();
+          float f[64];
+          // a row that sees nothing gives zeros, whatever the accumulator holds
+#pragma unroll
+          for (int i = 0; i < 64; ++i) f[i] = see > 0 && n ? __uint_as_float(o[i / 32][i % 32]) * inv : 0.f;
+          if (any && n) {
+            for (int i = 0; i < 4 * kPfMasked; ++i) {
+              uint32_t bits = poison[i];
+              while (bits) {
+                const int key = e_jm * kPfRows + i * 32 + __ffs(bits) - 1;
+                bits &= bits - 1;
+                if (key >= see) continue;
+                const T* vr = static_cast<const T*>(p.v) + (int64_t)(e_k0 + key) * p.sv_t + (int64_t)p.by_group(e_h) * p.sv_h + c;
+#pragma unroll
+                for (int d = 0; d < 64; ++d) {
+                  const float v = to_f32(vr[d]);
+                  if (!isfinite(v)) f[d] += v;
+                }
+              }
+            }
+          }
+          if (!whole) {
+            if (live) {
+              float* po = p.part_o + at * D + c;
+#pragma unroll
+              for (int i = 0; i < 64; i += 4) *reinterpret_cast<float4*>(po + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+            }
+            continue;
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            stage[lane * 8 + (i ^ (lane & 7))] =
                 make_uint4(pack16<T>(f[8 * i], f[8 * i + 1]), pack16<T>(f[8 * i + 2], f[8 * i + 3]),
                            pack16<T>(f[8 * i + 4], f[8 * i + 5]), pack16<T>(f[8 * i + 6], f[8 * i + 7]));
-        }
-      }
-      if (whole) {
-        __syncwarp();
-        const int rows = min(32, e_lq - first);
+          __syncwarp();
+          const int rows = min(32, e_lq - first);
+          T* to = static_cast<T*>(p.out) + ((int64_t)(e_q0 + first) * p.heads + e_h) * D + c;
 #pragma unroll 4
-        for (int i = lane; i < rows * kPieces; i += 32) {
-          const int r = i / kPieces, c = i - r * kPieces;
-          *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + ((int64_t)(e_q0 + first + r) * p.heads + e_h) * D + c * 8) =
-              stage[r * kPieces + (c ^ (r & 7))];
+          for (int i = lane; i < rows * 8; i += 32)
+            *reinterpret_cast<uint4*>(to + (int64_t)(i >> 3) * p.heads * D + (i & 7) * 8) = stage[(i & ~7) + ((i ^ (i >> 3)) & 7)];
+          __syncwarp();
         }
       }
-    } else if (!n && live && p.splits > 1) {                     // this tile's rows see nothing here
-      p.part_ml[at] = make_float2(-INFINITY, 0.f);
-    } else if (!n && live) {
-#pragma unroll 1
-      for (int d = 0; d < D; d += 8) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0u, 0u, 0u, 0u);
+      // this warp's reads of the output come before the next item's MMAs
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctx_empty[item & 1]);
     }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512));
+  if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*(volatile uint32_t*)tmem_slot), "n"(512));
 }
 
 // Joins the splits' partial results: one thread per four columns.
@@ -732,7 +883,7 @@ static cudaError_t launch_prefill(const CUtensorMap* maps, const PrefillParams& 
 // items do not fill the SMs and the sequences are long, sharing the keys out
 // shortens the call; the number of items is estimated as one per 256 rows and
 // half a one more per sequence.  Two calls at 16 heads of 64: 901 queries
-// behind 6596 keys 66 us unsplit, 39 us in two.
+// behind 6596 keys 58 us unsplit, 37 us in two.
 static int prefill_splits(int B, int64_t rows, int64_t k_rows, int heads) {
   const int64_t items = (rows / (2 * kPfRows) + (B + 1) / 2) * heads;
   const int64_t by_sms = items > 0 ? (sm_count() + sm_count() / 4) / items : 1;
@@ -760,6 +911,7 @@ cudaError_t launch_attn_prefill(const void* q, const void* k, const void* v, int
   const int splits = workspace ? prefill_splits(B, rows, k_rows, heads) : 1;
   float* po = static_cast<float*>(workspace);
   const PrefillParams p{cu_q, cu_k, B, heads, heads / kv_heads, (int)rows, (int)k_rows, scale_log2, out, v, s[4], s[5],
+                        Divisor(heads), Divisor(heads / kv_heads), Divisor(splits), sm_count(),
                         splits, po, reinterpret_cast<float2*>(po + (size_t)splits * rows * heads * dim)};
   // at most one item more than whole ones per sequence (and for the rows behind the last)
   int64_t slots = rows / (2 * kPfRows) + B + 1;

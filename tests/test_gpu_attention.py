@@ -105,6 +105,36 @@ def test_prefill_many_sequences_in_order_of_place():
         a += n
 
 
+@pytest.mark.parametrize("dtype,dim,heads,kv_heads,nseq", [(BF16, 128, 28, 4, 40), (F16, 64, 20, 5, 21), (BF16, 64, 9, 3, 70)])
+def test_prefill_many_items_per_block(dtype, dim, heads, kv_heads, nseq):
+    # several items behind one another in a block, rows that see nothing,
+    # values that are not finite in some: every sequence as it comes out alone
+    import alpamayo_b200.ops as ops
+    q_lens = [(i * 101) % 700 if i % 7 else i % 3 for i in range(nseq)]
+    k_lens = [max(0, n + (i * 59) % 300 - 90) for i, n in enumerate(q_lens)]
+    q, k, v = packed(q_lens, k_lens, heads, kv_heads, dim, dtype, 43)
+    cq, ck = [0], [0]
+    for n, m in zip(q_lens, k_lens):
+        cq.append(cq[-1] + n)
+        ck.append(ck[-1] + m)
+    for i in range(0, nseq, 4):
+        if k_lens[i] > 8:
+            v[ck[i + 1] - 1 - i % 8, i % kv_heads, i % dim] = float("nan") if i % 8 else float("inf")
+    q, k, v = q.cuda(), k.cuda(), v.cuda()
+    out = ops.attention_prefill(q, k, v, R.cu(q_lens), R.cu(k_lens))
+    for i, (n, m) in enumerate(zip(q_lens, k_lens)):
+        if n == 0:
+            continue
+        a, b = slice(cq[i], cq[i + 1]), slice(ck[i], ck[i + 1])
+        alone = ops.attention_prefill(q[a], k[b], v[b], R.cu([n]), R.cu([m]))
+        assert torch.equal(torch.nan_to_num(out[a], 7.0, 8.0, 9.0), torch.nan_to_num(alone, 7.0, 8.0, 9.0)), i
+        row = n - 1
+        if m and torch.isfinite(v[b]).all():
+            ref, _, size, sb = R.attend(q[a][row:].double().cpu(), k[b].double().cpu(), v[b].double().cpu(), dim ** -0.5)
+            bound = R.out_bound(ref, size, sb, dtype, R.UNIT[dtype]) + (2.0 ** -25 if dtype == F16 else 0.0)
+            assert R.max_excess(out[a][row:], ref, bound) <= 1.0, i
+
+
 def test_prefill_long_rows_and_large_scores():
     import alpamayo_b200.ops as ops
     lens = [1500]
