@@ -23,7 +23,7 @@
 //    warps store the last one's output.  28 heads, 8 prompts of 1 to 1500
 //    tokens (560 items of 1 to 12 tiles): 61 us with an item per CTA, 58 with
 //    the items shared out evenly beforehand, 53 like this; one prompt of 8192
-//    gains 1 %; one of 37, whose items have a CTA each either way, takes 7.9
+//    gains 1 %; one of 37, whose items have a CTA each either way, takes 8.4
 //    us for 7.5 (the hand-over of its description).
 //  * warp 9: MMAs, one thread: S = Q K^T (both K-major in shared memory) and
 //    O += P V (P in tensor memory, V with its columns contiguous, i.e.
@@ -74,9 +74,9 @@ struct PrefillParams {
   void* out;
   const void* v;                   // for the values that are not finite
   int64_t sv_t, sv_h;
-  Divisor by_heads, by_group, by_splits;
+  Divisor by_heads, by_group;
   int sms;
-  int splits;                      // CTAs that share the keys of one item; > 1: partial results
+  int splits;                      // parts that an item's keys may be cut into; > 1: partial results, joined
   float* part_o;                   // [splits][rows][heads][dim] sums of terms times values
   float2* part_ml;                 // [splits][rows][heads] (reference maximum, sum of terms), in log2 units
 };
@@ -94,7 +94,7 @@ struct PrefillTile {
 };
 
 // An item as the loader hands it to the other warps.
-enum { kCtxStop, kCtxQ0, kCtxLq, kCtxR0, kCtxH, kCtxOff, kCtxLk, kCtxJm, kCtxK0, kCtxNk, kCtxSplit = kCtxNk + 2, kCtxWords };
+enum { kCtxStop, kCtxQ0, kCtxLq, kCtxR0, kCtxH, kCtxOff, kCtxLk, kCtxJm, kCtxK0, kCtxNk, kCtxSplit = kCtxNk + 2, kCtxParts, kCtxWords };
 
 namespace {
 
@@ -278,7 +278,7 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   // 256 x 176 + 128 x 152 = 384 x 168 registers.  The softmax warps need no
-  // more than 176; with 184 to 200 of them the same code took 1 to 3 % longer
+  // more than 176; with 184 to 200 of them the same code took up to 3 % longer
   // or the other warps' spilled.
   if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 152;");
   // Every warp meets here but the loader's, which needs nothing of the others
@@ -302,7 +302,44 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
         for (int b0 = 32; b0 <= p.B; b0 += 32) n += max(0, prefill_tiles(p, b0 + lane) - t);
         return __reduce_add_sync(0xffffffffu, n);
       };
-      const int total = left(0) * p.heads * p.splits;
+      const int items = left(0) * p.heads;
+      // Where keys may be shared out, an item of more than `part` key tiles is
+      // cut into parts.  A part is an SM's share of the work (an item costs
+      // about three tiles besides its own), four tiles at least, or up to half
+      // as much more if that leaves no more parts than SMs.
+      int part = 0x7FFFFFFF, parts = 1;
+      if (p.splits > 1) {
+        auto key_tiles = [&](int b) {
+          const int lo = min(max(p.cu_k[b], 0), p.k_rows);
+          return (min(max(p.cu_k[b + 1], lo), p.k_rows) - lo + kPfRows - 1) / kPfRows;
+        };
+        float work = 0.f;
+        int longest = 0;
+        for (int b = lane; b < p.B; b += 32) {
+          const int n = prefill_tiles(p, b), tiles = n ? key_tiles(b) : 0;
+          longest = max(longest, tiles);
+          // a place of a sequence sees two key tiles fewer than the next one
+          work += fmaxf((float)n * (float)(tiles - n + 1), (float)tiles) + 3.f * n;
+        }
+#pragma unroll
+        for (int i = 16; i; i >>= 1) work += __shfl_xor_sync(0xffffffffu, work, i);
+        longest = __reduce_max_sync(0xffffffffu, longest);
+        const int share = max(max(4, (longest + p.splits - 1) / p.splits),
+                              (int)fminf(ceilf(work * (float)p.heads / (float)p.sms), (float)longest));
+        part = share;
+#pragma unroll 1
+        for (int i = 0; i <= 4 && items <= p.sms; ++i) {
+          part = share + share * i / 8;
+          int n = 0;
+          for (int b = lane; b < p.B; b += 32) {
+            const int tiles = key_tiles(b);
+            for (int k = prefill_tiles(p, b) - 1, t = tiles; k >= 0; --k, t -= 2) n += max(1, (t + part - 1) / part);
+          }
+          if (__reduce_add_sync(0xffffffffu, n) * p.heads <= p.sms) break;
+        }
+        parts = max(1, (longest + part - 1) / part);
+      }
+      const int total = items * parts;
       auto load = [&](const CUtensorMap* map, uint8_t* dst, int head, int row, uint64_t* bar) {
         mbar_arrive_expect_tx(bar, C::kTileBytes);
 #pragma unroll
@@ -312,14 +349,21 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
       uint32_t q_phase[2] = {1u, 1u}, v_phase = 0, asked = 0;
       bool ok = true, open = false;              // open: a request has no answer yet
       int it = blockIdx.x;
-      for (int n = 0; ok; ++n) {
+      bool first = true;
+      for (int n = 0; ok;) {
         const int c = n & 1;
         if (n >= 2 && !all_wait(&ctx_empty[c], ((n >> 1) - 1) & 1)) break;
         // Items in order of their place in their sequence, the last places of
         // all sequences first (they see the most keys).  A CTA takes over the
         // items of CTAs that have not started, one while it works on the last.
-        if (n > 0) it = -1;
-        while (n > 0 && total > p.sms) {                // otherwise every item has a CTA of its own
+        // (With no more items than SMs each has a CTA already; a CTA without
+        // one clears away the others without one, which is quicker than
+        // starting them.)
+        // Parts beyond the launch's CTAs go to them in turn.
+        const bool turn = !first && it + (int)gridDim.x < total;
+        const bool claim = !turn && (first ? it >= total : total > p.sms);
+        it = turn ? it + (int)gridDim.x : first && !claim ? it : -1;
+        while (claim) {
           if (lane == 0) {
             mbar_arrive_expect_tx(next_full, 16);
             asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
@@ -349,6 +393,7 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
             break;
           }
         }
+        first = false;
         volatile int* ctx = ctxs + c * kCtxWords;
         if (it < 0 || it >= total) {
           if (lane == 0) {
@@ -357,7 +402,8 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
           }
           break;
         }
-        const int item = p.by_splits(it), split = it - item * p.splits;
+        int item = it, split = 0;
+        for (; item >= items; item -= items) ++split;
         int place = 0, hi = p.rows / (2 * kPfRows) + 1, above = 0, b = -1;
         while (hi - place > 1) {                           // the largest place with left(place) * heads > item
           const int mid = (place + hi) >> 1, n_mid = left(mid) * p.heads;
@@ -398,9 +444,13 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
           const int begin = r0 + s * kPfRows, end = min(lq, begin + kPfRows);
           nk[s] = begin < lq && end + off > 0 ? (end + off + kPfRows - 1) / kPfRows : 0;
         }
-        // this split's key tiles are j0 .. : from here on keys are counted from there
-        if (p.splits > 1) {
-          const int all = max(nk[0], nk[1]), share = p.by_splits(all + p.splits - 1), j0 = min(all, split * share);
+        // this part's key tiles are j0 .. : from here on keys are counted from there
+        int cut = 1;
+        if (parts > 1) {
+          const int all = max(nk[0], nk[1]);
+          cut = max(1, (all + part - 1) / part);
+          if (split >= cut) continue;                      // the item has fewer parts
+          const int share = (all + cut - 1) / cut, j0 = min(all, split * share);
 #pragma unroll
           for (int s = 0; s < 2; ++s) nk[s] = max(0, min(nk[s], j0 + share) - j0);
           k0 += j0 * kPfRows;
@@ -424,6 +474,7 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
           ctx[kCtxNk] = nk[0];
           ctx[kCtxNk + 1] = nk[1];
           ctx[kCtxSplit] = split;
+          ctx[kCtxParts] = cut;
           mbar_arrive(&ctx_full[c]);
           // position 2 j of the item is K_j, 2 j + 1 is V_j; the queries come behind K_0
 #pragma unroll 1
@@ -453,6 +504,7 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
           }
         }
         ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+        ++n;
       }
       // No copy is left in flight, whatever became of its readers: everything
       // that was issued has landed when each barrier's last phase is over.
@@ -732,9 +784,15 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
       const int first = ctx[kCtxR0] + s * kPfRows + quarter * 32, row = first + lane;   // within the sequence
       const bool live = row < e_lq;
       const int64_t at = ((int64_t)ctx[kCtxSplit] * p.rows + e_q0 + row) * p.heads + e_h;   // splits: partial row
-      // a split leaves its sums as they are, to be joined
-      const bool whole = p.splits == 1;
-      if (!whole && live) p.part_ml[at] = make_float2(sum == 0.f ? -INFINITY : m * scale, sum);
+      // one of several parts leaves its sums as they are, to be joined; an
+      // item of one part says that there is nothing to join
+      const bool whole = ctx[kCtxParts] == 1;
+      if (p.splits > 1 && live) {
+        p.part_ml[at] = whole ? make_float2(INFINITY, 0.f) : make_float2(sum == 0.f ? -INFINITY : m * scale, sum);
+        if (!whole && ctx[kCtxSplit] == 0)
+          for (int i = ctx[kCtxParts]; i < p.splits; ++i)
+            p.part_ml[at + (int64_t)i * p.rows * p.heads] = make_float2(-INFINITY, 0.f);
+      }
       if (n || whole) {
         // The rows go through shared memory, 64 columns at a time, so that a
         // store instruction writes whole lines: with one row per lane it
@@ -805,7 +863,7 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
   if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*(volatile uint32_t*)tmem_slot), "n"(512));
 }
 
-// Joins the splits' partial results: one thread per four columns.
+// Joins the parts of the items that have several: one thread per four columns.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) attn_prefill_join_kernel(const __grid_constant__ PrefillParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -813,9 +871,11 @@ __global__ void __launch_bounds__(256) attn_prefill_join_kernel(const __grid_con
   if (at >= n) return;
   const int d = (int)(e - at * (D / 4)) * 4;
   float2 ml[kPfSplits];
-  float mx = -INFINITY;
+  ml[0] = p.part_ml[at];
+  if (ml[0].x == INFINITY) return;                         // one part, already in place
+  float mx = ml[0].x;
 #pragma unroll
-  for (int i = 0; i < kPfSplits; ++i) {
+  for (int i = 1; i < kPfSplits; ++i) {
     ml[i] = i < p.splits ? p.part_ml[i * n + at] : make_float2(-INFINITY, 0.f);
     mx = fmaxf(mx, ml[i].x);
   }
@@ -863,8 +923,11 @@ static cudaError_t launch_prefill(const CUtensorMap* maps, const PrefillParams& 
   using C = PrefillTile<D>;
   cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(attn_prefill_kernel<T, D>), C::kSmem);
   if (e != cudaSuccess) return e;
-  attn_prefill_kernel<T, D><<<(unsigned)(slots * p.heads * p.splits), kPfThreads, C::kSmem, st>>>(maps[0], maps[1],
-                                                                                                  maps[2], p);
+  // Parts of items: nearly all of them make no more than a CTA per SM on top
+  // of the items; CTAs that find nothing to do cost time.
+  const int64_t more = slots * p.heads * (p.splits - 1);
+  const int64_t ctas = slots * p.heads + (more < sm_count() ? more : sm_count());
+  attn_prefill_kernel<T, D><<<(unsigned)ctas, kPfThreads, C::kSmem, st>>>(maps[0], maps[1], maps[2], p);
   if ((e = cudaGetLastError()) != cudaSuccess || p.splits == 1) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(((int64_t)p.rows * p.heads * (D / 4) + 255) / 256));
@@ -878,22 +941,34 @@ static cudaError_t launch_prefill(const CUtensorMap* maps, const PrefillParams& 
   return cudaLaunchKernelEx(&cfg, attn_prefill_join_kernel<T, D>, p);
 }
 
-// Into how many CTAs an item's keys are split.  An item (256 rows of one
-// head) takes as long as its keys whatever the number of rows, so where the
-// items do not fill the SMs and the sequences are long, sharing the keys out
-// shortens the call; the number of items is estimated as one per 256 rows and
-// half a one more per sequence.  Two calls at 16 heads of 64: 901 queries
-// behind 6596 keys 58 us unsplit, 37 us in two.
-static int prefill_splits(int B, int64_t rows, int64_t k_rows, int heads) {
-  const int64_t items = (rows / (2 * kPfRows) + (B + 1) / 2) * heads;
-  const int64_t by_sms = items > 0 ? (sm_count() + sm_count() / 4) / items : 1;
-  const int64_t by_keys = B > 0 ? k_rows / B / (4 * kPfRows) : 1;      // at least four key tiles each
-  const int64_t n = by_sms < by_keys ? by_sms : by_keys;
+// Into how many parts an item's keys may be cut (the device chooses, by the
+// lengths).  An item (256 rows of one head) takes as long as its keys whatever
+// the number of rows, so one long history among short ones, or few items on
+// many SMs, shorten when keys are shared out; the price is the second launch,
+// 2 to 3 us.  So only where an item may be of 8 key tiles or more, and
+//  * some sequences have keys before their queries, and the longest of them
+//    may be twice an SM's share of the work (key tiles, and three more per
+//    item; one item per 256 rows, half a one more per sequence), or
+//  * there are none, and the items leave half of the SMs without work.
+// 16 heads of 64, 901 queries behind 6596 keys: 58 us unsplit, 41 in two parts;
+// 2 heads of 128, 14 prompts of which one lies behind 5676 keys: 86 and 32 us;
+// 14 heads, 10 prompts of which one lies behind 1118 keys: 35 and 39 us.
+// Partial results take at most 256 MB.
+static int prefill_splits(int B, int64_t rows, int64_t k_rows, int heads, int dim) {
+  if (B < 1 || rows < 1) return 1;
+  const int64_t sms = sm_count(), before = k_rows - rows;
+  const int64_t longest = (before > 0 ? before + (rows + B - 1) / B : k_rows) / kPfRows;
+  if (longest < 8) return 1;
+  const double items = (double)(rows / (2 * kPfRows) + (B + 1) / 2) * heads;
+  const double work = (double)rows * rows / (4.0 * B * kPfRows * kPfRows) * heads + 3.0 * items;   // at least
+  if (before > 0 ? (double)longest * sms < 2 * work : 2 * items > sms) return 1;
+  const int64_t fit = (256LL << 20) / (rows * heads * (dim * 4 + 8));
+  const int64_t n = fit < longest / 4 ? fit : longest / 4;
   return n < 1 ? 1 : n > kPfSplits ? kPfSplits : (int)n;
 }
 
 size_t attn_prefill_workspace(int B, int64_t rows, int64_t k_rows, int heads, int dim) {
-  const int n = prefill_splits(B, rows, k_rows, heads);
+  const int n = prefill_splits(B, rows, k_rows, heads, dim);
   return n == 1 ? 0 : (size_t)n * rows * heads * (dim * 4 + 8);
 }
 
@@ -908,15 +983,15 @@ cudaError_t launch_attn_prefill(const void* q, const void* k, const void* v, int
     return cudaErrorInvalidValue;
   // a scale of zero still has to leave -infinity where a key is not seen
   const float scale_log2 = fmaxf(scale * 1.4426950408889634f, 1e-37f);
-  const int splits = workspace ? prefill_splits(B, rows, k_rows, heads) : 1;
+  const int splits = workspace ? prefill_splits(B, rows, k_rows, heads, dim) : 1;
   float* po = static_cast<float*>(workspace);
   const PrefillParams p{cu_q, cu_k, B, heads, heads / kv_heads, (int)rows, (int)k_rows, scale_log2, out, v, s[4], s[5],
-                        Divisor(heads), Divisor(heads / kv_heads), Divisor(splits), sm_count(),
+                        Divisor(heads), Divisor(heads / kv_heads), sm_count(),
                         splits, po, reinterpret_cast<float2*>(po + (size_t)splits * rows * heads * dim)};
   // at most one item more than whole ones per sequence (and for the rows behind the last)
   int64_t slots = rows / (2 * kPfRows) + B + 1;
   if (slots > rows) slots = rows;
-  if (slots * heads * splits > 0x7FFFFFFF || rows * heads * (dim / 4) / 256 >= 0x7FFFFFFF) return cudaErrorInvalidValue;
+  if (slots * heads * splits > 0x3FFFFFFF || rows * heads * (dim / 4) / 256 >= 0x7FFFFFFF) return cudaErrorInvalidValue;
   if (dtype == PARO_BF16)
     return dim == 128 ? launch_prefill<__nv_bfloat16, 128>(maps, p, slots, st)
                       : launch_prefill<__nv_bfloat16, 64>(maps, p, slots, st);

@@ -91,6 +91,27 @@ def test_prefill_keys_shared_out(q_lens, k_lens, dim, dtype):
     assert torch.equal(got[-1][:, rest], out[-1][:, rest])
 
 
+@pytest.mark.parametrize("dtype,dim,heads,kv_heads", [(BF16, 128, 12, 4), (F16, 64, 2, 2), (BF16, 64, 28, 4)])
+def test_prefill_one_long_history_among_short_ones(dtype, dim, heads, kv_heads):
+    # keys shared out for one sequence only, in more parts than blocks
+    import alpamayo_b200.ops as ops
+    q_lens, k_lens = [164, 69, 357, 0, 165, 64, 5, 178, 56], [5408, 110, 726, 0, 165, 60, 2, 178, 1134]
+    q, k, v = packed(q_lens, k_lens, heads, kv_heads, dim, dtype, 47)
+    out = ops.attention_prefill(q.cuda(), k.cuda(), v.cuda(), R.cu(q_lens), R.cu(k_lens))
+    assert torch.equal(out, ops.attention_prefill(q.cuda(), k.cuda(), v.cuda(), R.cu(q_lens), R.cu(k_lens)))
+    a = b = 0
+    for n, m in zip(q_lens, k_lens):
+        for i in sorted({0, n // 2, n - 1} - {-1}) if n else []:
+            see = max(0, i + 1 + m - n)
+            if not see:
+                assert (out[a + i] == 0).all()
+                continue
+            ref, _, size, sb = R.attend(q[a + i:a + i + 1].double(), k[b:b + see].double(), v[b:b + see].double(), dim ** -0.5)
+            bound = R.out_bound(ref, size, sb, dtype, R.UNIT[dtype]) + (2.0 ** -25 if dtype == F16 else 0.0)
+            assert R.max_excess(out[a + i:a + i + 1], ref, bound) <= 1.0, (n, m, i)
+        a, b = a + n, b + m
+
+
 def test_prefill_many_sequences_in_order_of_place():
     # over 32 sequences, of all numbers of tiles
     import alpamayo_b200.ops as ops
