@@ -52,6 +52,7 @@ constexpr int kPfRows = 128;       // query rows per tile, keys per tile
 constexpr int kPfThreads = 384;
 constexpr int kPfSplits = 8;       // splits of an item's keys, at most
 constexpr int kPfMasked = 3;       // key tiles that a CTA's rows see in part, at most
+constexpr float kInPlace = -1.f;
 
 // Division of 0 .. 2^31 - 1 by a divisor that the host knows: the rounded-up
 // reciprocal gives the quotient or one more.
@@ -78,7 +79,8 @@ struct PrefillParams {
   int sms;
   int splits;                      // parts that an item's keys may be cut into; > 1: partial results, joined
   float* part_o;                   // [splits][rows][heads][dim] sums of terms times values
-  float2* part_ml;                 // [splits][rows][heads] (reference maximum, sum of terms), in log2 units
+  float2* part_ml;                 // [splits][rows][heads] (reference maximum, sum of terms), in log2 units; a
+                                   // sum of kInPlace, which no sum of terms is: one part, the row is in `out`
 };
 
 template <int D>
@@ -788,7 +790,7 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
       // item of one part says that there is nothing to join
       const bool whole = ctx[kCtxParts] == 1;
       if (p.splits > 1 && live) {
-        p.part_ml[at] = whole ? make_float2(INFINITY, 0.f) : make_float2(sum == 0.f ? -INFINITY : m * scale, sum);
+        p.part_ml[at] = whole ? make_float2(0.f, kInPlace) : make_float2(sum == 0.f ? -INFINITY : m * scale, sum);
         if (!whole && ctx[kCtxSplit] == 0)
           for (int i = ctx[kCtxParts]; i < p.splits; ++i)
             p.part_ml[at + (int64_t)i * p.rows * p.heads] = make_float2(-INFINITY, 0.f);
@@ -872,7 +874,7 @@ __global__ void __launch_bounds__(256) attn_prefill_join_kernel(const __grid_con
   const int d = (int)(e - at * (D / 4)) * 4;
   float2 ml[kPfSplits];
   ml[0] = p.part_ml[at];
-  if (ml[0].x == INFINITY) return;                         // one part, already in place
+  if (ml[0].y == kInPlace) return;                         // one part, already in place
   float mx = ml[0].x;
 #pragma unroll
   for (int i = 1; i < kPfSplits; ++i) {

@@ -1,0 +1,85 @@
+"""Attention and cache operators where an input or a table is out of the
+ordinary: infinite scores, rows of no sequence, pages that are not there,
+values of extreme sizes."""
+import ctypes
+
+import pytest
+import torch
+
+import attn_ref as R
+
+pytestmark = pytest.mark.gpu
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+INF = float("inf")
+
+
+@pytest.fixture(autouse=True)
+def _clean_error_word(request):
+    import alpamayo_b200.ops as ops
+    ops.device_error_word()
+    yield
+    if "bad_" not in request.node.name:
+        assert ops.device_error_word() == 0
+
+
+def prefill_into_dirty_memory(q, k, v, cu_q, cu_k=None, scale=None):
+    """attention_prefill with an output that lies where the same number of
+    bytes held 123 before: a place that is not written shows."""
+    import alpamayo_b200.ops as ops
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    dirty = [torch.full(q.shape, 123.0, dtype=q.dtype, device="cuda") for _ in range(4)]
+    del dirty
+    return ops.attention_prefill(q, k, v, cu_q, cu_k, scale)
+
+
+def prefill_unsplit(q, k, v, cu_q, cu_k):
+    """The entry point without a workspace, whose rows are never shared out."""
+    from alpamayo_b200 import _native
+    out = torch.full_like(q, 123.0)
+    st = (ctypes.c_int64 * 6)(*(t.stride(d) for t in (q, k, v) for d in (0, 1)))
+    rc = _native.capi().paro_attention_prefill(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), 2 if q.dtype == BF16 else 1, st, cu_q.data_ptr(), cu_k.data_ptr(),
+        cu_q.numel() - 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2], q.shape[2] ** -0.5,
+        out.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    return out
+
+
+def shared_out(q_rows, k_rows, heads, kv_heads, dim, dtype, seed):
+    from alpamayo_b200 import _native
+    assert _native.capi().paro_attention_prefill_workspace_size(1, q_rows, k_rows, heads, dim) > 0
+    g = torch.Generator().manual_seed(seed)
+    q = (torch.randn(q_rows, heads, dim, generator=g) * 1.5).to(dtype)
+    q[:, :, 3] = torch.where(q[:, :, 3] == 0, torch.ones_like(q[:, :, 3]), q[:, :, 3])
+    return q, *(torch.randn(k_rows, kv_heads, dim, generator=g).to(dtype) for _ in range(2))
+
+
+@pytest.mark.parametrize("dtype,dim", [(BF16, 128), (F16, 64)])
+@pytest.mark.parametrize("at", [5, 2600, 4000])
+def test_prefill_infinite_key_in_keys_shared_out(at, dim, dtype):
+    # a score of +inf makes the row NaN whichever part it lies in; one of
+    # -inf takes the key out, i.e. the row is that of the other keys
+    n, m, heads = 64, 4096, 4
+    q, k, v = shared_out(n, m, heads, 2, dim, dtype, 70)
+    k[at, 0, 3] = INF
+    cq, ck = R.cu([n]), R.cu([m])
+    out = prefill_into_dirty_memory(q.cuda(), k.cuda(), v.cuda(), cq, ck)
+    want_nan = torch.zeros(n, heads, dtype=torch.bool)
+    want_nan[:, :2] = q[:, :2, 3] > 0
+    if at > m - n:                                        # the first rows do not see it
+        want_nan[:at - (m - n)] = False
+    assert torch.equal(torch.isnan(out).all(-1).cpu(), want_nan)
+    assert torch.equal(torch.isnan(out).any(-1).cpu(), want_nan)
+    assert torch.equal(torch.isnan(prefill_unsplit(q.cuda(), k.cuda(), v.cuda(), cq, ck)).any(-1).cpu(), want_nan)
+    for i in (0, n // 2, n - 1):
+        for h in range(heads):
+            if want_nan[i, h]:
+                continue
+            keep = torch.arange(i + 1 + m - n)
+            if h < 2:
+                keep = keep[keep != at]
+            ref, _, size, sb = R.attend(q[i:i + 1, h:h + 1].double(), k[keep, h // 2:h // 2 + 1].double(),
+                                        v[keep, h // 2:h // 2 + 1].double(), dim ** -0.5)
+            bound = R.out_bound(ref, size, sb, dtype, R.UNIT[dtype]) + (2.0 ** -25 if dtype == F16 else 0.0)
+            assert R.max_excess(out[i:i + 1, h:h + 1], ref, bound) <= 1.0, (i, h)
