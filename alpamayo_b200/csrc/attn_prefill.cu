@@ -96,7 +96,7 @@ struct PrefillTile {
 };
 
 // An item as the loader hands it to the other warps.
-enum { kCtxStop, kCtxQ0, kCtxLq, kCtxR0, kCtxH, kCtxOff, kCtxLk, kCtxJm, kCtxK0, kCtxNk, kCtxSplit = kCtxNk + 2, kCtxParts, kCtxWords };
+enum { kCtxStop, kCtxQ0, kCtxLq, kCtxR0, kCtxH, kCtxOff, kCtxLk, kCtxJm, kCtxK0, kCtxNk, kCtxSplit = kCtxNk + 2, kCtxParts, kCtxLead, kCtxWords };
 
 namespace {
 
@@ -171,9 +171,11 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 // 256-row items of sequence i (i = B: the rows behind the last sequence).
+// The rows before the first sequence are in front of its own in its items; they
+// give zeros.
 __device__ __forceinline__ int prefill_tiles(const PrefillParams& p, int i) {
   if (i > p.B) return 0;
-  const int lo = min(max(p.cu_q[i], 0), p.rows), hi = i < p.B ? min(max(p.cu_q[i + 1], lo), p.rows) : p.rows;
+  const int lo = i == 0 ? 0 : min(max(p.cu_q[i], 0), p.rows), hi = i < p.B ? min(max(p.cu_q[i + 1], lo), p.rows) : p.rows;
   return (hi - lo + 2 * kPfRows - 1) / (2 * kPfRows);
 }
 
@@ -434,11 +436,12 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
         const int ck0 = __shfl_sync(0xffffffffu, cu_k0, b & 31), ck1 = __shfl_sync(0xffffffffu, cu_k0, (b + 1) & 31);
         const int bq0 = kept ? cq0 : p.cu_q[b], bq1 = last ? p.rows : kept ? cq1 : p.cu_q[b + 1];
         const int bk0 = last ? 0 : kept ? ck0 : p.cu_k[b], bk1 = last ? 0 : kept ? ck1 : p.cu_k[b + 1];
-        const int q0 = min(max(bq0, 0), p.rows), lq = min(max(bq1, q0), p.rows) - q0;
+        const int qb = min(max(bq0, 0), p.rows), q0 = b == 0 ? 0 : qb, lq = min(max(bq1, qb), p.rows) - q0;
+        const int lead = qb - q0;                          // rows before the first sequence, in front of its own
         int k0 = min(max(bk0, 0), p.k_rows), lk = min(max(bk1, k0), p.k_rows) - k0;
-        if (lane == 0 && !last && (q0 != bq0 || lq != bq1 - q0 || k0 != bk0 || lk != bk1 - k0)) report_error(kErrBadPage);
+        if (lane == 0 && !last && (qb != bq0 || lq - lead != bq1 - qb || k0 != bk0 || lk != bk1 - k0)) report_error(kErrBadPage);
         const int r0 = place * 2 * kPfRows;
-        int off = lk - lq;                                 // row i sees keys j <= i + off
+        int off = lk - lq;                                 // row i sees keys j <= i + off (lead rows: none)
         // key tiles of each row tile (0: no rows, or none that sees a key)
         int nk[2];
 #pragma unroll
@@ -477,6 +480,7 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
           ctx[kCtxNk + 1] = nk[1];
           ctx[kCtxSplit] = split;
           ctx[kCtxParts] = cut;
+          ctx[kCtxLead] = lead;
           mbar_arrive(&ctx_full[c]);
           // position 2 j of the item is K_j, 2 j + 1 is V_j; the queries come behind K_0
 #pragma unroll 1
@@ -702,7 +706,8 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
       if (!all_wait(&ctx_full[item & 1], (item >> 1) & 1) || ctx[kCtxStop]) break;
       // keys that the tile's first row sees, and this row
       const int seen_by_all = ctx[kCtxR0] + ctx[kCtxOff] + s * kPfRows + 1;
-      const int see = min(ctx[kCtxLk], seen_by_all + quarter * 32 + lane), n = ctx[kCtxNk + s];
+      const bool lead = ctx[kCtxR0] + s * kPfRows + quarter * 32 + lane < ctx[kCtxLead];
+      const int see = lead ? 0 : min(ctx[kCtxLk], seen_by_all + quarter * 32 + lane), n = ctx[kCtxNk + s];
       float m = -INFINITY, sum = 0.f;                            // reference maximum of the raw scores, sum of terms
       const float scale = p.scale_log2;
       bool fail = false;
@@ -790,7 +795,7 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
       // item of one part says that there is nothing to join
       const bool whole = ctx[kCtxParts] == 1;
       if (p.splits > 1 && live) {
-        p.part_ml[at] = whole ? make_float2(0.f, kInPlace) : make_float2(sum == 0.f ? -INFINITY : m * scale, sum);
+        p.part_ml[at] = whole ? make_float2(0.f, kInPlace) : make_float2(sum == 0.f ? -INFINITY : m * scale, see > 0 ? sum : 0.f);
         if (!whole && ctx[kCtxSplit] == 0)
           for (int i = ctx[kCtxParts]; i < p.splits; ++i)
             p.part_ml[at + (int64_t)i * p.rows * p.heads] = make_float2(-INFINITY, 0.f);

@@ -518,7 +518,8 @@ typedef struct paro_kv8_cache {
  * Causal attention over packed sequences with grouped heads:
  *   o_i = sum_{j <= i + Lk - Lq} softmax_j(scale * q_i . k_j) v_j
  * for query i (of Lq) of each sequence over that sequence's Lk keys; a query
- * that sees no key gives zeros, and so do rows behind the last sequence.
+ * that sees no key gives zeros, and so do rows before the first sequence and
+ * behind the last.
  * What a query does not see has no effect on it, whatever it holds.
  *   q   : [rows][heads][head_dim] of dtype (F16 / BF16), strides in elements
  *   k, v: [k_rows][kv_heads][head_dim] of the same dtype

@@ -83,3 +83,26 @@ def test_prefill_infinite_key_in_keys_shared_out(at, dim, dtype):
                                         v[keep, h // 2:h // 2 + 1].double(), dim ** -0.5)
             bound = R.out_bound(ref, size, sb, dtype, R.UNIT[dtype]) + (2.0 ** -25 if dtype == F16 else 0.0)
             assert R.max_excess(out[i:i + 1, h:h + 1], ref, bound) <= 1.0, (i, h)
+
+
+@pytest.mark.parametrize("dtype,dim", [(BF16, 128), (F16, 64)])
+@pytest.mark.parametrize("first,q_lens,k_lens", [(7, [33, 40], None), (300, [20, 0, 290], None), (5, [50, 9], [70, 4]),
+                                                 (40, [60, 30], [3000, 30]), (260, [3], [2600])])
+def test_prefill_rows_before_the_first_sequence_are_zero(first, q_lens, k_lens, dim, dtype):
+    import alpamayo_b200.ops as ops
+    end = first + sum(q_lens)
+    rows, m = end + 11, sum(k_lens or q_lens)
+    k_first = 2 if k_lens else first
+    k_rows = m + k_first + 3 if k_lens else rows
+    g = torch.Generator().manual_seed(71)
+    q = torch.randn(rows, 4, dim, generator=g).to(dtype).cuda()
+    k, v = (torch.randn(k_rows, 2, dim, generator=g).to(dtype).cuda() for _ in range(2))
+    cq = R.cu(q_lens) + first
+    ck = R.cu(k_lens) + k_first if k_lens else None
+    out = prefill_into_dirty_memory(q, k, v, cq, ck)
+    assert (out[:first] == 0).all() and (out[end:] == 0).all()
+    want = ops.attention_prefill(q[first:end].contiguous(), k[k_first:k_first + m].contiguous(),
+                                 v[k_first:k_first + m].contiguous(), R.cu(q_lens), R.cu(k_lens) if k_lens else None)
+    # the rows before the first sequence move its tiles: the same sums in another order
+    diff = (out[first:end].double() - want.double()).abs()
+    assert float(diff.max()) <= 4 * R.UNIT[dtype] * float(v.abs().max())
