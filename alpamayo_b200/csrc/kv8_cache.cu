@@ -350,11 +350,13 @@ __global__ void __launch_bounds__(kGatherThreads) kv8_gather_kernel(GatherParams
   const int64_t r0 = (int64_t)blockIdx.x * kGatherRows;
   if (threadIdx.x < 32) {
     int64_t first;
-    int b = warp_find_seq(r0, p.B, [&](int i) -> int64_t { return max(0, p.cu[i + 1] - p.cu[i]); }, &first);
+    // the sequence of the first row here, or the first with rows behind it
+    const int64_t into = max((int64_t)0, r0 - (p.B > 0 ? p.cu[0] : 0));
+    int b = warp_find_seq(into, p.B, [&](int i) -> int64_t { return max(0, p.cu[i + 1] - p.cu[i]); }, &first);
     const int64_t row = r0 + threadIdx.x;
     int page = -1, at = 0;
     while (b >= 0 && b < p.B && row >= p.cu[b + 1]) ++b;
-    if (row < p.rows && b >= 0 && b < p.B) {               // rows behind the last sequence read as zeros
+    if (row < p.rows && b >= 0 && b < p.B && row >= p.cu[b]) {   // rows outside the sequences read as zeros
       const int64_t tok = (int64_t)p.starts[b] + (row - p.cu[b]), blk = tok >> c.page_shift;
       if (tok < 0 || blk >= c.table_width) report_error(kErrBadPage);
       else page = kv8_page(c, b, (int)blk);

@@ -567,7 +567,7 @@ int paro_kv8_append(const paro_kv8_cache* cache, const int32_t* page_table, int 
 /*
  * Reads token ranges back: output rows cu[b] .. cu[b + 1] - 1 are sequence
  * b's tokens starts[b], starts[b] + 1, ..., code * scale rounded to dtype.
- * Rows behind cu[B] are zeros.  out_k, out_v: [rows][kv_heads][head_dim].
+ * Rows before cu[0] and behind cu[B] are zeros.  out_k, out_v: [rows][kv_heads][head_dim].
  */
 int paro_kv8_gather(const paro_kv8_cache* cache, const int32_t* page_table, int table_width,
                     const int32_t* starts, const int32_t* cu, int B, int64_t rows, void* out_k,

@@ -106,3 +106,14 @@ def test_prefill_rows_before_the_first_sequence_are_zero(first, q_lens, k_lens, 
     # the rows before the first sequence move its tiles: the same sums in another order
     diff = (out[first:end].double() - want.double()).abs()
     assert float(diff.max()) <= 4 * R.UNIT[dtype] * float(v.abs().max())
+
+
+def test_gather_rows_outside_the_ranges_are_zero():
+    import alpamayo_b200.ops as ops
+    *cache, table = R.make_pool([100, 40, 0, 70], 16, 3, 64, 72)
+    starts, lens, first = [37, 0, 0, 5], [50, 40, 0, 60], 70
+    want_k, want_v = ops.kv8_gather(*cache, table, R.i32(starts), R.cu(lens), 150, F32)
+    k, v = ops.kv8_gather(*cache, table, R.i32(starts), R.cu(lens) + first, 230, F32)
+    for got, want in ((k, want_k), (v, want_v)):
+        assert (got[:first] == 0).all() and (got[220:] == 0).all()
+        assert torch.equal(got[first:220], want)
