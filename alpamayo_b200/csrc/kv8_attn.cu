@@ -85,6 +85,7 @@ __device__ __forceinline__ void cp_async8(uint32_t dst, const void* src) {
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
+__device__ __forceinline__ void st_shared(uint32_t dst, float x) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst), "f"(x) : "memory"); }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -166,7 +167,7 @@ struct DecodeTile {
   static constexpr int kTeams = kDecWarps / kWr;
   static constexpr int kWarpRows = RB / kWr;             // 8 or 16
   static constexpr int kSlots = D / 8;                   // 16-byte slots per lane and stage (K and V)
-  static constexpr int kStage = kSlots * 512 + 32;       // + the unit's four scales
+  static constexpr int kStage = kSlots * 512 + 32;       // + the unit's four scales and a term of the scores of either half
   static constexpr int kCtas = 3;                        // CTAs per SM
   static constexpr int kStages = kWr == 4 ? 4 : kWr == 2 ? 3 : D == 128 ? 2 : 4;
   // Teams of four: the expanded codes, shared by the team, as the 16-byte
@@ -257,9 +258,9 @@ __global__ void __launch_bounds__(kDecWarps * 32, (DecodeTile<D, RB>::kCtas)) kv
       for (int i = 0; i < 2; ++i) {
         if (n.id[i] < 0 || n.id[i] >= c.num_pages) {
           report_error(kErrBadPage);
-          n.id[i] = 0;
+          n.id[i] = -1;                     // page 0 is copied in its place, and nothing of it seen
         }
-        kb[i] = kv8_base(c, n.id[i], n.head) + (int64_t)((n.tok + 16 * i) & (page - 1)) * D;
+        kb[i] = kv8_base(c, max(0, n.id[i]), n.head) + (int64_t)((n.tok + 16 * i) & (page - 1)) * D;
       }
       const uint32_t at = smem_u32(ring + stage * C::kStage), dst = at + lane * 16;
       // the team's warps take the pieces in turn
@@ -294,9 +295,12 @@ __global__ void __launch_bounds__(kDecWarps * 32, (DecodeTile<D, RB>::kCtas)) kv
             else cp_async8(at + 4 * 512 + (kk * 4 + x) * 256 + lane * 8, c.v_codes + off);
           }
       }
-      if (lane < 4 && wr == 0) {
-        const float* sc = (lane < 2 ? c.k_scale : c.v_scale) + (int64_t)((lane & 1) ? n.id[1] : n.id[0]) * c.kv_heads + n.head;
-        cp_async4(at + C::kSlots * 512 + lane * 4, sc);
+      if (lane < 6 && wr == 0) {
+        const int id = (lane & 1) ? n.id[1] : n.id[0];
+        const float* sc = (lane < 2 ? c.k_scale : c.v_scale) + (int64_t)id * c.kv_heads + n.head;
+        // a half without a page: keys of zero, and minus infinity for its scores
+        if (lane < 4 && id >= 0) cp_async4(at + C::kSlots * 512 + lane * 4, sc);
+        else st_shared(at + C::kSlots * 512 + lane * 4, lane < 4 || id >= 0 ? 0.f : -INFINITY);
       }
     }
     cp_commit();
@@ -439,7 +443,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, (DecodeTile<D, RB>::kCtas)) kv
           fv[(slot + 1) * 32] = make_uint4(codes_f16x2(a_hi, 0x4140), codes_f16x2(c_hi, 0x4140),
                                            codes_f16x2(a_hi, 0x4342), codes_f16x2(c_hi, 0x4342));
         }
-        if (wr == 0 && lane < 4)
+        if (wr == 0 && lane < 6)
           reinterpret_cast<float*>(frags + buf * C::kFrag + 2 * (D / 8) * 512)[lane] =
               reinterpret_cast<const float*>(raw + C::kSlots * 512)[lane];
         __syncwarp();
@@ -488,7 +492,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, (DecodeTile<D, RB>::kCtas)) kv
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int e = max(-60, min(60, (int)((__float_as_uint(vs[i]) >> 23) & 0xff) - 127));
-        ve[i] = (float)e;
+        ve[i] = (float)e + sc[4 + i];                         // - infinity: left out
         vi[i] = __uint_as_float((uint32_t)(127 - e) << 23);   // 2^-e
         vf[i] = vs[i] * vi[i];
       }
@@ -786,7 +790,11 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const __grid_con
   // joined; a masked or padded score is loaded (inside its row) but never
   // used.
   const int quads = tokens / 4, rg = threadIdx.x / quads, tok = chunk * tokens + threadIdx.x % quads * 4;
-  const bool live = tok < len;
+  bool live = tok < len;
+  if (live) {                                 // a page (of four tokens at least) outside the pool: nothing is seen
+    const int id = c.table[(int64_t)b * c.table_width + (tok >> c.page_shift)];
+    live = id >= 0 && id < c.num_pages;
+  }
   const float* s = p.scores + (int64_t)bh * p.rows * p.score_cap + tok;
   const int64_t wat = (int64_t)bh * p.cap + tok;
   float4 v[kJoinRows];
@@ -838,7 +846,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const __grid_con
       const float x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (tok + e < see) mass[e] = fmaf(ex2(x[e] - row.x), row.y, mass[e]);
+        if (live && tok + e < see) mass[e] = fmaf(ex2(x[e] - row.x), row.y, mass[e]);
     }
   }
   if (p.row_groups > 1) {

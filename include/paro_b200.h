@@ -501,7 +501,8 @@ int paro_w4a8_gemm_noalloc(const int8_t* xq, const float* xscale, int64_t M, int
  * page_size 16, 32, 64 or 128; head_dim 64 or 128.  A page belongs to one
  * sequence while it is written.  A page-table entry outside the pool, or a
  * length beyond the table's row, sets bit 8 of the device error word, and
- * the tokens concerned are left out (nothing out of bounds is touched).
+ * the tokens concerned are left out (nothing out of bounds is touched):
+ * not written, read back as zeros, not attended to and given no weight.
  */
 typedef struct paro_kv8_cache {
   int8_t* k_codes;

@@ -117,3 +117,58 @@ def test_gather_rows_outside_the_ranges_are_zero():
     for got, want in ((k, want_k), (v, want_v)):
         assert (got[:first] == 0).all() and (got[220:] == 0).all()
         assert torch.equal(got[first:220], want)
+
+
+def attend_seen(q, k, v, see, scale):
+    """q [h, d], k / v [m, g, d] in 64 bits, see [m]: output, weights [h, m],
+    and the parts of R.out_bound, over the tokens of `see` alone."""
+    h, d, m = q.shape[0], q.shape[1], k.shape[0]
+    out, w = torch.zeros(1, h, d, dtype=torch.float64), torch.zeros(h, m, dtype=torch.float64)
+    size, sb = torch.zeros(1, h, d, dtype=torch.float64), torch.zeros(h, 1, dtype=torch.float64)
+    js = see.nonzero()[:, 0]
+    if len(js):
+        o, p, size, sb = R.attend(q[None], k[js], v[js], scale)
+        out, w[:, js] = o, p[:, 0]
+    return out, w, size, sb
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,T", [(2, 1, 64, 1), (14, 2, 128, 1), (12, 1, 64, 1), (6, 2, 128, 9), (16, 1, 64, 6)])
+@pytest.mark.parametrize("page", [16, 64])
+def test_kv8_attention_tokens_of_bad_pages_are_left_out(page, heads, kv_heads, dim, T):
+    # page 0 belongs to another sequence: nothing of it may show
+    import alpamayo_b200.ops as ops
+    lens = [5 * page - 3, 3 * page, 2 * page - 1, 4 * page]
+    *cache, table = R.make_pool(lens, page, kv_heads, dim, 73)
+    cache[2][0], cache[3][0] = 50.0, 50.0
+    bad = {0: [1, 4], 1: [0], 2: [0, 1], 3: []}
+    for b, blocks in bad.items():
+        for i, blk in enumerate(blocks):
+            table[b, blk] = -1 - i if i % 2 else cache[0].shape[0] + b
+    q = torch.randn(4, T, heads, dim, generator=torch.Generator().manual_seed(74)).to(BF16).cuda()
+    w = torch.full((4, kv_heads, table.shape[1] * page), 3.0, device="cuda")
+    out = ops.attention_kv8(q, *cache, table, R.i32(lens), None, w)
+    assert ops.device_error_word() & 8
+    again = ops.attention_kv8(q, *cache, table, R.i32(lens))
+    assert ops.device_error_word() & 8 and torch.equal(out, again)
+    w = w.cpu().double()
+    for b, n in enumerate(lens):
+        ok = torch.ones(n, dtype=torch.bool)
+        for blk in bad[b]:
+            ok[blk * page:(blk + 1) * page] = False
+        t = table.clone()
+        t[b, bad[b]] = 0
+        k, v = (torch.stack([R.read(cache, which, t, b, h, n) for h in range(kv_heads)], 1) for which in (0, 1))
+        mass = torch.zeros(kv_heads, n, dtype=torch.float64)
+        err = torch.zeros(kv_heads, n, dtype=torch.float64)
+        for i in range(T):
+            see = ok & (torch.arange(n) <= n - T + i)
+            ref, p, size, sb = attend_seen(q[b, i].double().cpu(), k, v, see, dim ** -0.5)
+            if not see.any():
+                assert (out[b, i] == 0).all()
+            assert R.max_excess(out[b, i:i + 1], ref, R.out_bound(ref, size, sb, BF16, 2.0 ** -11)) <= 1.0, (b, i)
+            mass += p.view(kv_heads, -1, n).sum(1)
+            err += (p * (2.0 * sb + 2.0 ** -18)).view(kv_heads, -1, n).sum(1)
+        got = w[b, :, :n] - 3.0
+        # 3 + the mass, rounded to float32
+        assert ((got - mass).abs() <= err + (3.0 + mass) * 2.0 ** -23).all(), b
+        assert (got[:, ~ok] == 0).all()
