@@ -706,8 +706,7 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
       if (!all_wait(&ctx_full[item & 1], (item >> 1) & 1) || ctx[kCtxStop]) break;
       // keys that the tile's first row sees, and this row
       const int seen_by_all = ctx[kCtxR0] + ctx[kCtxOff] + s * kPfRows + 1;
-      const bool lead = ctx[kCtxR0] + s * kPfRows + quarter * 32 + lane < ctx[kCtxLead];
-      const int see = lead ? 0 : min(ctx[kCtxLk], seen_by_all + quarter * 32 + lane), n = ctx[kCtxNk + s];
+      const int reach = min(ctx[kCtxLk], seen_by_all + quarter * 32 + lane), n = ctx[kCtxNk + s];
       float m = -INFINITY, sum = 0.f;                            // reference maximum of the raw scores, sum of terms
       const float scale = p.scale_log2;
       bool fail = false;
@@ -720,7 +719,7 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
         tc_fence_after();
         uint32_t x[4][32];
         const bool masked = (j + 1) * kPfRows > seen_by_all;
-        const int here = see - j * kPfRows;
+        const int here = reach - j * kPfRows;
         float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, x[c]);
@@ -790,6 +789,7 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
       const int e_q0 = ctx[kCtxQ0], e_lq = ctx[kCtxLq], e_h = ctx[kCtxH], e_k0 = ctx[kCtxK0], e_jm = ctx[kCtxJm];
       const int first = ctx[kCtxR0] + s * kPfRows + quarter * 32, row = first + lane;   // within the sequence
       const bool live = row < e_lq;
+      const int see = row < ctx[kCtxLead] ? 0 : reach;
       const int64_t at = ((int64_t)ctx[kCtxSplit] * p.rows + e_q0 + row) * p.heads + e_h;   // splits: partial row
       // one of several parts leaves its sums as they are, to be joined; an
       // item of one part says that there is nothing to join

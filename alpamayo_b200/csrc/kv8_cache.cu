@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(kGatherThreads) kv8_gather_kernel(GatherParams
   if (threadIdx.x < 32) {
     int64_t first;
     // the sequence of the first row here, or the first with rows behind it
-    const int64_t into = max((int64_t)0, r0 - (p.B > 0 ? p.cu[0] : 0));
+    const int64_t into = max((int64_t)0, r0 - p.cu[0]);
     int b = warp_find_seq(into, p.B, [&](int i) -> int64_t { return max(0, p.cu[i + 1] - p.cu[i]); }, &first);
     const int64_t row = r0 + threadIdx.x;
     int page = -1, at = 0;
