@@ -127,16 +127,22 @@ class ClipCache:
 
     def prompt(self, lens):
         """Attention for lens[b] packed new tokens of each clip: causal among
-        themselves and, where the clip has cached tokens, over those too (read
-        back from the cache)."""
+        themselves and, where the clip has cached tokens, over those too.  New
+        tokens are seen as they are, cached ones as the cache holds them, so a
+        clip's result does not depend on the other clips."""
         before = self._grow(list(lens))
         cu = _offsets(lens, self.device)
         starts = torch.tensor(before, dtype=torch.int32, device=self.device)
         table, behind = self.table, any(n and m for n, m in zip(before, lens))
         if behind:
-            # only clips with new tokens need their keys
+            # only clips with new tokens need their keys; `new`: the rows of the new tokens among all keys
             ends = [n if m else 0 for n, m in zip(self.lens, lens)]
             cu_k, rows, zero = _offsets(ends, self.device), sum(ends), torch.zeros_like(starts)
+            new, at = [], 0
+            for n, m in zip(ends, lens):
+                at += n
+                new += range(at - m, at)
+            new = torch.tensor(new, dtype=torch.int64, device=self.device)
 
         def attention(layer, qkv):
             q, k, v = self._split(qkv)
@@ -144,6 +150,8 @@ class ClipCache:
             cache.append(k, v, cu, starts, table)
             if behind:
                 kk, vv = cache.gather(table, zero, cu_k, rows, q.dtype)
+                kk.index_copy_(0, new, k)
+                vv.index_copy_(0, new, v)
                 out = ops.attention_prefill(q, kk, vv, cu, cu_k)
             else:
                 out = ops.attention_prefill(q, k, v, cu)

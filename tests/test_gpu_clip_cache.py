@@ -137,3 +137,23 @@ def test_decoder_stack_with_attention():
     # and without one, nothing has changed
     ident = stack.forward(y)
     assert torch.equal(ident, stack.forward(y, attention=lambda i, qkv: qkv[:, :HEADS * HEAD_DIM].contiguous()))
+
+
+def test_a_prompt_does_not_depend_on_the_other_clips():
+    # a clip's first prompt beside another clip's second chunk: bit for bit what it is alone
+    import alpamayo_b200.ops as ops
+    x, y, z = qkv(60, 90), qkv(33, 91), qkv(21, 92)
+    alone = new(1).prompt([33])(0, y)
+    c = new(3)
+    c.prompt([60, 0, 0])(0, x)
+    out = c.prompt([21, 33, 0])(0, torch.cat([z, y]))
+    assert torch.equal(out[21:], alone)
+    # the chunk sees its own tokens as they are and the cached ones as the cache holds them
+    k, v = c.caches[0].gather(c.table, R.i32([0, 0, 0]), R.cu([60, 0, 0]), 60, BF16)
+    t = z.view(21, H + 2 * G, D)
+    want = ops.attention_prefill(t[:, :H], torch.cat([k, t[:, H:H + G]]), torch.cat([v, t[:, H + G:]]), R.cu([21]), R.cu([81]))
+    assert torch.equal(out[:21], want.view(21, -1))
+    # and the cache holds both
+    k, v = c.caches[0].gather(c.table, R.i32([0, 0, 0]), R.cu([81, 33, 0]), 114, torch.float32)
+    assert float((k[81:] - y.view(33, H + 2 * G, D)[:, H:H + G].float()).abs().max()) <= 6 / 254 * 1.01
+    assert c.lens == [81, 33, 0]
