@@ -42,6 +42,8 @@
 // relative error of 2^-9 that bf16 operands of the tensor core have anyhow;
 // it is of the size of the output's own rounding); sums, maxima and the
 // output stay in float32, and the denominator adds the unrounded terms.
+#include <cfloat>
+
 #include "umma.cuh"
 
 namespace paro {
@@ -795,7 +797,10 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_const
       // item of one part says that there is nothing to join
       const bool whole = ctx[kCtxParts] == 1;
       if (p.splits > 1 && live) {
-        p.part_ml[at] = whole ? make_float2(0.f, kInPlace) : make_float2(sum == 0.f ? -INFINITY : m * scale, see > 0 ? sum : 0.f);
+        // a row that sees nothing: -infinity and 0; one whose scores are all
+        // minus infinity: a finite maximum and 0
+        const float top = sum != 0.f ? m * scale : -FLT_MAX;
+        p.part_ml[at] = whole ? make_float2(0.f, kInPlace) : see > 0 ? make_float2(top, sum) : make_float2(-INFINITY, 0.f);
         if (!whole && ctx[kCtxSplit] == 0)
           for (int i = ctx[kCtxParts]; i < p.splits; ++i)
             p.part_ml[at + (int64_t)i * p.rows * p.heads] = make_float2(-INFINITY, 0.f);
@@ -899,7 +904,8 @@ __global__ void __launch_bounds__(256) attn_prefill_join_kernel(const __grid_con
     acc.w = fmaf(v.w, f, acc.w);
     sum = fmaf(ml[i].y, f, sum);
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  // nothing seen: zeros; scores of minus infinity alone: 0 / 0
+  const float inv = sum != 0.f ? 1.f / sum : mx == -INFINITY ? 0.f : __uint_as_float(0x7fffffffu);
   const T o[4] = {from_f32<T>(acc.x * inv), from_f32<T>(acc.y * inv), from_f32<T>(acc.z * inv), from_f32<T>(acc.w * inv)};
   *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at * D + d) = *reinterpret_cast<const uint2*>(o);
 }

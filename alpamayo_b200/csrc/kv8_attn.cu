@@ -39,6 +39,8 @@
 // kernel 75, join 16), one clip of 300 tokens 9 us; 8 verify tokens of 8
 // clips with 32000, fp16, 50 us.  Bound by the instructions per unit (some
 // 820, 12 warps per SM), and with many rows by mma.sync and the widening.
+#include <cfloat>
+
 #include "kv8.cuh"
 
 namespace paro {
@@ -500,7 +502,10 @@ __global__ void __launch_bounds__(kDecWarps * 32, (DecodeTile<D, RB>::kCtas)) kv
 #pragma unroll
       for (int hf = 0; hf < kHalves; ++hf) {
         float x[4][2];
-        float top = -INFINITY;
+        // A row that sees a token has a finite maximum, so that one whose
+        // scores are all minus infinity (0 / 0: NaN) differs from one that
+        // sees nothing (zeros).
+        float top = fmaxf(tok0 < lim[hf] ? ve[0] - FLT_MAX : -INFINITY, tok0 + 16 < lim[hf] ? ve[1] - FLT_MAX : -INFINITY);
         const int r = row0 + hf * 8 + g;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -700,13 +705,19 @@ constexpr int kJoinRows = 8;                  // rows of scores in flight per th
 constexpr int kMaxRows = 512;
 
 // (m, l) joined with (m2, l2); f, f2: what the two sides' values are scaled
-// by.  A side that has seen nothing has l = 0; a NaN stays NaN.
+// by.  A side that has seen nothing has l = 0, m = -infinity; one that has seen
+// scores of minus infinity alone l = 0 and a finite m; a NaN stays NaN.
 __device__ __forceinline__ void join_stats(float& m, float& l, float m2, float l2, float& f, float& f2) {
   const float mx = fmaxf(m, m2);
   f = l == 0.f ? 0.f : exp2f(m - mx);
   f2 = l2 == 0.f ? 0.f : exp2f(m2 - mx);
   l = l * f + l2 * f2;
   m = mx;
+}
+
+// 1 / sum of a row's terms, with what it has seen as above.
+__device__ __forceinline__ float inv_sum(float m, float l) {
+  return l != 0.f ? 1.f / l : m == -INFINITY ? 0.f : __uint_as_float(0x7fffffffu);
 }
 
 template <typename T, int D, int RB>
@@ -777,7 +788,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const __grid_con
         }
     }
     if (part == 0 && r < p.rows) {
-      const float inv = l == 0.f ? 0.f : 1.f / l;   // zeros where the row sees nothing
+      const float inv = inv_sum(m, l);   // zeros where the row sees nothing
       T* dst = static_cast<T*>(p.out) + (((int64_t)b * p.T + r / p.group) * p.heads + h * p.group + r % p.group) * D + col * 4;
       const T o[4] = {from_f32<T>(acc.x * inv), from_f32<T>(acc.y * inv), from_f32<T>(acc.z * inv),
                       from_f32<T>(acc.w * inv)};
@@ -829,8 +840,8 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const __grid_con
       join_stats(m, l, m2, l2, f, f2);
     }
     if (r < p.rows && threadIdx.x % per_row == 0) {
-      s_ml[r] = make_float2(m, l == 0.f ? 0.f : 1.f / l);
-      s_see[r] = l == 0.f ? 0 : len - p.T + r / p.group + 1;
+      s_ml[r] = make_float2(m, inv_sum(m, l));
+      s_see[r] = m == -INFINITY && l == 0.f ? 0 : len - p.T + r / p.group + 1;
     }
   }
   __syncthreads();

@@ -172,3 +172,38 @@ def test_kv8_attention_tokens_of_bad_pages_are_left_out(page, heads, kv_heads, d
         # 3 + the mass, rounded to float32
         assert ((got - mass).abs() <= err + (3.0 + mass) * 2.0 ** -23).all(), b
         assert (got[:, ~ok] == 0).all()
+
+
+@pytest.mark.parametrize("dtype,dim", [(BF16, 128), (F16, 64)])
+@pytest.mark.parametrize("n,m", [(40, 40), (64, 4096)])
+def test_prefill_rows_of_minus_infinity_are_nan(n, m, dim, dtype):
+    # every seen score -inf: 0 / 0 by the formula, whether keys are shared out or not
+    q, k, v = shared_out(n, m, 4, 2, dim, dtype, 75) if m > n else (t.clone() for t in shared_out(64, 4096, 4, 2, dim, dtype, 75))
+    q, k, v = q[:n], k[:m], v[:m]
+    q[:, :2, 3] = q[:, :2, 3].abs()
+    k[:, 0, 3] = -INF
+    cq, ck = R.cu([n]), R.cu([m])
+    for out in (prefill_into_dirty_memory(q.cuda(), k.cuda(), v.cuda(), cq, ck), prefill_unsplit(q.cuda(), k.cuda(), v.cuda(), cq, ck)):
+        assert torch.isnan(out[:, :2]).all() and torch.isfinite(out[:, 2:]).all()
+    # one seen score is finite: its value alone
+    k[0, 0, 3] = 0.0
+    for out in (prefill_into_dirty_memory(q.cuda(), k.cuda(), v.cuda(), cq, ck), prefill_unsplit(q.cuda(), k.cuda(), v.cuda(), cq, ck)):
+        assert torch.equal(out[:, :2].cpu(), v[0, 0].expand(n, 2, dim))
+
+
+@pytest.mark.parametrize("heads,T", [(2, 1), (7, 1), (12, 1), (9, 3), (8, 8)])
+@pytest.mark.parametrize("n", [20, 900])
+def test_kv8_attention_rows_of_minus_infinity_are_nan(n, heads, T):
+    import alpamayo_b200.ops as ops
+    *cache, table = R.make_pool([n, 30], 16, 1, 64, 76)
+    cache[0][..., 3] = -5
+    q = torch.randn(2, T, heads, 64, generator=torch.Generator().manual_seed(77)).to(BF16)
+    q[0, 0, 0, 3] = INF                                    # times -5 everywhere: -inf for every token
+    q = q.cuda()
+    w = torch.zeros(2, 1, table.shape[1] * 16, device="cuda")
+    out = ops.attention_kv8(q, *cache, table, R.i32([n, 30]), None, w)
+    assert torch.isnan(out[0, 0, 0]).all()
+    rest = out.clone()
+    rest[0, 0, 0] = 0
+    assert torch.isfinite(rest).all()
+    assert torch.isnan(w[0, 0, :n - T + 1]).all() and torch.isfinite(w[0, 0, n - T + 1:]).all() and torch.isfinite(w[1]).all()
