@@ -207,3 +207,38 @@ def test_kv8_attention_rows_of_minus_infinity_are_nan(n, heads, T):
     rest[0, 0, 0] = 0
     assert torch.isfinite(rest).all()
     assert torch.isnan(w[0, 0, :n - T + 1]).all() and torch.isfinite(w[0, 0, n - T + 1:]).all() and torch.isfinite(w[1]).all()
+
+
+@pytest.mark.parametrize("factor", [2.0 ** 62, 1e25, 1e34])
+@pytest.mark.parametrize("every", [True, False])
+def test_kv8_attention_values_of_extreme_sizes(every, factor):
+    import alpamayo_b200.ops as ops
+    lens = [200, 7]
+    *cache, table = R.make_pool(lens, 16, 1, 128, 78)
+    big = table[0, :13] if every else table[0, 2:5]
+    cache[3][big.long()] *= factor
+    q = torch.randn(2, 1, 4, 128, generator=torch.Generator().manual_seed(79)).to(BF16).cuda()
+    w = torch.zeros(2, 1, table.shape[1] * 16, device="cuda")
+    out = ops.attention_kv8(q, *cache, table, R.i32(lens), None, w)
+    for b, n in enumerate(lens):
+        k, v = R.read(cache, 0, table, b, 0, n)[:, None], R.read(cache, 1, table, b, 0, n)[:, None]
+        ref, p, size, sb = R.attend(q[b].double().cpu(), k, v, 128 ** -0.5)
+        assert R.max_excess(out[b], ref, R.out_bound(ref, size, sb, BF16, 2.0 ** -11)) <= 1.0, b
+        mass = p.sum((0, 1))
+        assert ((w[b, 0, :n].double().cpu() - mass).abs() <= mass * (2.0 * float(sb.max()) + 2.0 ** -17)).all()
+
+
+def test_kv8_attention_queries_near_the_largest_bf16():
+    import alpamayo_b200.ops as ops
+    lens = [100, 100]
+    *cache, table = R.make_pool(lens, 16, 1, 64, 80)
+    q = torch.randn(2, 1, 2, 64, generator=torch.Generator().manual_seed(81))
+    q[0] *= 5e37 / float(q[0].abs().max())
+    q[1] *= 1e36 / float(q[1].abs().max())
+    q = q.to(BF16).cuda()
+    scale = 1e-37
+    out = ops.attention_kv8(q, *cache, table, R.i32(lens), scale)
+    for b, n in enumerate(lens):
+        k, v = R.read(cache, 0, table, b, 0, n)[:, None], R.read(cache, 1, table, b, 0, n)[:, None]
+        ref, _, size, sb = R.attend(q[b].double().cpu(), k, v, scale)
+        assert R.max_excess(out[b], ref, R.out_bound(ref, size, sb, BF16, 2.0 ** -11)) <= 1.0, b
