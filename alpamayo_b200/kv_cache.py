@@ -205,17 +205,26 @@ class ClipCache:
         the tokens kept, per layer."""
         if self.totals is None:
             raise RuntimeError("eviction needs a ClipCache with totals=True")
+        if sink < 0 or recent < 0 or budget <= 0 or sink + recent > budget:
+            raise ValueError("budget must be positive and hold sink + recent tokens")
         width = -(-budget // self.page_size)
         if width > self.width:
             raise ValueError("budget is larger than the cache's capacity")
-        fresh = [self._take(-(-min(n, budget) // self.page_size)) for n in self.lens]
-        out_table = torch.tensor([p + [-1] * (width - len(p)) for p in fresh], dtype=torch.int32, device=self.device)
+        need = [-(-min(n, budget) // self.page_size) for n in self.lens]
+        taken = self._take(sum(need))
+        fresh = [[taken.pop() for _ in range(n)] for n in need]
+        try:
+            out_table = torch.tensor([p + [-1] * (width - len(p)) for p in fresh], dtype=torch.int32, device=self.device)
+            cut = [cache.evict(totals, self.table, self.seq_lens, out_table, budget, sink, recent)
+                   for cache, totals in zip(self.caches, self.totals)]
+        except BaseException:
+            self.free += [p for pages in fresh for p in pages]
+            raise
         kept = []
-        for i, cache in enumerate(self.caches):
-            tokens, totals, _ = cache.evict(self.totals[i], self.table, self.seq_lens, out_table, budget, sink, recent)
+        for totals, (tokens, new_totals, _) in zip(self.totals, cut):
             kept.append(tokens)
-            self.totals[i].zero_()
-            self.totals[i][:, :, :budget] = totals
+            totals.zero_()
+            totals[:, :, :budget] = new_totals
         for b in range(len(self.lens)):
             self.free += self.pages[b]
             self.pages[b] = fresh[b]
