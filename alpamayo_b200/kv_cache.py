@@ -200,9 +200,10 @@ class ClipCache:
         self._state()
 
     def evict(self, budget, sink=4, recent=0):
-        """Cut every clip to its `budget` most attended tokens per KV head (and
-        layer), its first `sink` and last `recent` ones among them.  Returns
-        the tokens kept, per layer."""
+        """Cut every clip of more tokens to its `budget` most attended ones per
+        KV head (and layer), its first `sink` and last `recent` ones among
+        them; a shorter clip stays in its pages as it is.  Returns the tokens
+        kept, per layer: int32 [clips, kv_heads, budget], -1 behind the last."""
         if self.totals is None:
             raise RuntimeError("eviction needs a ClipCache with totals=True")
         if sink < 0 or recent < 0 or budget <= 0 or sink + recent > budget:
@@ -210,24 +211,32 @@ class ClipCache:
         width = -(-budget // self.page_size)
         if width > self.width:
             raise ValueError("budget is larger than the cache's capacity")
-        need = [-(-min(n, budget) // self.page_size) for n in self.lens]
+        over = [n > budget for n in self.lens]
+        places = torch.arange(budget, dtype=torch.int32, device=self.device)
+        whole = torch.where(places < self.seq_lens[:, None], places, -1)[:, None]     # a clip that keeps all
+        if not any(over):
+            return [whole.repeat(1, self.kv_heads, 1) for _ in self.caches]
+        need = [width if o else 0 for o in over]
         taken = self._take(sum(need))
         fresh = [[taken.pop() for _ in range(n)] for n in need]
         try:
             out_table = torch.tensor([p + [-1] * (width - len(p)) for p in fresh], dtype=torch.int32, device=self.device)
-            cut = [cache.evict(totals, self.table, self.seq_lens, out_table, budget, sink, recent)
+            cuts = (self.seq_lens > budget)[:, None, None]
+            lens = torch.where(cuts[:, 0, 0], self.seq_lens, 0)                       # nothing is moved for the others
+            cut = [cache.evict(totals, self.table, lens, out_table, budget, sink, recent)
                    for cache, totals in zip(self.caches, self.totals)]
         except BaseException:
             self.free += [p for pages in fresh for p in pages]
             raise
         kept = []
         for totals, (tokens, new_totals, _) in zip(self.totals, cut):
-            kept.append(tokens)
-            totals.zero_()
-            totals[:, :, :budget] = new_totals
-        for b in range(len(self.lens)):
-            self.free += self.pages[b]
-            self.pages[b] = fresh[b]
-            self.lens[b] = min(self.lens[b], budget)
+            kept.append(torch.where(cuts, tokens, whole))
+            totals[:, :, :budget] = torch.where(cuts, new_totals, totals[:, :, :budget])
+            totals[:, :, budget:] = 0
+        for b, o in enumerate(over):
+            if o:
+                self.free += self.pages[b]
+                self.pages[b] = fresh[b]
+                self.lens[b] = budget
         self._state()
         return kept

@@ -157,3 +157,34 @@ def test_a_prompt_does_not_depend_on_the_other_clips():
     k, v = c.caches[0].gather(c.table, R.i32([0, 0, 0]), R.cu([81, 33, 0]), 114, torch.float32)
     assert float((k[81:] - y.view(33, H + 2 * G, D)[:, H:H + G].float()).abs().max()) <= 6 / 254 * 1.01
     assert c.lens == [81, 33, 0]
+
+
+def test_evict_leaves_clips_under_budget_where_they_are():
+    c = new(3, totals=True, capacity=128)
+    x = qkv(190, 93)
+    c.prompt([100, 50, 40])(0, x)
+    live = torch.arange(128, device="cuda")[None] < c.seq_lens[:, None]
+    for t in c.totals:
+        t.copy_(torch.rand_like(t))
+        t *= live[:, None]
+    totals, pages = [t.clone() for t in c.totals], [list(p) for p in c.pages]
+    tensors = [t.clone() for t in c.caches[0].tensors]
+    c.free = c.free[:4]                                     # room for the first clip's 50 tokens, and no more
+    kept = c.evict(50, sink=2, recent=8)
+    assert c.lens == [50, 50, 40] and c.seq_lens.tolist() == c.lens
+    assert c.pages[1:] == pages[1:] and sorted(c.free) == sorted(pages[0])
+    for b, n in ((1, 50), (2, 40)):
+        p = torch.tensor(pages[b])
+        assert all(torch.equal(t[p], u[p]) for t, u in zip(c.caches[0].tensors, tensors))
+        for layer in range(2):
+            assert kept[layer][b].tolist() == [list(range(n)) + [-1] * (50 - n)] * G
+            assert torch.equal(c.totals[layer][b], totals[layer][b])
+    for layer in range(2):
+        assert kept[layer].shape == (3, G, 50) and kept[layer].dtype == torch.int32
+        idx = kept[layer][0].long()
+        assert torch.equal(c.totals[layer][0, :, :50], totals[layer][0].gather(1, idx)) and (c.totals[layer][0, :, 50:] == 0).all()
+    # nothing to evict: nothing moves, no pages needed
+    c.free = []
+    pages = [list(p) for p in c.pages]
+    kept = c.evict(64)
+    assert c.pages == pages and c.lens == [50, 50, 40] and kept[1][2].tolist() == [list(range(40)) + [-1] * 24] * G
