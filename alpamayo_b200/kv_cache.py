@@ -58,11 +58,19 @@ class KV8Cache:
         return ops.kv8_evict(weights, *self.tensors, page_table, seq_lens, out_table, budget, sink, recent)
 
 
+def _send(values, device, dtype=torch.int32):
+    """Host integers on the device without waiting for its stream: the copy
+    comes from pinned memory, which the allocator keeps until it has run."""
+    if torch.device(device).type != "cuda":
+        return torch.tensor(values, dtype=dtype, device=device)
+    return torch.tensor(values, dtype=dtype, pin_memory=True).to(device, non_blocking=True)
+
+
 def _offsets(lens, device):
     cu = [0]
     for n in lens:
         cu.append(cu[-1] + n)
-    return torch.tensor(cu, dtype=torch.int32, device=device)
+    return _send(cu, device)
 
 
 class ClipCache:
@@ -72,8 +80,9 @@ class ClipCache:
     prompt(), step() and verify() return the attention of the next forward
     pass, a callable (layer, qkv) -> attention output for
     ``DecoderStack.forward(x, attention=...)``, with qkv [rows, (heads + 2 *
-    kv_heads) * head_dim].  Lengths and pages are counted on the host; nothing
-    synchronises.  With ``totals`` the softmax weight of every cached token is
+    kv_heads) * head_dim].  Lengths and pages are counted on the host and sent to
+    the device on the current stream, which orders all of a cache's calls; no
+    call waits for the device.  With ``totals`` the softmax weight of every cached token is
     accumulated by step() and verify(), which evict() needs.  `spare` tokens of
     pages per clip are held free for evict()."""
 
@@ -93,8 +102,8 @@ class ClipCache:
 
     def _state(self):
         rows = [p + [-1] * (self.width - len(p)) for p in self.pages]
-        self.table = torch.tensor(rows, dtype=torch.int32, device=self.device)
-        self.seq_lens = torch.tensor(self.lens, dtype=torch.int32, device=self.device)
+        self.table = _send(rows, self.device)
+        self.seq_lens = _send(self.lens, self.device)
 
     def _take(self, n):
         if n > len(self.free):
@@ -132,7 +141,7 @@ class ClipCache:
         clip's result does not depend on the other clips."""
         before = self._grow(list(lens))
         cu = _offsets(lens, self.device)
-        starts = torch.tensor(before, dtype=torch.int32, device=self.device)
+        starts = _send(before, self.device)
         table, behind = self.table, any(n and m for n, m in zip(before, lens))
         if behind:
             # only clips with new tokens need their keys; `new`: the rows of the new tokens among all keys
@@ -142,7 +151,7 @@ class ClipCache:
             for n, m in zip(ends, lens):
                 at += n
                 new += range(at - m, at)
-            new = torch.tensor(new, dtype=torch.int64, device=self.device)
+            new = _send(new, self.device, torch.int64)
 
         def attention(layer, qkv):
             q, k, v = self._split(qkv)
@@ -165,7 +174,7 @@ class ClipCache:
         clips = len(self.lens)
         before = self._grow([new] * clips)
         cu = _offsets([new] * clips, self.device)
-        starts = torch.tensor(before, dtype=torch.int32, device=self.device)
+        starts = _send(before, self.device)
         table, seq_lens = self.table, self.seq_lens
 
         def attention(layer, qkv):
@@ -220,7 +229,7 @@ class ClipCache:
         taken = self._take(sum(need))
         fresh = [[taken.pop() for _ in range(n)] for n in need]
         try:
-            out_table = torch.tensor([p + [-1] * (width - len(p)) for p in fresh], dtype=torch.int32, device=self.device)
+            out_table = _send([p + [-1] * (width - len(p)) for p in fresh], self.device)
             cuts = (self.seq_lens > budget)[:, None, None]
             lens = torch.where(cuts[:, 0, 0], self.seq_lens, 0)                       # nothing is moved for the others
             cut = [cache.evict(totals, self.table, lens, out_table, budget, sink, recent)

@@ -188,3 +188,39 @@ def test_evict_leaves_clips_under_budget_where_they_are():
     pages = [list(p) for p in c.pages]
     kept = c.evict(64)
     assert c.pages == pages and c.lens == [50, 50, 40] and kept[1][2].tolist() == [list(range(40)) + [-1] * 24] * G
+
+
+def test_no_call_waits_for_the_device():
+    c = new(2, totals=True, spare=64)
+    x = qkv(140, 94)
+
+    def all_calls():
+        c.prompt([30, 20])(0, x[:50])
+        c.prompt([20, 0])(0, x[50:70])
+        c.step()(0, x[70:72])
+        c.verify(3)(0, x[72:78])
+        c.accept([1, 0])
+        c.evict(40, sink=2, recent=8)
+    all_calls()                                             # what is allocated or loaded once
+    torch.cuda.synchronize()
+    mode = torch.cuda.get_sync_debug_mode()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        all_calls()
+    finally:
+        torch.cuda.set_sync_debug_mode(mode)
+    assert c.seq_lens.tolist() == c.lens
+
+
+def test_lengths_and_tables_sent_far_ahead_of_the_device():
+    c = new(2, totals=True)
+    torch.cuda.synchronize()
+    torch.cuda._sleep(200_000_000)                          # about a tenth of a second: every copy below waits behind it
+    seen = []
+    for i in range(150):
+        c._grow([1, 2 if i < 20 else 0])
+        seen.append((c.seq_lens, c.table, list(c.lens), [list(p) for p in c.pages]))
+    torch.cuda.synchronize()
+    for lens, table, want, pages in seen:
+        assert lens.tolist() == want
+        assert table.tolist() == [p + [-1] * (c.width - len(p)) for p in pages]
