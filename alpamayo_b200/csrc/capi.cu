@@ -889,7 +889,7 @@ int paro_kv8_append(const paro_kv8_cache* cache, const int32_t* page_table, int 
   if (rows == 0 || B == 0) return PARO_OK;
   if (!k || !v || !strides || !cu || !starts) return PARO_ERR_INVALID_ARGUMENT;
   if (rows > 0x7FFFFFFF) return PARO_ERR_TOO_LARGE;
-  if (!aligned(k, 16) || !aligned(v, 16)) return PARO_ERR_MISALIGNED;
+  if (!aligned(k, 16) || !aligned(v, 16) || !aligned(cu, 4) || !aligned(starts, 4)) return PARO_ERR_MISALIGNED;
   for (int i = 0; i < 4; ++i)
     if (strides[i] < 0 || strides[i] % (16 / (int64_t)elem_bytes(dtype))) return PARO_ERR_MISALIGNED;
   if (int d = device_check()) return d;
@@ -906,7 +906,7 @@ int paro_kv8_gather(const paro_kv8_cache* cache, const int32_t* page_table, int 
   if (rows == 0) return PARO_OK;
   if (!out_k || !out_v || !cu || !starts) return PARO_ERR_INVALID_ARGUMENT;
   if (rows > 0x7FFFFFFF) return PARO_ERR_TOO_LARGE;
-  if (!aligned(out_k, 16) || !aligned(out_v, 16)) return PARO_ERR_MISALIGNED;
+  if (!aligned(out_k, 16) || !aligned(out_v, 16) || !aligned(cu, 4) || !aligned(starts, 4)) return PARO_ERR_MISALIGNED;
   if (int d = device_check()) return d;
   return cuda_status(launch_kv8_gather(c, starts, cu, B, rows, out_k, out_v, dtype, (cudaStream_t)stream));
 }
@@ -926,7 +926,9 @@ int paro_attention_kv8(const paro_kv8_cache* cache, const int32_t* page_table, i
   if (weights && cap < (int64_t)table_width * c_page(c)) return PARO_ERR_SHAPE;
   // pieces of 32 tokens of all sequences and heads are counted in 31 bits
   if ((int64_t)table_width * c_page(c) / 16 * B >= 0x7FFFFFFF / c.kv_heads) return PARO_ERR_TOO_LARGE;
-  if (!aligned(q, 16) || !aligned(out, 16) || !aligned(workspace, 256)) return PARO_ERR_MISALIGNED;
+  if (!aligned(q, 16) || !aligned(out, 16) || !aligned(workspace, 256) || !aligned(lens, 4) || !aligned(weights, 4) ||
+      !aligned(weights_out, 4))
+    return PARO_ERR_MISALIGNED;
   for (int i = 0; i < 3; ++i)
     if (strides[i] < 0 || strides[i] % 8) return PARO_ERR_MISALIGNED;
   if (workspace_bytes < kv8_attn_workspace(c, B, T, heads, weights != nullptr)) return PARO_ERR_WORKSPACE;
@@ -946,6 +948,9 @@ int paro_kv8_evict(const paro_kv8_cache* cache, const int32_t* page_table, int t
   if ((int64_t)out_width * c_page(c) < budget || cap < (int64_t)table_width * c_page(c)) return PARO_ERR_SHAPE;
   if (B == 0) return PARO_OK;
   if (!weights || !lens || !kept || !new_weights || !new_lens || !out_table) return PARO_ERR_INVALID_ARGUMENT;
+  if (!aligned(weights, 4) || !aligned(lens, 4) || !aligned(kept, 4) || !aligned(new_weights, 4) ||
+      !aligned(new_lens, 4) || !aligned(out_table, 4))
+    return PARO_ERR_MISALIGNED;
   if (int d = device_check()) return d;
   return cuda_status(launch_kv8_evict(c, weights, cap, lens, B, budget, sink, recent, kept, new_weights, new_lens,
                                       out_table, out_width, (cudaStream_t)stream));

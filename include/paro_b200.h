@@ -498,7 +498,8 @@ int paro_w4a8_gemm_noalloc(const int8_t* xq, const float* xscale, int64_t M, int
  *   page_table       : int32 [B][table_width]; token t of sequence b lies in
  *                      page page_table[b][t / page_size]; entries behind a
  *                      sequence's last token are not read
- * page_size 16, 32, 64 or 128; head_dim 64 or 128.  A page belongs to one
+ * page_size 16, 32, 64 or 128; head_dim 64 or 128; int32 and float32 arrays
+ * of these entry points are 4-byte aligned.  A page belongs to one
  * sequence while it is written.  A page-table entry outside the pool, or a
  * length beyond the table's row, sets bit 8 of the device error word, and
  * the tokens concerned are left out (nothing out of bounds is touched):

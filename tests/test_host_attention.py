@@ -113,3 +113,19 @@ def test_evict_statuses(L):
     assert ev(budget=33) == SHAPE                    # two pages of 16
     assert ev(cap=63) == SHAPE
     assert ev(B=0) == OK
+
+
+def test_misaligned_index_and_weight_pointers(L):
+    odd = P + 2                                      # int32 and float32 arrays begin on 4-byte boundaries
+    c, table = cache(), P
+    st4, st3 = strides(512, 128, 512, 128), strides(3584, 3584, 128)
+    app = lambda cu=P, starts=P: L.paro_kv8_append(ctypes.byref(c), table, 4, P, P, 2, st4, cu, starts, 2, 8, None)  # noqa: E731
+    gat = lambda cu=P, starts=P: L.paro_kv8_gather(ctypes.byref(c), table, 4, starts, cu, 2, 8, P, P, 2, None)  # noqa: E731
+    att = lambda lens=P, w=P, wo=P: L.paro_attention_kv8(ctypes.byref(c), table, 4, P, 2, st3, 2, 1, 28, lens, 1.0, w,  # noqa: E731
+                                                         wo, 64, P, P, 1 << 40, None)
+    ev = lambda w=P, lens=P, kept=P, nw=P, nl=P, out=P: L.paro_kv8_evict(ctypes.byref(c), table, 4, w, 64, lens, 2, 32, 4,  # noqa: E731
+                                                                         8, kept, nw, nl, out, 2, None)
+    assert app(cu=odd) == app(starts=odd) == MISALIGNED
+    assert gat(cu=odd) == gat(starts=odd) == MISALIGNED
+    assert att(lens=odd) == att(w=odd) == att(wo=odd) == MISALIGNED
+    assert [ev(**{k: odd}) for k in ("w", "lens", "kept", "nw", "nl", "out")] == [MISALIGNED] * 6
