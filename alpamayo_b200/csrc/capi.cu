@@ -148,6 +148,10 @@ int device_check() {
 namespace {
 int64_t c_page(const Kv8View& c) { return (int64_t)1 << c.page_shift; }
 
+// Rows and tokens of a call, at most: the kernels step through them in ints,
+// up to 4096 at a time, and round them up to whole tiles.
+constexpr int64_t kMaxTokens = 0x7FFF0000;
+
 // The cache and its page table as the kernels take them, or a status.
 int kv8_view(const paro_kv8_cache* cache, const int32_t* table, int table_width, int B, Kv8View* out) {
   if (!cache || !table || B < 0 || table_width <= 0) return PARO_ERR_INVALID_ARGUMENT;
@@ -159,7 +163,7 @@ int kv8_view(const paro_kv8_cache* cache, const int32_t* table, int table_width,
   if (cache->head_dim != 64 && cache->head_dim != 128) return PARO_ERR_SHAPE;
   // grid dimensions: kv_heads in y, 2 B in z; lengths are 32-bit
   if (cache->kv_heads > 1024 || B > 32767 || cache->num_pages > 0x7FFFFFFF ||
-      (int64_t)table_width * cache->page_size > 0x7FFFFFFF)
+      (int64_t)table_width * cache->page_size > kMaxTokens)
     return PARO_ERR_TOO_LARGE;
   if (!aligned(cache->k_codes, 16) || !aligned(cache->v_codes, 16) || !aligned(cache->k_scale, 4) ||
       !aligned(cache->v_scale, 4) || !aligned(table, 4))
@@ -857,7 +861,7 @@ int paro_attention_prefill_ws(const void* q, const void* k, const void* v, int d
   if (dtype != PARO_BF16 && dtype != PARO_F16) return PARO_ERR_UNSUPPORTED;
   if (heads % kv_heads || (head_dim != 64 && head_dim != 128)) return PARO_ERR_SHAPE;
   if (!(scale >= 0.f) || scale > 3.0e38f) return PARO_ERR_INVALID_ARGUMENT;
-  if (rows > 0x7FFFFFFF || k_rows > 0x7FFFFFFF || heads > 65535) return PARO_ERR_TOO_LARGE;
+  if (rows > kMaxTokens || k_rows > kMaxTokens || heads > 65535) return PARO_ERR_TOO_LARGE;
   if (rows == 0) return PARO_OK;
   if (!q || !out || !strides || !cu_q || !cu_k || (k_rows > 0 && (!k || !v))) return PARO_ERR_INVALID_ARGUMENT;
   if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16) || !aligned(cu_q, 4) ||
@@ -945,6 +949,7 @@ int paro_kv8_evict(const paro_kv8_cache* cache, const int32_t* page_table, int t
   if (int rc = kv8_view(cache, page_table, table_width, B, &c)) return rc;
   if (budget <= 0 || sink < 0 || recent < 0 || (int64_t)sink + recent > budget || out_width <= 0)
     return PARO_ERR_INVALID_ARGUMENT;
+  if (budget > kMaxTokens) return PARO_ERR_TOO_LARGE;
   if ((int64_t)out_width * c_page(c) < budget || cap < (int64_t)table_width * c_page(c)) return PARO_ERR_SHAPE;
   if (B == 0) return PARO_OK;
   if (!weights || !lens || !kept || !new_weights || !new_lens || !out_table) return PARO_ERR_INVALID_ARGUMENT;

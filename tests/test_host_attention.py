@@ -129,3 +129,16 @@ def test_misaligned_index_and_weight_pointers(L):
     assert gat(cu=odd) == gat(starts=odd) == MISALIGNED
     assert att(lens=odd) == att(w=odd) == att(wo=odd) == MISALIGNED
     assert [ev(**{k: odd}) for k in ("w", "lens", "kept", "nw", "nl", "out")] == [MISALIGNED] * 6
+
+
+def test_sizes_next_to_the_largest_int(L):
+    # the kernels step through rows and tokens in ints, some thousands at a time
+    top = 0x7FFFFFFF
+    st4 = strides(512, 128, 512, 128)
+    c = cache()
+    ev = lambda budget, width: L.paro_kv8_evict(ctypes.byref(c), P, 4, P, 64, P, 2, budget, 4, 8, P, P, P, P, width, None)  # noqa: E731
+    assert ev(top, 1 << 27) == TOO_LARGE
+    assert ev(top - 4000, 1 << 27) == TOO_LARGE
+    assert L.paro_kv8_append(ctypes.byref(c), P, top // 16, P, P, 2, st4, P, P, 2, 8, None) == TOO_LARGE
+    assert prefill(L, rows=top) == TOO_LARGE
+    assert prefill(L, k_rows=top) == TOO_LARGE
