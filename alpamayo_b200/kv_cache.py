@@ -20,6 +20,7 @@ import torch
 from . import ops
 
 PAGE_SIZES, HEAD_DIMS = (16, 32, 64, 128), (64, 128)
+MAX_ROWS = 512   # of ops.attention_kv8: new tokens times query heads per KV head
 
 
 class KV8Cache:
@@ -171,6 +172,8 @@ class ClipCache:
     def verify(self, new):
         """Attention for `new` tokens of every clip (rows clip by clip), as a
         draft's verification runs them; accept() says how many of them stay."""
+        if new * (self.heads // self.kv_heads) > MAX_ROWS:
+            raise ValueError(f"{new} tokens at a time: at most {MAX_ROWS // (self.heads // self.kv_heads)}")
         clips = len(self.lens)
         before = self._grow([new] * clips)
         cu = _offsets([new] * clips, self.device)

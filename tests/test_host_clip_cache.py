@@ -52,3 +52,15 @@ def test_evict_gives_pages_back_when_a_layer_fails(monkeypatch):
     with pytest.raises(RuntimeError, match="no"):
         c.evict(32)
     assert books(c) == before and all(torch.equal(a, b) for a, b in zip(c.totals, totals))
+
+
+def test_verify_refuses_more_rows_than_the_kernels_take():
+    # 512 query rows to a KV head: 170 tokens at three heads each
+    c = new(2, capacity=256)
+    before = books(c)
+    for tokens in (171, 200, -1):
+        with pytest.raises(ValueError):
+            c.verify(tokens)
+        assert books(c) == before
+    c.verify(170)
+    assert c.lens == [170, 170]
