@@ -206,7 +206,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> kv8_evict(const at::Tensor& weigh
               "paro_b200: weights must be float32 [B, kv_heads, capacity]");
   TORCH_CHECK(out_table.dim() == 2 && out_table.size(0) == c.B && out_table.size(1) <= INT32_MAX,
               "paro_b200: out_table must be int32 [B, pages per sequence]");
-  TORCH_CHECK(budget > 0 && budget <= INT32_MAX && sink >= 0 && recent >= 0 && sink + recent <= budget,
+  TORCH_CHECK(budget > 0 && budget <= INT32_MAX && sink >= 0 && recent >= 0 && sink <= budget && recent <= budget - sink,
               "paro_b200: budget must be positive and hold sink + recent tokens");
   c10::cuda::CUDAGuard guard(k_codes.device());
   at::Tensor kept = at::empty({c.B, c.c.kv_heads, budget}, lens.options());

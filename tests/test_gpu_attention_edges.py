@@ -242,3 +242,13 @@ def test_kv8_attention_queries_near_the_largest_bf16():
         k, v = R.read(cache, 0, table, b, 0, n)[:, None], R.read(cache, 1, table, b, 0, n)[:, None]
         ref, _, size, sb = R.attend(q[b].double().cpu(), k, v, scale)
         assert R.max_excess(out[b], ref, R.out_bound(ref, size, sb, BF16, 2.0 ** -11)) <= 1.0, b
+
+
+def test_evict_refuses_sinks_whose_sum_overflows():
+    import alpamayo_b200.ops as ops
+    *cache, table = R.make_pool([64], 16, 1, 64, 82, extra=4)
+    w = torch.rand(1, 1, 64, device="cuda")
+    with pytest.raises(RuntimeError):
+        ops.kv8_evict(w, *cache, table, R.i32([64]), R.i32([[0, 1]]), 32, 2 ** 62 + 5, 2 ** 62 + 5)
+    with pytest.raises(RuntimeError):
+        ops.kv8_evict(w, *cache, table, R.i32([64]), R.i32([[0, 1]]), 32, 4, 2 ** 63 - 1)
