@@ -252,3 +252,28 @@ def test_evict_refuses_sinks_whose_sum_overflows():
         ops.kv8_evict(w, *cache, table, R.i32([64]), R.i32([[0, 1]]), 32, 2 ** 62 + 5, 2 ** 62 + 5)
     with pytest.raises(RuntimeError):
         ops.kv8_evict(w, *cache, table, R.i32([64]), R.i32([[0, 1]]), 32, 4, 2 ** 63 - 1)
+
+
+def test_operators_trace_as_they_run():
+    # schemas (what is written, what aliases) and traced shapes against the real calls
+    import alpamayo_b200.ops as ops  # noqa: F401
+    _ops = torch.ops.paro_b200
+    lens = [30, 9]
+    *cache, table = R.make_pool(lens, 16, 2, 64, 83, extra=6)
+    cache = [t.clone() for t in cache]
+    used = set(table.flatten().tolist())
+    free = [p for p in range(cache[0].shape[0]) if p not in used]
+    q = torch.randn(39, 4, 64, device="cuda").to(BF16)
+    k, v = (torch.randn(39, 2, 64, device="cuda").to(BF16) for _ in range(2))
+    w = torch.rand(2, 2, table.shape[1] * 16, device="cuda")
+    cu, n = R.cu(lens), R.i32(lens)
+    calls = [(_ops.attention_prefill, (q, k, v, cu, None, 0.1)),
+             (_ops.attention_prefill, (q[:2], k, v, R.cu([1, 1]), cu, 0.1)),
+             (_ops.kv8_append, (k, v, cu, R.i32([0, 0]), *cache, table)),
+             (_ops.kv8_gather, (*cache, table, R.i32([0, 0]), cu, 39, F16)),
+             (_ops.attention_kv8, (q[:2, None], *cache, table, n, 0.1, None, None)),
+             (_ops.attention_kv8, (q[:2, None], *cache, table, n, 0.1, w, torch.empty_like(w))),
+             (_ops.kv8_evict, (w, *cache, table, n, R.i32(free[:4]).view(2, 2), 20, 2, 3))]
+    for op, args in calls:
+        for check in ("test_schema", "test_faketensor"):
+            torch.library.opcheck(op.default, args, test_utils=check)
