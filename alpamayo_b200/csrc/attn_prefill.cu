@@ -23,7 +23,7 @@
 //    warps store the last one's output.  28 heads, 8 prompts of 1 to 1500
 //    tokens (560 items of 1 to 12 tiles): 61 us with an item per CTA, 58 with
 //    the items shared out evenly beforehand, 53 like this; one prompt of 8192
-//    gains 1 %; one of 37, whose items have a CTA each either way, takes 8.4
+//    gains 1 %; one of 37, whose items have a CTA each either way, takes 8.6
 //    us for 7.5 (the hand-over of its description).
 //  * warp 9: MMAs, one thread: S = Q K^T (both K-major in shared memory) and
 //    O += P V (P in tensor memory, V with its columns contiguous, i.e.

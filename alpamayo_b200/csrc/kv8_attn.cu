@@ -36,10 +36,15 @@
 // accumulates them, one writer per element, so every result is independent
 // of timing.
 //
-// 28 query over 4 key/value heads of 128, bf16: one clip of 131072 tokens 41 us
-// (134 MB, 3.3 TB/s over all, some 5 in the steady part: 8 us go into start-up
-// and join), 64 clips with 262144 tokens and weights 91 us (278 MB; first
-// kernel 75, join 16), one clip of 300 tokens 9 us; 8 verify tokens of 8
+// A page that the table does not have in the pool is copied from page 0 with
+// key scales of zero, and minus infinity is added to its scores.  A row that
+// sees a token has a finite maximum, whatever its scores are: it tells a row
+// of nothing but minus infinity (NaN) from one that sees nothing (zeros).
+//
+// 28 query over 4 key/value heads of 128, bf16: one clip of 131072 tokens 42 us
+// (134 MB, 3.2 TB/s over all, some 5 in the steady part: 8 us go into start-up
+// and join), 64 clips with 262144 tokens and weights 90 us (278 MB; first
+// kernel 74, join 16), one clip of 300 tokens 10 us; 8 verify tokens of 8
 // clips with 32000, fp16, 50 us.  Bound by the instructions per unit (some
 // 820, 12 warps per SM), and with many rows by mma.sync and the widening.
 #include <cfloat>

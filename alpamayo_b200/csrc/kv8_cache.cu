@@ -14,10 +14,12 @@
 //  * compact (eviction's second half): code * scale of the kept tokens,
 //    requantised per destination page.
 //
-// 4 heads of 128: 8192 tokens of six prompts appended in 20 us (51 MB), one
-// token of 64 clips in 10; 64 clips with 262144 tokens cut to 2048 each, and
-// read back, in 167 us (614 MB; compaction 78, selection 30); one clip of
-// 32768 cut to 4096 in 32, most of it the selection's chain of barriers.
+// 4 heads of 128, bf16: 8192 tokens of six prompts appended in 12 us (25 MB),
+// appended and read back in 20 (51 MB); one token of 64 clips in 5, and with
+// its pages read back in 11; 64 clips with 262144 tokens cut to 2048 each, and
+// read back, in 170 us (614 MB; compaction 78, selection 30); one clip of
+// 32768 cut to 4096, and read back, in 34, most of it the selection's chain of
+// barriers.
 #include <cooperative_groups.h>
 
 #include "kv8.cuh"

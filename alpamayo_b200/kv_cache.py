@@ -83,9 +83,14 @@ class ClipCache:
     ``DecoderStack.forward(x, attention=...)``, with qkv [rows, (heads + 2 *
     kv_heads) * head_dim].  Lengths and pages are counted on the host and sent to
     the device on the current stream, which orders all of a cache's calls; no
-    call waits for the device.  With ``totals`` the softmax weight of every cached token is
-    accumulated by step() and verify(), which evict() needs.  `spare` tokens of
-    pages per clip are held free for evict()."""
+    call waits for the device.  With ``totals`` the softmax weight of every
+    cached token is accumulated by step() and verify(), which evict() needs.
+    `spare` tokens of pages per clip are held free for evict(), which moves the
+    clips that it cuts.
+
+    `position` (q [rows, heads, head_dim], k [rows, kv_heads, head_dim]) -> (q,
+    k) is called for each layer's new rows before they are cached; it keeps its
+    own count of positions, which after evict() are no longer the lengths."""
 
     def __init__(self, layers, clips, capacity, heads, kv_heads, head_dim=128, page_size=64, totals=False, spare=0,
                  position=None, device="cuda"):

@@ -226,8 +226,8 @@ def attention_prefill(q, k, v, cu_seqlens, cu_seqlens_k=None, scale=None):
     int32 [B + 1]: each sequence's first row, and the end.  With
     ``cu_seqlens_k`` the queries are the last ones of longer sequences of
     keys (a chunk behind its history): query i of Lq sees the keys j <= i +
-    Lk - Lq, and one that sees none gives zeros.  What a query does not see
-    has no effect on it.  ``scale`` defaults to dim ** -0.5."""
+    Lk - Lq, and one that sees none gives zeros, as do rows of no sequence.
+    What a query does not see has no effect on it.  ``scale`` defaults to dim ** -0.5."""
     return _ops.attention_prefill(q, k, v, cu_seqlens, cu_seqlens_k, q.shape[-1] ** -0.5 if scale is None else scale)
 
 
@@ -242,7 +242,8 @@ def kv8_append(k, v, cu_seqlens, starts, k_codes, v_codes, k_scale, v_scale, pag
 
 def kv8_gather(k_codes, v_codes, k_scale, v_scale, page_table, starts, cu_seqlens, rows, dtype=torch.bfloat16):
     """Token ranges of the cache as (k, v) [rows, kv_heads, dim] of ``dtype``:
-    output rows cu_seqlens[b] .. are sequence b's tokens starts[b], ... ."""
+    output rows cu_seqlens[b] .. are sequence b's tokens starts[b], ...; rows
+    of no sequence are zeros."""
     return _ops.kv8_gather(k_codes, v_codes, k_scale, v_scale, page_table, starts, cu_seqlens, rows, dtype)
 
 

@@ -267,7 +267,8 @@ int paro_silu_mul(const void* x, int64_t M, int I, void* out, paro_stream_t stre
  * out, 2 = tensor-memory allocation failed, 4 = a wait for the other CTAs of
  * the same launch timed out, 8 = a page-table entry outside the page pool, or
  * lengths that do not fit their page table or packed rows: the tokens
- * concerned were left out); synchronises with the device to read them.  clear != 0 resets the word.  Returns -1 if it cannot be read.
+ * concerned were left out); synchronises with the device to read them.
+ * clear != 0 resets the word.  Returns -1 if it cannot be read.
  *
  * Recovery: a kernel whose wait ran out stops where it was, so the outputs
  * of the calls made since the last clean read are invalid, and the
@@ -499,11 +500,12 @@ int paro_w4a8_gemm_noalloc(const int8_t* xq, const float* xscale, int64_t M, int
  *                      page page_table[b][t / page_size]; entries behind a
  *                      sequence's last token are not read
  * page_size 16, 32, 64 or 128; head_dim 64 or 128; int32 and float32 arrays
- * of these entry points are 4-byte aligned.  A page belongs to one
- * sequence while it is written.  A page-table entry outside the pool, or a
- * length beyond the table's row, sets bit 8 of the device error word, and
- * the tokens concerned are left out (nothing out of bounds is touched):
- * not written, read back as zeros, not attended to and given no weight.
+ * of these entry points are 4-byte aligned; a table's row holds at most
+ * 0x7FFF0000 tokens.  A page belongs to one sequence while it is written.  A
+ * page-table entry outside the pool, or a length beyond the table's row, sets
+ * bit 8 of the device error word, and the tokens concerned are left out
+ * (nothing out of bounds is touched): not written, read back and moved as
+ * zeros, not attended to and given no weight.
  */
 typedef struct paro_kv8_cache {
   int8_t* k_codes;
@@ -521,8 +523,8 @@ typedef struct paro_kv8_cache {
  *   o_i = sum_{j <= i + Lk - Lq} softmax_j(scale * q_i . k_j) v_j
  * for query i (of Lq) of each sequence over that sequence's Lk keys; a query
  * that sees no key gives zeros, and so do rows before the first sequence and
- * behind the last.
- * What a query does not see has no effect on it, whatever it holds.
+ * behind the last.  What a query does not see has no effect on it, whatever
+ * it holds; infinite scores that it sees make it NaN (+inf, or all -inf).
  *   q   : [rows][heads][head_dim] of dtype (F16 / BF16), strides in elements
  *   k, v: [k_rows][kv_heads][head_dim] of the same dtype
  *   strides[6]: q token, q head, k token, k head, v token, v head; multiples
@@ -531,7 +533,7 @@ typedef struct paro_kv8_cache {
  *               the end; the same pointer for whole prompts
  *   out : [rows][heads][head_dim] of dtype, contiguous
  * head_dim 64 or 128; heads a multiple of kv_heads; pointers 16-byte aligned;
- * scale finite and not negative.
+ * scale finite and not negative; rows and k_rows at most 0x7FFF0000.
  */
 int paro_attention_prefill(const void* q, const void* k, const void* v, int dtype, const int64_t* strides,
                            const int32_t* cu_q, const int32_t* cu_k, int B, int64_t rows, int64_t k_rows,
@@ -579,7 +581,7 @@ int paro_kv8_gather(const paro_kv8_cache* cache, const int32_t* page_table, int 
  * Attention of the newest T tokens of each sequence over the cache (their
  * own keys and values already appended): query i of sequence b sees the
  * tokens t <= lens[b] - T + i.  Sums and softmax statistics in float32; a
- * query that sees nothing gives zeros.
+ * query that sees nothing gives zeros, one whose seen scores are all -inf NaN.
  *   q   : [B][T][heads][head_dim] of dtype (F16 / BF16); strides[3]: batch,
  *         token, head in elements, multiples of 8
  *   lens: int32 [B] on the device
@@ -590,7 +592,9 @@ int paro_kv8_gather(const paro_kv8_cache* cache, const int32_t* page_table, int 
  *         same buffer; apart, a verify step whose draft is rejected can be
  *         dropped.
  *   workspace: paro_attention_kv8_workspace_size bytes, 256-byte aligned, of
- *         any content
+ *         any content; with weights it holds a float32 score for each query,
+ *         head and place of the page table (lengths are known on the device
+ *         only): 4 * B * T * heads * table_width * page_size bytes
  * T * heads / kv_heads at most 512.
  */
 size_t paro_attention_kv8_workspace_size(const paro_kv8_cache* cache, int table_width, int B, int T,
