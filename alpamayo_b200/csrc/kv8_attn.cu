@@ -25,8 +25,8 @@
 // running maximum M is of score + e_t, with 2^e_t the power of two below
 // vs_t, so the rounded value exp2(score + e_t - M + 14) * (vs_t / 2^e_t)
 // stays below 2^15 whatever the page scales are (e_t is kept within -60 and
-// 120: a page of smaller values loses bits, and no finite input has a larger
-// scale than 2^121).  The denominator keeps the unrounded float32 terms, but
+// 121: a page of smaller values loses bits, and no finite input has a scale of
+// 2^122).  The denominator keeps the unrounded float32 terms, but
 // for those of pages whose scale (2^-60 for a page of zeros) is below 2^-126
 // of the largest.
 //
@@ -497,11 +497,11 @@ __global__ void __launch_bounds__(kDecWarps * 32, (DecodeTile<D, RB>::kCtas)) kv
           }
         }
       }
-      // page scales: 2^e <= |vs| < 2^(e + 1), e kept within -60 and 120
+      // page scales: 2^e <= |vs| < 2^(e + 1), e kept within -60 and 121
       float ve[2], vf[2], vi[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int e = max(-60, min(120, (int)((__float_as_uint(vs[i]) >> 23) & 0xff) - 127));
+        const int e = max(-60, min(121, (int)((__float_as_uint(vs[i]) >> 23) & 0xff) - 127));
         ve[i] = (float)e + sc[4 + i];                         // - infinity: left out
         vi[i] = __uint_as_float((uint32_t)(127 - e) << 23);   // 2^-e
         vf[i] = vs[i] * vi[i];
